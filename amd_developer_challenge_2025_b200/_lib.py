@@ -1,5 +1,5 @@
-"""ctypes binding of lib/libb200fp8mm.so (declarations: include/b200_fp8_mm.h, include/b200_mla_consumers.h), and the
-native module that makes the same calls for plain CUDA tensors without ctypes (csrc/host_calls.cpp).
+"""ctypes binding of lib/libb200fp8mm.so (declarations: include/b200_fp8_mm.h, include/b200_mla_consumers.h,
+include/b200_mla_cache.h), and the native module that makes the same calls for plain CUDA tensors without ctypes (csrc/host_calls.cpp).
 
 Loading the library fails loudly: there is no fallback implementation of the operator. The native module only checks and
 passes on arguments; without it the same is done in Python."""
@@ -16,7 +16,7 @@ LIB_PATH = os.environ.get("B200_FP8_MM_LIB") or os.path.join(HERE, "lib", "libb2
 
 ABI_VERSION = 7
 
-# Every symbol the two headers declare.
+# Every symbol the headers declare.
 EXPORTS = (
     "b200_fp8_mm",
     "b200_fp8_mm_planned",
@@ -36,6 +36,12 @@ EXPORTS = (
     # include/b200_mla_consumers.h
     "b200_mla_rope",
     "b200_mla_div_softmax",
+    # include/b200_mla_cache.h
+    "b200_mla_cache_append",
+    "b200_mla_cache_attend",
+    "b200_mla_cache_attend_workspace_bytes",
+    "b200_mla_cache_evict",
+    "b200_mla_cache_evict_workspace_bytes",
 )
 
 
@@ -51,6 +57,24 @@ class CPlan(ctypes.Structure):
         ("smem_bytes", ctypes.c_int),
         ("store_bufs", ctypes.c_int),
         ("full_tiles", ctypes.c_int),
+    ]
+
+
+class CMlaCache(ctypes.Structure):
+    _fields_ = [
+        ("data", ctypes.c_void_p),
+        ("block_table", ctypes.c_void_p),
+        ("lens", ctypes.c_void_p),
+        ("dtype", ctypes.c_int),
+        ("pages", ctypes.c_int),
+        ("page_size", ctypes.c_int),
+        ("dv", ctypes.c_int),
+        ("dr", ctypes.c_int),
+        ("batch", ctypes.c_int),
+        ("pages_per_seq", ctypes.c_int),
+        ("page_stride", ctypes.c_longlong),
+        ("slot_stride", ctypes.c_longlong),
+        ("table_stride", ctypes.c_longlong),
     ]
 
 
@@ -154,6 +178,18 @@ def load() -> ctypes.CDLL:
     lib.b200_mla_rope.restype = ctypes.c_int
     lib.b200_mla_div_softmax.argtypes = [ctypes.c_void_p] + [ctypes.c_int] * 5 + [ctypes.c_void_p]
     lib.b200_mla_div_softmax.restype = ctypes.c_int
+    p, i, n = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong
+    lib.b200_mla_cache_append.argtypes = [ctypes.POINTER(CMlaCache), p, n, p, ctypes.c_double, p, n, n, p, n, n, i, p, n, p, n, p]
+    lib.b200_mla_cache_append.restype = i
+    lib.b200_mla_cache_attend.argtypes = [ctypes.POINTER(CMlaCache), p, n, n, i, ctypes.c_float, p, n, n, p, p, n, p, n, i, p,
+                                          ctypes.c_size_t, p, p]
+    lib.b200_mla_cache_attend.restype = i
+    lib.b200_mla_cache_attend_workspace_bytes.argtypes = [i] * 6
+    lib.b200_mla_cache_attend_workspace_bytes.restype = ctypes.c_size_t
+    lib.b200_mla_cache_evict.argtypes = [ctypes.POINTER(CMlaCache), p, n, p, n, i, i, p, p, n, p, n, p, ctypes.c_size_t, p]
+    lib.b200_mla_cache_evict.restype = i
+    lib.b200_mla_cache_evict_workspace_bytes.argtypes = [i] * 3
+    lib.b200_mla_cache_evict_workspace_bytes.restype = ctypes.c_size_t
     lib.b200_fp8_mm_abi_version.argtypes = []
     lib.b200_fp8_mm_abi_version.restype = ctypes.c_int
     if lib.b200_fp8_mm_abi_version() != ABI_VERSION:
