@@ -1,5 +1,6 @@
 // Operators around a paged latent cache for B200 (sm_100a): append, attend, evict (include/b200_mla_cache.h).
 
+#include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -7,8 +8,12 @@
 #include <math.h>
 #include <stdint.h>
 
+#include <atomic>
+#include <type_traits>
+
 #include "b200_fp8_mm.h"
 #include "b200_mla_cache.h"
+#include "cache_walk.h"
 
 namespace {
 
@@ -145,102 +150,828 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_con
 
 constexpr float kLn2 = 0.69314718055994531f, kLog2E = 1.4426950408889634f;
 constexpr int kMaxD = 576;
-constexpr int kAttendThreads = 256;
-constexpr int kAttendWarps = kAttendThreads / 32;
-constexpr int kLaneD = kMaxD / 32;
-constexpr int kLaneV = 512 / 32;
+constexpr int kTile = cache_walk::kTileRows;   // rows of the cache per tile
+constexpr int kRowBytes = 128;                 // of a row that one swizzled chunk holds: 64 elements
+constexpr int kChunkBytes = kTile * kRowBytes; // 64 rows x 64 elements
+constexpr int kUnitBytes = 2 * kChunkBytes;    // 128 elements of the value: the rows of one second product
+constexpr int kMaxV = 16, kMaxR = 8;           // ring slots
+constexpr int kSoftmaxThreads = 128;
+constexpr int kAttendThreads = kSoftmaxThreads + 64;
+constexpr int kHeaderBytes = 2048;             // barriers and small arrays, behind the rings
+constexpr int kMaxSmem = 232448;               // 227 KiB opt-in limit per CTA on sm_100
+constexpr int kTmemCols = 512;
+constexpr int kTmemLogits = 256;               // two buffers of 64 columns behind the accumulators
+constexpr unsigned long long kWaitLimitNs = 2000000000ull;
+constexpr float kRescaleAbove = 8.f;  // log2: a running maximum is replaced when it is exceeded by this much
 
 struct AttendParams {
   CacheView cache;
-  const void* q;
   void* out;
-  float* lse;  // [batch][heads]
+  float* lse;              // [batch][heads] or null
   const float* score;
   float* score_out;
-  long long q_sb, q_sh, out_sb, out_sh, score_stride, score_out_stride;
-  int heads, max_len;
-  float scale_log2;  // scale * log2(e)
+  long long out_sb, out_sh, score_stride, score_out_stride;
+  int heads, head_tiles, max_len, batch;
+  int workers, least;      // workers per head tile, and the least tiles worth one
+  int copy_rows;           // cache_walk::copy_rows(page_size)
+  int v_slots, r_slots;    // ring slots of a unit each: value units, units of the elements behind the value
+  int v_units, r_chunks;   // units of a tile; chunks behind the value
+  float scale_log2;        // scale * log2(e)
+  // Workspace
+  long long* first_tile;   // [batch + 1]: tiles before each sequence, and all
+  float* lse2;             // [batch][heads]: log2 of the sum of 2^x
+  float2* part_stat;       // [worker][head tile][2][heads of a tile]: maximum and sum
+  float* part_out;         // the same, times dv
+  float* logits;           // [batch][tile][heads][64] in log2, or null
+  int logit_tiles;
+  int* status;             // may be null
 };
 
-// scale * log2(e) * (q . row of slot j), the same value in every lane
-template <typename T>
-__device__ __forceinline__ float logit(const CacheView& c, const float (&q)[kLaneD], int b, int j, int lane, float scale_log2,
-                                       float (&x)[kLaneD]) {
-  const long long at = slot_offset(c, b, j);
-  const T* row = static_cast<const T*>(c.data) + at;
-  float s = 0.f;
-#pragma unroll
-  for (int i = 0; i < kLaneD; ++i) {
-    const int e = lane + 32 * i;
-    x[i] = (at >= 0 && e < c.d) ? to_float(row[e]) : 0.f;
-    s += q[i] * x[i];
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-  return s * scale_log2;
+__device__ __forceinline__ uint32_t smem_u32(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
+
+__device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
+}
+__device__ __forceinline__ void mbar_expect_tx(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+// One probe; the hint (nanoseconds) lets the hardware park the thread until the phase completes.
+__device__ __forceinline__ uint32_t mbar_try_wait(uint32_t bar, uint32_t parity, uint32_t hint) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity), "r"(hint)
+      : "memory");
+  return ok;
+}
+__device__ __forceinline__ uint32_t mbar_test(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok;
+}
+__device__ __forceinline__ unsigned long long global_ns() {
+  unsigned long long t;
+  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+  return t;
 }
 
-// One CTA per (head, sequence): the warps share the rows, each with its own running maximum, sum and weighted sum.
-template <typename T>
-__global__ void __launch_bounds__(kAttendThreads) attend_kernel(const __grid_constant__ AttendParams p) {
-  __shared__ float part[kAttendWarps][512];
-  __shared__ float2 stat[kAttendWarps];
+// Every wait is bounded: the first that expires raises the CTA's flag and reports itself, all others see the flag.
+struct Waits {
+  volatile int* expired;  // shared memory
+  int* status;            // global, may be null
+
+  __device__ bool give_up(unsigned long long t0, uint32_t parity, int where) const {
+    if (*expired) return true;
+    if (global_ns() - t0 <= kWaitLimitNs) return false;
+    *expired = 1;
+    if (status != nullptr && atomicCAS(status, 0, B200_FP8_MM_DEV_WAIT_EXPIRED) == 0) {
+      status[1] = where;
+      status[2] = static_cast<int>(blockIdx.x);
+      status[3] = static_cast<int>(parity);
+    }
+    return true;
+  }
+  __device__ __noinline__ bool slow(uint32_t bar, uint32_t parity, int where) const {
+    const unsigned long long t0 = global_ns();
+    while (!mbar_try_wait(bar, parity, 200000)) {
+      if (give_up(t0, parity, where)) return false;
+    }
+    return true;
+  }
+  __device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, int where) const {
+    return mbar_try_wait(bar, parity, 200000) || slow(bar, parity, where);
+  }
+};
+
+enum Where { kAtQFull = 0x201, kAtVFull, kAtRFull, kAtVEmpty, kAtREmpty, kAtQEmpty, kAtSFull, kAtSFree, kAtPFull, kAtPvDone, kAtOFree };
+
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+      "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(bar)
+      : "memory");
+}
+
+__device__ __forceinline__ void tcgen05_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tcgen05_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+
+// Matrix descriptors as 32-bit halves, as in the GEMM: low word address and leading offset, high word stride offset, version
+// and the 128-byte swizzle. Only the address changes between instructions.
+__device__ __forceinline__ void umma_f16(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t hi, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
+      "mov.b64 da, {%1, %3};\n\t"
+      "mov.b64 db, {%2, %3};\n\t"
+      "setp.ne.b32 p, %5, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %4, p;\n\t}" ::"r"(d),
+      "r"(a_lo), "r"(b_lo), "r"(hi), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void umma_commit(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+
+// 16 lanes x 64 columns: thread t gets columns 8 i + 2 (t % 4) + {0, 1} of lane t / 4 in v[4 i + {0, 1}], of lane t / 4 + 8 in
+// v[4 i + {2, 3}].
+__device__ __forceinline__ void tmem_ld_16x64(uint32_t taddr, uint32_t (&v)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x8.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
+        "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]),
+        "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]),
+        "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+      : "r"(taddr)
+      : "memory");
+}
+// 32 lanes x 16 columns: thread t gets lane t.
+__device__ __forceinline__ void tmem_ld_32x16(uint32_t taddr, uint32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
+        "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_32x16(uint32_t taddr, const uint32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]),
+      "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+      : "memory");
+}
+
+// 2^x, the hardware's (relative error about 2^-22; 0 below 2^-126).
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ uint32_t pack2(float lo, float hi, __nv_bfloat16) {
+  uint32_t r;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ uint32_t pack2(float lo, float hi, __half) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+__device__ __forceinline__ void softmax_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kSoftmaxThreads) : "memory"); }
+__device__ __forceinline__ bool softmax_any(bool mine) {
+  uint32_t any;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.or.pred q, 1, %2, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(any)
+      : "r"(static_cast<uint32_t>(mine)), "n"(kSoftmaxThreads)
+      : "memory");
+  return any != 0;
+}
+
+// What the roles of a CTA share, at the end of its shared memory.
+struct alignas(8) AttendShared {
+  uint64_t v_full[kMaxV], v_empty[kMaxV], r_full[kMaxR], r_empty[kMaxR];
+  uint64_t q_full, q_empty, s_full[2], s_free[2], p_full, pv_done, o_free, drained;
+  float factor[64];   // by which a head's accumulators are multiplied when its maximum is replaced
+  float inverse[64];  // 1 / sum of weights
+  float2 stat[64];
+  long long sums[kAttendThreads / 32];
+  long long share, share_end;
+  uint32_t tmem_base;
+  int expired, first_seq, first_tile;
+};
+static_assert(sizeof(AttendShared) <= kHeaderBytes, "the header is too small");
+
+// A worker's walk over its share: segment after segment, each a run of tiles of one sequence.
+struct Walk {
+  int b, t;        // sequence, first tile of the segment
+  int rows, count; // rows of the sequence, tiles of the segment
+  long long left;
+
+  __device__ __forceinline__ Walk(const AttendShared& sh) : b(sh.first_seq), t(sh.first_tile), rows(0), count(0), left(sh.share_end - sh.share) {}
+  __device__ __forceinline__ bool next(const AttendParams& p) {
+    t += count;
+    count = 0;
+    while (left > 0) {
+      rows = rows_of(p.cache, b, p.max_len);
+      const int tiles = cache_walk::tiles_of(rows);
+      if (t < tiles) {
+        count = static_cast<int>(min(static_cast<long long>(tiles - t), left));
+        left -= count;
+        return true;
+      }
+      ++b;
+      t = 0;
+    }
+    return false;
+  }
+  __device__ __forceinline__ bool whole() const { return t == 0 && count == cache_walk::tiles_of(rows); }
+};
+
+// Flash attention of one token per sequence over a latent cache: heads x rows x (d + dv) products per row of d elements read.
+//
+//   S = Q K^T        [64 heads x 64 rows]   M = heads (64), K = d:     Q and the rows as they lie (K-major)
+//   O^T += V^T P^T   [128 x heads] x dv/128 M = value elements, K = rows: the same rows read as an MN-major operand, so that
+//                                            a tile is fetched once for both products and never transposed
+// With the value's elements in the lanes, the accumulators of 64 heads take 256 of the 512 TMEM columns; with the heads in the
+// lanes, 128 heads would take them all and leave none for S. Fewer heads shrink N (16 or 32) and what Q takes of shared memory.
+//
+// One CTA per SM and worker: warp 4 copies (TMA, 128-byte swizzle; Q once per segment, rows in units of 128 value elements that
+// are freed one by one), warp 5 issues the products, warps 0 to 3 do the softmax (S comes as the 16 x 256-bit fragments: 4 threads
+// to a head) and the epilogue. S is double buffered; the next tile's first product runs under this tile's softmax. The running
+// maximum is replaced only when a logit exceeds it by 2^8: the weights stay below 2^8, which no type here minds, and rescaling the
+// accumulators is rare. Sums are kept in fp32, weights are rounded to the cache's type for the second product, as matrix operands
+// have to be.
+template <typename T, int HT>
+__global__ void __launch_bounds__(kAttendThreads, 1)
+attend_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap row_map, const __grid_constant__ AttendParams p) {
+  extern __shared__ __align__(1024) uint8_t smem[];
+  const CacheView& c = p.cache;
+  const int chunks = 2 * p.v_units + p.r_chunks;
+  uint8_t* const q_smem = smem;
+  uint8_t* const v_ring = q_smem + chunks * HT * kRowBytes;
+  uint8_t* const r_ring = v_ring + p.v_slots * kUnitBytes;
+  uint8_t* const p_smem = r_ring + p.r_slots * p.r_chunks * kChunkBytes;
+  AttendShared& sh = *reinterpret_cast<AttendShared*>(p_smem + HT * kRowBytes);
+  const int tid = static_cast<int>(threadIdx.x), warp = tid >> 5, lane = tid & 31;
+  const int head_tile = static_cast<int>(blockIdx.x) % p.head_tiles, worker = static_cast<int>(blockIdx.x) / p.head_tiles;
+  const int head0 = head_tile * HT;
+  const Waits waits{&sh.expired, p.status};
+  if (tid == 0) {
+    for (int i = 0; i < kMaxV; ++i) {
+      mbar_init(smem_u32(&sh.v_full[i]), 1);
+      mbar_init(smem_u32(&sh.v_empty[i]), 1);
+    }
+    for (int i = 0; i < kMaxR; ++i) {
+      mbar_init(smem_u32(&sh.r_full[i]), 1);
+      mbar_init(smem_u32(&sh.r_empty[i]), 1);
+    }
+    mbar_init(smem_u32(&sh.q_full), 1);
+    mbar_init(smem_u32(&sh.q_empty), 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(smem_u32(&sh.s_full[i]), 1);
+      mbar_init(smem_u32(&sh.s_free[i]), 4);
+    }
+    mbar_init(smem_u32(&sh.p_full), 4);
+    mbar_init(smem_u32(&sh.pv_done), 1);
+    mbar_init(smem_u32(&sh.o_free), 4);
+    mbar_init(smem_u32(&sh.drained), 1);
+    sh.expired = (smem_u32(smem) & 1023u) != 0;  // the swizzle needs it; never so with no static shared memory before it
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&q_map) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&row_map) : "memory");
+  }
+  if (warp == 5) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem_base)), "r"(kTmemCols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
   pdl_wait();
   pdl_launch_dependents();
-  const CacheView& c = p.cache;
-  const int h = static_cast<int>(blockIdx.x), b = static_cast<int>(blockIdx.y);
-  const int warp = static_cast<int>(threadIdx.x) >> 5, lane = static_cast<int>(threadIdx.x) & 31;
-  const int n = rows_of(c, b, p.max_len);
-  const T* qrow = static_cast<const T*>(p.q) + b * p.q_sb + h * p.q_sh;
-  float q[kLaneD], x[kLaneD], acc[kLaneV] = {};
+  // Tiles before each thread's run of sequences, and where this worker's share begins.
+  const int run = (p.batch + kAttendThreads - 1) / kAttendThreads;
+  const int b0 = min(p.batch, tid * run), b1 = min(p.batch, b0 + run);
+  long long mine = 0;
+  for (int b = b0; b < b1; ++b) mine += cache_walk::tiles_of(rows_of(c, b, p.max_len));
+  long long upto = mine;
 #pragma unroll
-  for (int i = 0; i < kLaneD; ++i) q[i] = lane + 32 * i < c.d ? to_float(qrow[lane + 32 * i]) : 0.f;
-  float m = -INFINITY, l = 0.f;
-  for (int j = warp; j < n; j += kAttendWarps) {
-    const float s = logit<T>(c, q, b, j, lane, p.scale_log2, x);
-    const float top = fmaxf(m, s);
-    const float base = top == -INFINITY ? 0.f : top;
-    const float keep = exp2f(m - base), w = exp2f(s - base);
-    l = l * keep + w;
-#pragma unroll
-    for (int i = 0; i < kLaneV; ++i) acc[i] = acc[i] * keep + w * x[i];
-    m = top;
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long v = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += v;
   }
-#pragma unroll
-  for (int i = 0; i < kLaneV; ++i) part[warp][lane + 32 * i] = acc[i];
-  if (lane == 0) stat[warp] = make_float2(m, l);
+  if (lane == 31) sh.sums[warp] = upto;
+  tcgen05_fence_before();
   __syncthreads();
-  float top = -INFINITY, sum = 0.f;
-  for (int w = 0; w < kAttendWarps; ++w) top = fmaxf(top, stat[w].x);
-  const float base = top == -INFINITY ? 0.f : top;
-  for (int w = 0; w < kAttendWarps; ++w) sum += stat[w].y * exp2f(stat[w].x - base);
-  T* out = static_cast<T*>(p.out) + b * p.out_sb + h * p.out_sh;
-  for (int e = static_cast<int>(threadIdx.x); e < c.dv; e += kAttendThreads) {
-    float v = 0.f;
-    for (int w = 0; w < kAttendWarps; ++w) v += part[w][e] * exp2f(stat[w].x - base);
-    from_float(n == 0 ? 0.f : v / sum, &out[e]);
+  tcgen05_fence_after();
+  const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(&sh.tmem_base);
+  {
+    long long before = upto - mine, tiles = 0;
+    for (int w = 0; w < kAttendThreads / 32; ++w) {
+      if (w < warp) before += sh.sums[w];
+      tiles += sh.sums[w];
+    }
+    const int workers = cache_walk::workers_of(tiles, p.workers, p.least);
+    const long long begin = worker < workers ? cache_walk::share_begin(tiles, workers, worker) : 0;
+    const long long end = worker < workers ? cache_walk::share_begin(tiles, workers, worker + 1) : 0;
+    if (tid == 0) {
+      sh.share = begin;
+      sh.share_end = end;
+    }
+    if (begin < end && before <= begin && begin < before + mine) {
+      long long at = begin - before;
+      int b = b0;
+      for (;; ++b) {
+        const int n = cache_walk::tiles_of(rows_of(c, b, p.max_len));
+        if (at < n) break;
+        at -= n;
+      }
+      sh.first_seq = b;
+      sh.first_tile = static_cast<int>(at);
+    }
+    if (blockIdx.x == 0) {
+      for (int b = b0; b < b1; ++b) {
+        p.first_tile[b] = before;
+        before += cache_walk::tiles_of(rows_of(c, b, p.max_len));
+      }
+      if (tid == 0) p.first_tile[p.batch] = tiles;
+    }
   }
-  if (threadIdx.x == 0) p.lse[static_cast<long long>(b) * p.heads + h] = n == 0 ? -INFINITY : (base + log2f(sum)) * kLn2;
+  __syncthreads();
+
+  if (warp == 4) {
+    // Copies. A lane takes the pieces (copy_rows rows of one page) lane, lane + 32 of a tile.
+    const int pieces = kTile / p.copy_rows, r_bytes = p.r_chunks * kChunkBytes;
+    int v = 0, r = 0, segment = 0;
+    uint32_t v_phase = 0, r_phase = 0;
+    bool ok = sh.expired == 0;
+    auto all_wait = [&](uint64_t* bar, uint32_t parity, int where) {
+      return __all_sync(0xffffffffu, waits.wait(smem_u32(bar), parity, where)) != 0;
+    };
+    Walk walk(sh);
+    while (ok && walk.next(p)) {
+      const int* table = c.block_table + walk.b * c.table_stride;
+      // (page, slot) of this lane's pieces of a tile; rows behind the sequence come from a page behind the last, as zeros
+      auto place = [&](int tile, int k, int* page, int* slot) {
+        const int row = tile * kTile + (lane + 32 * k) * p.copy_rows;
+        *page = c.pages;
+        *slot = 0;
+        if (lane + 32 * k < pieces && tile < walk.t + walk.count && row < walk.rows) {
+          const int at = row / c.page_size;
+          *slot = row - at * c.page_size;
+          const int id = table[at];
+          *page = id < 0 || id > c.pages ? c.pages : id;
+        }
+      };
+      int page[2], slot[2];
+      for (int k = 0; k < 2; ++k) place(walk.t, k, &page[k], &slot[k]);
+      for (int tile = walk.t; ok && tile < walk.t + walk.count; ++tile) {
+        int next_page[2], next_slot[2];
+        for (int k = 0; k < 2; ++k) place(tile + 1, k, &next_page[k], &next_slot[k]);  // on their way during this tile's waits
+        auto copy = [&](uint8_t* dst, int chunk0, int n, uint64_t* full) {
+          if (lane == 0) mbar_expect_tx(smem_u32(full), n * kChunkBytes);
+          __syncwarp();
+          for (int k = 0; k < 2; ++k) {
+            const int piece = lane + 32 * k;
+            if (piece >= pieces) break;
+            for (int i = 0; i < n; ++i)
+              tma_load_3d(smem_u32(dst) + i * kChunkBytes + piece * p.copy_rows * kRowBytes, &row_map, (chunk0 + i) * 64, slot[k], page[k],
+                          smem_u32(full));
+          }
+        };
+        if (p.r_chunks > 0) {
+          if (!(ok = all_wait(&sh.r_empty[r], r_phase ^ 1, kAtREmpty))) break;
+          copy(r_ring + r * r_bytes, 2 * p.v_units, p.r_chunks, &sh.r_full[r]);
+          if (++r == p.r_slots) r = 0, r_phase ^= 1;
+        }
+        for (int u = 0; u < p.v_units; ++u) {
+          if (!(ok = all_wait(&sh.v_empty[v], v_phase ^ 1, kAtVEmpty))) break;
+          copy(v_ring + v * kUnitBytes, 2 * u, 2, &sh.v_full[v]);
+          if (++v == p.v_slots) v = 0, v_phase ^= 1;
+        }
+        if (ok && tile == walk.t) {
+          // The queries of this segment, once the first products of the segment before are over.
+          if (segment > 0 && !(ok = all_wait(&sh.q_empty, (segment - 1) & 1, kAtQEmpty))) break;
+          if (lane == 0) {
+            mbar_expect_tx(smem_u32(&sh.q_full), chunks * HT * kRowBytes);
+            for (int i = 0; i < chunks; ++i)
+              tma_load_3d(smem_u32(q_smem) + i * HT * kRowBytes, &q_map, i * 64, head0, walk.b, smem_u32(&sh.q_full));
+          }
+        }
+        for (int k = 0; k < 2; ++k) page[k] = next_page[k], slot[k] = next_slot[k];
+      }
+      ++segment;
+    }
+    if (sh.expired != 0 && lane == 0) {
+      // A wait has expired somewhere: no copy may still be in flight when the CTA ends. A slot's last copies belong to the phase
+      // that its barrier completed last or is in; waiting for the other parity returns at once where none are in flight.
+      auto drain = [&](uint64_t* bar, uint32_t parity) {
+        for (int i = 0; i < 1000 && !mbar_try_wait(smem_u32(bar), parity, 10000); ++i) {
+        }
+      };
+      for (int i = 0; i < p.v_slots; ++i) drain(&sh.v_full[i], i < v ? v_phase : v_phase ^ 1);
+      for (int i = 0; i < p.r_slots; ++i) drain(&sh.r_full[i], i < r ? r_phase : r_phase ^ 1);
+      for (uint32_t parity = 0; parity < 2; ++parity) drain(&sh.q_full, parity);
+    }
+    __syncwarp();
+  } else if (warp == 5) {
+    if (lane == 0) {
+      constexpr uint32_t kType = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+      constexpr uint32_t kIdesc = (1u << 4) | (kType << 7) | (kType << 10);
+      constexpr uint32_t kIdescS = kIdesc | (static_cast<uint32_t>(kTile >> 3) << 17) | (64u >> 4 << 24);
+      constexpr uint32_t kIdescO = kIdesc | (1u << 15) | (static_cast<uint32_t>(HT >> 3) << 17) | (128u >> 4 << 24);  // A is MN-major
+      constexpr uint32_t kHi = (1024u >> 4) | (1u << 14) | (2u << 29);
+      constexpr uint32_t kLoK = 1u << 16;                                             // K-major: no leading offset
+      constexpr uint32_t kLoV = static_cast<uint32_t>(kChunkBytes >> 4) << 16;        // MN-major: to the next 64 elements
+      const uint32_t q_lo = kLoK | (smem_u32(q_smem) >> 4), p_lo = kLoK | (smem_u32(p_smem) >> 4);
+      const uint32_t v_base = smem_u32(v_ring) >> 4, r_base = smem_u32(r_ring) >> 4;
+      int v = 0, r = 0, i = 0, segment = 0;
+      uint32_t v_phase = 0, r_phase = 0;
+      bool ok = sh.expired == 0;
+      // The second product that is still to be issued: of tile i - 1, whose value units begin at slot pv.
+      bool pending = false, pending_first = false;
+      int pv = 0, pv_segment = 0, pv_tile = 0;
+      auto second = [&]() {
+        pending = false;
+        if (pending_first && pv_segment > 0 && !(ok = waits.wait(smem_u32(&sh.o_free), (pv_segment - 1) & 1, kAtOFree))) return;
+        tcgen05_fence_after();
+        for (int u = 0; u < p.v_units; ++u) {
+          const uint32_t a = kLoV | (v_base + pv * (kUnitBytes >> 4));
+#pragma unroll
+          for (int k = 0; k < kTile / 16; ++k)
+            umma_f16(tmem + u * HT, a + k * (16 * kRowBytes >> 4), p_lo + k * 2, kHi, kIdescO, !(pending_first && k == 0));
+          umma_commit(smem_u32(&sh.v_empty[pv]));
+          if (++pv == p.v_slots) pv = 0;
+        }
+        umma_commit(smem_u32(&sh.pv_done));
+      };
+      // Waits for `bar`; while it is not there, the second product goes out as soon as its weights are.
+      auto wait_or_second = [&](uint64_t* bar, uint32_t parity, int where) {
+        if (!pending) return waits.wait(smem_u32(bar), parity, where);
+        const unsigned long long t0 = global_ns();
+        for (uint32_t spins = 0; !mbar_test(smem_u32(bar), parity); ++spins) {
+          if (mbar_test(smem_u32(&sh.p_full), pv_tile & 1)) {
+            second();
+            return ok && waits.wait(smem_u32(bar), parity, where);
+          }
+          if ((spins & 63u) == 63u && waits.give_up(t0, parity, where)) return false;
+        }
+        return true;
+      };
+      Walk walk(sh);
+      while (ok && walk.next(p)) {
+        for (int tile = 0; ok && tile < walk.count; ++tile, ++i) {
+          const uint32_t s = tmem + kTmemLogits + (i & 1) * kTile;
+          if (!(ok = waits.wait(smem_u32(&sh.s_free[i & 1]), ((i >> 1) & 1) ^ 1, kAtSFree))) break;
+          if (tile == 0 && !(ok = wait_or_second(&sh.q_full, segment & 1, kAtQFull))) break;
+          uint32_t accumulate = 0;
+          auto first = [&](uint32_t rows, int chunk) {
+            const uint32_t a = q_lo + chunk * (HT * kRowBytes >> 4);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              umma_f16(s, a + k * 2, (kLoK | rows) + k * 2, kHi, kIdescS, accumulate);
+              accumulate = 1;
+            }
+          };
+          if (p.r_chunks > 0) {
+            if (!(ok = wait_or_second(&sh.r_full[r], r_phase, kAtRFull))) break;
+            tcgen05_fence_after();
+            for (int n = 0; n < p.r_chunks; ++n) first(r_base + (r * p.r_chunks + n) * (kChunkBytes >> 4), 2 * p.v_units + n);
+            umma_commit(smem_u32(&sh.r_empty[r]));
+            if (++r == p.r_slots) r = 0, r_phase ^= 1;
+          }
+          const int v0 = v;
+          for (int u = 0; u < p.v_units; ++u) {
+            if (!(ok = wait_or_second(&sh.v_full[v], v_phase, kAtVFull))) break;
+            tcgen05_fence_after();
+            for (int n = 0; n < 2; ++n) first(v_base + v * (kUnitBytes >> 4) + n * (kChunkBytes >> 4), 2 * u + n);
+            if (++v == p.v_slots) v = 0, v_phase ^= 1;
+          }
+          if (!ok) break;
+          umma_commit(smem_u32(&sh.s_full[i & 1]));
+          if (tile == walk.count - 1) umma_commit(smem_u32(&sh.q_empty));
+          if (pending) {
+            if (!(ok = waits.wait(smem_u32(&sh.p_full), pv_tile & 1, kAtPFull))) break;
+            second();
+            if (!ok) break;
+          }
+          pending = true;
+          pending_first = tile == 0;
+          pv = v0;
+          pv_segment = segment;
+          pv_tile = i;
+        }
+        ++segment;
+      }
+      if (ok && pending && waits.wait(smem_u32(&sh.p_full), pv_tile & 1, kAtPFull)) second();
+      if (sh.expired != 0) {  // none in flight past here
+        umma_commit(smem_u32(&sh.drained));
+        for (int n = 0; n < 1000 && !mbar_try_wait(smem_u32(&sh.drained), 0, 10000); ++n) {
+        }
+      }
+    }
+    __syncwarp();
+  } else {
+    // Softmax: warp w has heads 16 w .. 16 w + 15 of the tile, thread t rows (heads) t / 4 and t / 4 + 8 of these.
+    const bool active = 16 * warp < HT;
+    const int row0 = 16 * warp + lane / 4, row1 = row0 + 8;
+    const uint32_t lanes = static_cast<uint32_t>(32 * warp) << 16;
+    int i = 0, v = 0;
+    bool ok = sh.expired == 0;
+    // A wait that has expired does not end this role, because the other warps meet it at the barriers below: the rest of the walk
+    // goes by without waiting, over whatever is there.
+    auto wait = [&](uint64_t* bar, uint32_t parity, int where) {
+      if (ok) ok = waits.wait(smem_u32(bar), parity, where);
+    };
+    Walk walk(sh);
+    bool first_segment = true;
+    while (walk.next(p)) {
+      float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
+      for (int tile = 0; tile < walk.count; ++tile, ++i) {
+        wait(&sh.s_full[i & 1], (i >> 1) & 1, kAtSFull);
+        tcgen05_fence_after();
+        uint32_t x[32];
+        if (active) tmem_ld_16x64(tmem + lanes + kTmemLogits + (i & 1) * kTile, x);
+        tcgen05_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&sh.s_free[i & 1]));
+        const int left = walk.rows - (walk.t + tile) * kTile;  // rows that exist from this tile on
+        float t0 = -INFINITY, t1 = -INFINITY;
+        if (active) {
+#pragma unroll
+          for (int n = 0; n < 32; ++n) {
+            const int col = 8 * (n / 4) + 2 * (lane % 4) + (n & 1);
+            const float xs = col < left ? __uint_as_float(x[n]) * p.scale_log2 : -INFINITY;
+            x[n] = __float_as_uint(xs);
+            if (n & 2) t1 = fmaxf(t1, xs); else t0 = fmaxf(t0, xs);
+          }
+          if (p.logits != nullptr) {
+            float* to = p.logits + ((static_cast<long long>(walk.b) * p.logit_tiles + walk.t + tile) * p.heads + head0) * kTile + 2 * (lane % 4);
+#pragma unroll
+            for (int n = 0; n < 8; ++n) {
+              if (row0 < HT && head0 + row0 < p.heads)
+                *reinterpret_cast<uint2*>(to + row0 * kTile + 8 * n) = make_uint2(x[4 * n], x[4 * n + 1]);
+              if (row1 < HT && head0 + row1 < p.heads)
+                *reinterpret_cast<uint2*>(to + row1 * kTile + 8 * n) = make_uint2(x[4 * n + 2], x[4 * n + 3]);
+            }
+          }
+#pragma unroll
+          for (int o = 1; o < 4; o <<= 1) {
+            t0 = fmaxf(t0, __shfl_xor_sync(0xffffffffu, t0, o));
+            t1 = fmaxf(t1, __shfl_xor_sync(0xffffffffu, t1, o));
+          }
+        }
+        bool rescale = false;
+        __syncwarp();
+        if (tile == 0) {
+          m0 = t0;
+          m1 = t1;
+        } else {
+          const bool up0 = active && t0 > m0 + kRescaleAbove, up1 = active && t1 > m1 + kRescaleAbove;
+          rescale = softmax_any(up0 || up1);
+          if (rescale && active) {
+            const float f0 = up0 ? exp2_fast(m0 - t0) : 1.f, f1 = up1 ? exp2_fast(m1 - t1) : 1.f;
+            if (up0) m0 = t0;
+            if (up1) m1 = t1;
+            l0 *= f0;
+            l1 *= f1;
+            if (lane % 4 == 0) {
+              sh.factor[row0] = f0;
+              sh.factor[row1] = f1;
+            }
+          }
+        }
+        const float z0 = m0 == -INFINITY ? 0.f : m0, z1 = m1 == -INFINITY ? 0.f : m1;
+        if (active) {
+#pragma unroll
+          for (int n = 0; n < 8; ++n) {
+            const float a = exp2_fast(__uint_as_float(x[4 * n]) - z0), b = exp2_fast(__uint_as_float(x[4 * n + 1]) - z0);
+            const float e = exp2_fast(__uint_as_float(x[4 * n + 2]) - z1), f = exp2_fast(__uint_as_float(x[4 * n + 3]) - z1);
+            l0 += a + b;
+            l1 += e + f;
+            x[2 * n] = pack2(a, b, T());
+            x[2 * n + 1] = pack2(e, f, T());
+          }
+        }
+        // The weights before are read, and the accumulators at rest, once the second product of the tile before is over.
+        if (i > 0) wait(&sh.pv_done, (i - 1) & 1, kAtPvDone);
+        if (rescale) {
+          softmax_sync();
+          tcgen05_fence_after();
+          for (int col = 0; col < p.v_units * HT; col += 16) {
+            uint32_t o[16];
+            tmem_ld_32x16(tmem + lanes + col, o);
+#pragma unroll
+            for (int n = 0; n < 16; ++n) o[n] = __float_as_uint(__uint_as_float(o[n]) * sh.factor[col % HT + n]);
+            tmem_st_32x16(tmem + lanes + col, o);
+          }
+          asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+          tcgen05_fence_before();
+        }
+        if (active) {
+          // 16-byte piece n of row r lies at piece n ^ (r % 8) of its 128 bytes (the swizzle of K-major operands)
+          uint8_t* to = p_smem + 4 * (lane % 4);
+#pragma unroll
+          for (int n = 0; n < 8; ++n) {
+            const int piece = 16 * (n ^ (lane / 4));
+            *reinterpret_cast<uint32_t*>(to + row0 * kRowBytes + piece) = x[2 * n];
+            *reinterpret_cast<uint32_t*>(to + row1 * kRowBytes + piece) = x[2 * n + 1];
+          }
+        }
+        if (left < kTile) {
+          // What lies behind the sequence in its last page may be anything: as values it has to be 0, because 0 weights times
+          // infinity or NaN would be NaN.
+          int slot = v;
+          for (int u = 0; u < p.v_units; ++u) {
+            for (int at = left * kRowBytes + tid * 16; at < kChunkBytes; at += kSoftmaxThreads * 16) {
+              uint8_t* to = v_ring + slot * kUnitBytes + at;
+              *reinterpret_cast<uint4*>(to) = make_uint4(0u, 0u, 0u, 0u);
+              *reinterpret_cast<uint4*>(to + kChunkBytes) = make_uint4(0u, 0u, 0u, 0u);
+            }
+            if (++slot == p.v_slots) slot = 0;
+          }
+        }
+        v += p.v_units;
+        if (v >= p.v_slots) v -= p.v_slots;
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&sh.p_full));
+      }
+      // End of the segment: sums over the four threads of a head, then the accumulators, a value element per thread.
+      if (active) {
+#pragma unroll
+        for (int o = 1; o < 4; o <<= 1) {
+          l0 += __shfl_xor_sync(0xffffffffu, l0, o);
+          l1 += __shfl_xor_sync(0xffffffffu, l1, o);
+        }
+        if (lane % 4 == 0) {
+          sh.stat[row0] = make_float2(m0, l0);
+          sh.stat[row1] = make_float2(m1, l1);
+          sh.inverse[row0] = 1.f / l0;
+          sh.inverse[row1] = 1.f / l1;
+        }
+      }
+      softmax_sync();
+      wait(&sh.pv_done, (i - 1) & 1, kAtPvDone);
+      tcgen05_fence_after();
+      const int heads = min(HT, p.heads - head0);
+      if (walk.whole()) {
+        T* out = static_cast<T*>(p.out) + walk.b * p.out_sb + head0 * p.out_sh + tid;
+        for (int u = 0; u < p.v_units; ++u) {
+          for (int h0 = 0; h0 < HT; h0 += 16) {
+            uint32_t o[16];
+            tmem_ld_32x16(tmem + lanes + u * HT + h0, o);
+#pragma unroll
+            for (int n = 0; n < 16; ++n) {
+              const int h = h0 + n;
+              if (h < heads) from_float(__uint_as_float(o[n]) * sh.inverse[h], out + h * p.out_sh + u * 128);
+            }
+          }
+        }
+        if (tid < heads) {
+          const float2 st = sh.stat[tid];
+          const float lse2 = (st.x == -INFINITY ? 0.f : st.x) + log2f(st.y);
+          const long long at = static_cast<long long>(walk.b) * p.heads + head0 + tid;
+          p.lse2[at] = lse2;
+          if (p.lse != nullptr) p.lse[at] = lse2 * kLn2;
+        }
+      } else {
+        const long long part = (static_cast<long long>(worker) * p.head_tiles + head_tile) * 2 + (first_segment ? 0 : 1);
+        float* out = p.part_out + part * HT * c.dv + tid;
+        for (int u = 0; u < p.v_units; ++u) {
+          for (int h0 = 0; h0 < HT; h0 += 16) {
+            uint32_t o[16];
+            tmem_ld_32x16(tmem + lanes + u * HT + h0, o);
+#pragma unroll
+            for (int n = 0; n < 16; ++n)
+              if (h0 + n < heads) out[(h0 + n) * c.dv + u * 128] = __uint_as_float(o[n]);
+          }
+        }
+        if (tid < heads) p.part_stat[part * HT + tid] = sh.stat[tid];
+      }
+      first_segment = false;
+      tcgen05_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&sh.o_free));
+    }
+  }
+  tcgen05_fence_before();
+  __syncthreads();
+  if (warp == 5) {
+    tcgen05_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
+  }
 }
 
-// score_out = score + the weights of all heads: one warp per slot.
+// Joins the parts of split sequences, in the order of their rows, and writes what sequences without rows get. A group of dv / 4
+// threads takes every fourth part of a head.
+constexpr int kJoinGroups = 4;
+constexpr int kJoinThreads = kJoinGroups * 128;
+
 template <typename T>
-__global__ void __launch_bounds__(kAttendThreads) attend_score_kernel(const __grid_constant__ AttendParams p) {
+__global__ void __launch_bounds__(kJoinThreads) attend_join_kernel(const __grid_constant__ AttendParams p, int tile_heads) {
+  __shared__ float4 sums[kJoinGroups][128];
+  __shared__ float2 stats[512];
+  __shared__ float scratch[2][kJoinThreads / 32];
   pdl_wait();
   pdl_launch_dependents();
-  const CacheView& c = p.cache;
-  const int b = static_cast<int>(blockIdx.y), lane = static_cast<int>(threadIdx.x) & 31;
-  const int j = static_cast<int>(blockIdx.x) * kAttendWarps + (static_cast<int>(threadIdx.x) >> 5);
-  if (j >= rows_of(c, b, p.max_len)) return;
-  float sum = 0.f, q[kLaneD], x[kLaneD];
-  for (int h = 0; h < p.heads; ++h) {
-    const T* qrow = static_cast<const T*>(p.q) + b * p.q_sb + h * p.q_sh;
-#pragma unroll
-    for (int i = 0; i < kLaneD; ++i) q[i] = lane + 32 * i < c.d ? to_float(qrow[lane + 32 * i]) : 0.f;
-    const float s = logit<T>(c, q, b, j, lane, p.scale_log2, x);
-    sum += exp2f(s - p.lse[static_cast<long long>(b) * p.heads + h] * kLog2E);
+  const int b = static_cast<int>(blockIdx.y), tid = static_cast<int>(threadIdx.x);
+  const long long tiles = p.first_tile[p.batch], begin = p.first_tile[b], end = p.first_tile[b + 1];
+  const int lanes = p.cache.dv / 4, group = tid >> 7, e = tid & 127;
+  int g0 = 0, parts = 0, workers = 1;
+  if (begin < end) {
+    workers = cache_walk::workers_of(tiles, p.workers, p.least);
+    g0 = cache_walk::worker_of(tiles, workers, begin);
+    parts = cache_walk::worker_of(tiles, workers, end - 1) - g0 + 1;
+    if (parts == 1) return;  // written by its worker
   }
-  if (lane == 0) p.score_out[b * p.score_out_stride + j] = p.score[b * p.score_stride + j] + sum;
+  for (int h = static_cast<int>(blockIdx.x); h < p.heads; h += static_cast<int>(gridDim.x)) {
+    T* out = static_cast<T*>(p.out) + b * p.out_sb + h * p.out_sh;
+    const long long at = static_cast<long long>(b) * p.heads + h;
+    if (parts == 0) {
+      for (int i = tid; i < p.cache.dv; i += kJoinThreads) from_float(0.f, out + i);
+      if (tid == 0) {
+        p.lse2[at] = -INFINITY;
+        if (p.lse != nullptr) p.lse[at] = -INFINITY;
+      }
+      continue;
+    }
+    const int head_tile = h / tile_heads;
+    auto part_of = [&](int i) {
+      const int g = g0 + i;
+      const int slot = cache_walk::part_slot(cache_walk::share_begin(tiles, workers, g), begin);
+      return ((static_cast<long long>(g) * p.head_tiles + head_tile) * 2 + slot) * tile_heads + (h - head_tile * tile_heads);
+    };
+    // The largest maximum; parts fit the array because there are no more than workers (checked by the launch).
+    __syncthreads();
+    float top = -INFINITY;
+    for (int i = tid; i < parts; i += kJoinThreads) {
+      stats[i] = p.part_stat[part_of(i)];
+      top = fmaxf(top, stats[i].x);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    if ((tid & 31) == 0) scratch[0][tid >> 5] = top;
+    __syncthreads();
+    for (int w = 0; w < kJoinThreads / 32; ++w) top = fmaxf(top, scratch[0][w]);
+    const float base = top == -INFINITY ? 0.f : top;
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+    float total = 0.f;
+    for (int i = 0; i < parts; ++i) total += stats[i].y * exp2_fast(stats[i].x - base);
+    if (e < lanes) {
+#pragma unroll 4
+      for (int i = group; i < parts; i += kJoinGroups) {
+        const float w = exp2_fast(stats[i].x - base);
+        const float4 v = *reinterpret_cast<const float4*>(p.part_out + part_of(i) * p.cache.dv + 4 * e);
+        sum.x += w * v.x;
+        sum.y += w * v.y;
+        sum.z += w * v.z;
+        sum.w += w * v.w;
+      }
+      sums[group][e] = sum;
+    }
+    __syncthreads();
+    if (group == 0 && e < lanes) {
+#pragma unroll
+      for (int k = 1; k < kJoinGroups; ++k) {
+        const float4 v = sums[k][e];
+        sum.x += v.x;
+        sum.y += v.y;
+        sum.z += v.z;
+        sum.w += v.w;
+      }
+      const float inverse = 1.f / total;
+      from_float(sum.x * inverse, out + 4 * e);
+      from_float(sum.y * inverse, out + 4 * e + 1);
+      from_float(sum.z * inverse, out + 4 * e + 2);
+      from_float(sum.w * inverse, out + 4 * e + 3);
+    }
+    if (tid == 0) {
+      const float lse2 = base + log2f(total);
+      p.lse2[at] = lse2;
+      if (p.lse != nullptr) p.lse[at] = lse2 * kLn2;
+    }
+  }
+}
+
+// score_out = score + the weights of all heads, from the logits that the attention left: a CTA per tile, four groups of heads.
+constexpr int kScoreThreads = 4 * kTile;
+
+__global__ void __launch_bounds__(kScoreThreads) attend_score_kernel(const __grid_constant__ AttendParams p) {
+  __shared__ float sums[4][kTile];
+  pdl_wait();
+  pdl_launch_dependents();
+  const int b = static_cast<int>(blockIdx.y), tile = static_cast<int>(blockIdx.x);
+  const int rows = rows_of(p.cache, b, p.max_len);
+  if (tile * kTile >= rows) return;
+  const int col = static_cast<int>(threadIdx.x) % kTile, group = static_cast<int>(threadIdx.x) / kTile;
+  const float* x = p.logits + (static_cast<long long>(b) * p.logit_tiles + tile) * p.heads * kTile + col;
+  const float* lse2 = p.lse2 + static_cast<long long>(b) * p.heads;
+  float sum = 0.f;
+#pragma unroll 4
+  for (int h = group; h < p.heads; h += 4) sum += exp2_fast(x[static_cast<long long>(h) * kTile] - lse2[h]);
+  sums[group][col] = sum;
+  __syncthreads();
+  const int j = tile * kTile + col;
+  if (group == 0 && j < rows)
+    p.score_out[b * p.score_out_stride + j] = p.score[b * p.score_stride + j] + ((sums[0][col] + sums[1][col]) + (sums[2][col] + sums[3][col]));
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -411,8 +1142,8 @@ __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const __grid_c
 // ---------------------------------------------------------------------------------------------
 
 // <<<grid, threads>>> on `stream`, allowed to begin under the kernel before it (see pdl_wait).
-template <typename Params>
-int launch_pdl(void (*kernel)(Params), dim3 grid, int threads, size_t smem, void* stream, const Params& params) {
+template <typename... Params>
+int launch_pdl(void (*kernel)(Params...), dim3 grid, int threads, size_t smem, void* stream, const std::decay_t<Params>&... params) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = dim3(static_cast<unsigned>(threads), 1, 1);
@@ -423,7 +1154,7 @@ int launch_pdl(void (*kernel)(Params), dim3 grid, int threads, size_t smem, void
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  if (cudaLaunchKernelEx(&cfg, kernel, params) != cudaSuccess) {
+  if (cudaLaunchKernelEx(&cfg, kernel, params...) != cudaSuccess) {
     (void)cudaGetLastError();
     return B200_FP8_MM_ERR_LAUNCH;
   }
@@ -450,6 +1181,121 @@ int view_of(const b200_mla_cache* c, CacheView* v) {
   *v = CacheView{c->data, c->block_table, c->lens, c->pages, c->page_size, c->pages_per_seq, static_cast<int>(capacity),
                  c->dv, d, c->page_stride, c->slot_stride, c->table_stride};
   return B200_FP8_MM_OK;
+}
+
+constexpr int kMaxHeads = 1 << 16;
+constexpr int kMaxDevices = 64;
+constexpr int kLeastTiles = 1;
+
+int current_device() {
+  int dev = -1;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) {
+    (void)cudaGetLastError();
+    return -1;
+  }
+  return dev;
+}
+
+// SM count of the current device, looked up once; B200's where there is none (sizes are asked for on hosts without a GPU too).
+int sm_count_for_sizing() {
+  static std::atomic<int> known[kMaxDevices];
+  const int dev = current_device();
+  if (dev < 0) return 148;
+  int n = known[dev].load(std::memory_order_relaxed);
+  if (n == 0) {
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) {
+      (void)cudaGetLastError();
+      return 148;
+    }
+    known[dev].store(n, std::memory_order_relaxed);
+  }
+  return n;
+}
+
+// Heads per tile. N of the second product, and what the queries take of shared memory.
+int tile_heads_for(int heads) { return heads <= 16 ? 16 : heads <= 32 ? 32 : 64; }
+
+// Workers per head tile: one CTA per SM.
+int attend_workers(int heads, int sms) {
+  const int ht = tile_heads_for(heads), tiles = (heads + ht - 1) / ht;
+  const int n = sms / tiles;
+  return n < 1 ? 1 : n < 512 ? n : 512;  // (the join holds the statistics of 512 parts)
+}
+
+struct AttendWorkspace {
+  size_t lse2, part_stat, part_out, logits, bytes;
+};
+
+AttendWorkspace attend_workspace(int batch, int heads, int dv, int max_len, bool with_score, int sms) {
+  const size_t ht = tile_heads_for(heads), head_tiles = (heads + ht - 1) / ht;
+  const size_t parts = 2 * head_tiles * attend_workers(heads, sms) * ht;
+  auto up = [](size_t n) { return (n + 255) / 256 * 256; };
+  AttendWorkspace w;
+  w.lse2 = up((static_cast<size_t>(batch) + 1) * sizeof(long long));
+  w.part_stat = w.lse2 + up(static_cast<size_t>(batch) * heads * sizeof(float));
+  w.part_out = w.part_stat + up(parts * sizeof(float2));
+  w.logits = w.part_out + up(parts * dv * sizeof(float));
+  w.bytes = w.logits + (with_score ? up(static_cast<size_t>(batch) * cache_walk::tiles_of(max_len) * heads * kTile * sizeof(float)) : 0);
+  return w;
+}
+
+// Ring slots: as many tiles as fit, the value in units that are freed one by one. Returns the shared memory of the CTA.
+size_t plan_rings(int ht, AttendParams* p) {
+  const int fixed = kHeaderBytes + (2 * p->v_units + p->r_chunks) * ht * kRowBytes + ht * kRowBytes;
+  const int r_bytes = p->r_chunks * kChunkBytes;
+  p->r_slots = p->r_chunks > 0 ? 2 : 0;
+  auto units = [&](int r) {
+    const int n = (kMaxSmem - fixed - r * r_bytes) / kUnitBytes;
+    return n < kMaxV ? n : kMaxV;
+  };
+  while (p->r_chunks > 0 && p->r_slots < kMaxR && units(p->r_slots + 1) > p->v_units * p->r_slots) ++p->r_slots;
+  p->v_slots = units(p->r_slots);
+  return static_cast<size_t>(fixed) + p->v_slots * kUnitBytes + p->r_slots * r_bytes;
+}
+
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+// [outer][inner][d] of 16-bit elements, box: 64 elements of `rows` inner rows, 128-byte swizzle. What lies outside reads as 0.
+bool encode_rows(CUtensorMap* map, const void* base, bool bf16, int d, int inner, int outer, long long inner_stride, long long outer_stride,
+                 int rows) {
+  static const EncodeTiledFn fn = []() -> EncodeTiledFn {
+    void* ptr = nullptr;
+    cudaDriverEntryPointQueryResult found;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &found) != cudaSuccess || found != cudaDriverEntryPointSuccess) {
+      (void)cudaGetLastError();
+      return nullptr;
+    }
+    return reinterpret_cast<EncodeTiledFn>(ptr);
+  }();
+  if (fn == nullptr) return false;
+  const cuuint64_t dims[3] = {static_cast<cuuint64_t>(d), static_cast<cuuint64_t>(inner), static_cast<cuuint64_t>(outer)};
+  const cuuint64_t strides[2] = {static_cast<cuuint64_t>(inner_stride) * 2, static_cast<cuuint64_t>(outer_stride) * 2};
+  const cuuint32_t box[3] = {64, static_cast<cuuint32_t>(rows), 1}, steps[3] = {1, 1, 1};
+  return fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(base), dims, strides, box,
+            steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+typedef void (*AttendFn)(const CUtensorMap, const CUtensorMap, const AttendParams);
+
+AttendFn attend_fn(bool bf16, int ht) {
+  if (bf16) return ht == 16 ? attend_kernel<__nv_bfloat16, 16> : ht == 32 ? attend_kernel<__nv_bfloat16, 32> : attend_kernel<__nv_bfloat16, 64>;
+  return ht == 16 ? attend_kernel<__half, 16> : ht == 32 ? attend_kernel<__half, 32> : attend_kernel<__half, 64>;
+}
+
+// Lets the kernel take all of an SM's shared memory, once per device.
+bool opt_in(AttendFn fn, bool bf16, int ht, int device) {
+  static std::atomic<bool> done[kMaxDevices][6];
+  std::atomic<bool>& d = done[device][(bf16 ? 0 : 3) + (ht == 16 ? 0 : ht == 32 ? 1 : 2)];
+  if (d.load(std::memory_order_relaxed)) return true;
+  if (cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem) != cudaSuccess) {
+    (void)cudaGetLastError();
+    return false;
+  }
+  d.store(true, std::memory_order_relaxed);
+  return true;
 }
 
 int evict_most(long long capacity, int budget) {
@@ -495,47 +1341,72 @@ int b200_mla_cache_append(const b200_mla_cache* cache, const void* row, long lon
 }
 
 size_t b200_mla_cache_attend_workspace_bytes(int batch, int heads, int dv, int dr, int max_len, int with_score) {
-  (void)dv, (void)dr, (void)max_len, (void)with_score;
-  if (batch <= 0 || heads <= 0) return 0;
-  return (static_cast<size_t>(batch) * heads * sizeof(float) + 255) / 256 * 256;
+  (void)dr;
+  if (batch <= 0 || heads <= 0 || dv <= 0 || max_len <= 0) return 0;
+  return attend_workspace(batch, heads, dv, max_len, with_score != 0, sm_count_for_sizing()).bytes;
 }
 
 int b200_mla_cache_attend(const b200_mla_cache* cache, const void* q, long long q_sb, long long q_sh, int heads, float scale,
                           void* out, long long out_sb, long long out_sh, float* lse, const float* score,
                           long long score_stride, float* score_out, long long score_out_stride, int max_len, void* workspace,
                           size_t workspace_bytes, int* device_status, void* stream) {
-  AttendParams p;
+  AttendParams p = {};
   int rc = view_of(cache, &p.cache);
   if (rc != B200_FP8_MM_OK) return rc;
   if (q == nullptr || out == nullptr || (score_out != nullptr && score == nullptr)) return B200_FP8_MM_ERR_NULL;
-  if (heads <= 0 || heads > (1 << 16) || max_len < 0 || !isfinite(scale)) return B200_FP8_MM_ERR_SHAPE;
-  if (q_sb % 8 != 0 || q_sh % 8 != 0 || q_sb < 0 || q_sh < 0) return B200_FP8_MM_ERR_STRIDE;
+  if (heads <= 0 || heads > kMaxHeads || max_len < 0 || !isfinite(scale)) return B200_FP8_MM_ERR_SHAPE;
+  if (cache->batch == 1) q_sb = p.cache.d;  // (no second one)
+  if (heads == 1) q_sh = p.cache.d;
+  if (q_sb % 8 != 0 || q_sh % 8 != 0 || q_sb < p.cache.d || q_sh < p.cache.d) return B200_FP8_MM_ERR_STRIDE;
   if (!aligned16(q)) return B200_FP8_MM_ERR_ALIGN;
-  (void)device_status;
   if (max_len == 0 || max_len > p.cache.capacity) max_len = p.cache.capacity;
-  if (workspace == nullptr || reinterpret_cast<uintptr_t>(workspace) % 256 != 0 ||
-      workspace_bytes < b200_mla_cache_attend_workspace_bytes(cache->batch, heads, cache->dv, cache->dr, max_len, score_out != nullptr))
-    return B200_FP8_MM_ERR_WORKSPACE;
-  p.q = q;
+  const int sms = sm_count_for_sizing();
+  const AttendWorkspace w = attend_workspace(cache->batch, heads, cache->dv, max_len, score_out != nullptr, sms);
+  if (workspace == nullptr || reinterpret_cast<uintptr_t>(workspace) % 256 != 0 || workspace_bytes < w.bytes) return B200_FP8_MM_ERR_WORKSPACE;
+  const int ht = tile_heads_for(heads), device = current_device();
+  if (device < 0) return B200_FP8_MM_ERR_DRIVER;
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
   p.out = out;
-  p.lse = lse != nullptr ? lse : static_cast<float*>(workspace);
+  p.lse = lse;
   p.score = score;
   p.score_out = score_out;
-  p.q_sb = q_sb;
-  p.q_sh = q_sh;
   p.out_sb = out_sb;
   p.out_sh = out_sh;
   p.score_stride = score_stride;
   p.score_out_stride = score_out_stride;
   p.heads = heads;
+  p.head_tiles = (heads + ht - 1) / ht;
   p.max_len = max_len;
+  p.batch = cache->batch;
+  p.workers = attend_workers(heads, sms);
+  p.least = kLeastTiles;
+  p.copy_rows = cache_walk::copy_rows(cache->page_size);
+  p.v_units = cache->dv / 128;
+  p.r_chunks = cache->dr / 64;
   p.scale_log2 = scale * kLog2E;
+  p.first_tile = reinterpret_cast<long long*>(ws);
+  p.lse2 = reinterpret_cast<float*>(ws + w.lse2);
+  p.part_stat = reinterpret_cast<float2*>(ws + w.part_stat);
+  p.part_out = reinterpret_cast<float*>(ws + w.part_out);
+  p.logits = score_out != nullptr ? reinterpret_cast<float*>(ws + w.logits) : nullptr;
+  p.logit_tiles = cache_walk::tiles_of(max_len);
+  p.status = device_status;
+  const size_t smem = plan_rings(ht, &p);
   const bool bf16 = cache->dtype == B200_MLA_CACHE_BF16;
-  const dim3 grid(static_cast<unsigned>(heads), static_cast<unsigned>(cache->batch));
-  rc = launch_pdl(bf16 ? attend_kernel<__nv_bfloat16> : attend_kernel<__half>, grid, kAttendThreads, 0, stream, p);
+  CUtensorMap q_map, row_map;
+  if (!encode_rows(&q_map, q, bf16, p.cache.d, heads, cache->batch, q_sh, q_sb, ht) ||
+      !encode_rows(&row_map, cache->data, bf16, p.cache.d, cache->page_size, cache->pages, cache->slot_stride, cache->page_stride, p.copy_rows))
+    return B200_FP8_MM_ERR_DRIVER;
+  const AttendFn fn = attend_fn(bf16, ht);
+  if (!opt_in(fn, bf16, ht, device)) return B200_FP8_MM_ERR_DRIVER;
+  rc = launch_pdl(fn, dim3(static_cast<unsigned>(p.workers) * p.head_tiles), kAttendThreads, smem, stream, q_map, row_map, p);
+  if (rc != B200_FP8_MM_OK) return rc;
+  // CTAs for every SM a few times over, however few sequences there are; those of a sequence share its heads.
+  const int each = (4 * sms + cache->batch - 1) / cache->batch;
+  const dim3 joins(static_cast<unsigned>(each < heads ? each : heads), static_cast<unsigned>(cache->batch));
+  rc = launch_pdl(bf16 ? attend_join_kernel<__nv_bfloat16> : attend_join_kernel<__half>, joins, kJoinThreads, 0, stream, p, ht);
   if (rc != B200_FP8_MM_OK || score_out == nullptr) return rc;
-  const dim3 slots(static_cast<unsigned>((max_len + kAttendWarps - 1) / kAttendWarps), static_cast<unsigned>(cache->batch));
-  return launch_pdl(bf16 ? attend_score_kernel<__nv_bfloat16> : attend_score_kernel<__half>, slots, kAttendThreads, 0, stream, p);
+  return launch_pdl(attend_score_kernel, dim3(static_cast<unsigned>(p.logit_tiles), static_cast<unsigned>(cache->batch)), kScoreThreads, 0, stream, p);
 }
 
 size_t b200_mla_cache_evict_workspace_bytes(int batch, int capacity, int budget) {

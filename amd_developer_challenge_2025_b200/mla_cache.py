@@ -179,8 +179,9 @@ def mla_cache_attend(q, cache, block_table, lens, dv: int, scale: float, out=Non
     _check_heads("q", q, cache, batch, d)
     heads = q.shape[1]
     _check(heads <= 1 << 16, "at most 65536 heads")
-    _check(q.stride(0) % 8 == 0 and q.stride(1) % 8 == 0 and q.data_ptr() % 16 == 0,
-           "q: strides must be multiples of 8 elements and the base address of 16 bytes")
+    _check(all(size == 1 or (stride % 8 == 0 and stride >= d) for size, stride in zip(q.shape[:2], q.stride()))
+           and q.data_ptr() % 16 == 0,
+           "q: strides must be multiples of 8 elements, at least a row's, and the base address a multiple of 16 bytes")
     scale = float(scale)
     _check(math.isfinite(scale), "scale must be finite")
     _check(max_len is None or (isinstance(max_len, int) and max_len > 0), "max_len must be a positive integer")
