@@ -151,16 +151,17 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_con
 constexpr float kLn2 = 0.69314718055994531f, kLog2E = 1.4426950408889634f;
 constexpr int kMaxD = 576;
 constexpr int kTile = cache_walk::kTileRows;   // rows of the cache per tile
-constexpr int kRowBytes = 128;                 // of a row that one swizzled chunk holds: 64 elements
-constexpr int kChunkBytes = kTile * kRowBytes; // 64 rows x 64 elements
-constexpr int kUnitBytes = 2 * kChunkBytes;    // 128 elements of the value: the rows of one second product
-constexpr int kMaxV = 16, kMaxR = 8;           // ring slots
+constexpr int kRowBytes = 128;                 // of a row that lie together under the 128-byte swizzle: a chunk of 64 elements
+constexpr int kGroupBytes = 8 * kRowBytes;     // 8 rows of a chunk, the swizzle's period
+constexpr int kMaxV = 15, kMaxR = 8;           // ring slots
+constexpr int kTurns = 16;                     // barriers of the products, one per tile in turn: a wait tells a phase's parity only,
+                                               // so there are more of them than tiles can be in the rings
 constexpr int kSoftmaxThreads = 128;
 constexpr int kAttendThreads = kSoftmaxThreads + 64;
 constexpr int kHeaderBytes = 2048;             // barriers and small arrays, behind the rings
 constexpr int kMaxSmem = 232448;               // 227 KiB opt-in limit per CTA on sm_100
 constexpr int kTmemCols = 512;
-constexpr int kTmemLogits = 256;               // two buffers of 64 columns behind the accumulators
+constexpr int kTmemLogits = 256;               // two buffers of a tile's columns behind the accumulators
 constexpr unsigned long long kWaitLimitNs = 2000000000ull;
 constexpr float kRescaleAbove = 8.f;  // log2: a running maximum is replaced when it is exceeded by this much
 
@@ -174,7 +175,7 @@ struct AttendParams {
   int heads, head_tiles, max_len, batch;
   int workers, least;      // workers per head tile, and the least tiles worth one
   int copy_rows;           // cache_walk::copy_rows(page_size)
-  int v_slots, r_slots;    // ring slots of a unit each: value units, units of the elements behind the value
+  int v_slots, r_slots;    // ring slots of a unit each: 128 elements of the value; all elements behind the value
   int v_units, r_chunks;   // units of a tile; chunks behind the value
   float scale_log2;        // scale * log2(e)
   // Workspace
@@ -182,7 +183,7 @@ struct AttendParams {
   float* lse2;             // [batch][heads]: log2 of the sum of 2^x
   float2* part_stat;       // [worker][head tile][2][heads of a tile]: maximum and sum
   float* part_out;         // the same, times dv
-  float* logits;           // [batch][tile][heads][64] in log2, or null
+  float* logits;           // [batch][tile][heads][rows of a tile] in log2, or null
   int logit_tiles;
   int* status;             // may be null
 };
@@ -253,14 +254,39 @@ struct Waits {
   __device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, int where) const {
     return mbar_try_wait(bar, parity, 200000) || slow(bar, parity, where);
   }
+  // For a whole warp, which leaves together.
+  __device__ __forceinline__ bool wait_all(uint32_t bar, uint32_t parity, int where) const {
+    return __all_sync(0xffffffffu, wait(bar, parity, where)) != 0;
+  }
 };
 
-enum Where { kAtQFull = 0x201, kAtVFull, kAtRFull, kAtVEmpty, kAtREmpty, kAtQEmpty, kAtSFull, kAtSFree, kAtPFull, kAtPvDone, kAtOFree };
+enum Where { kAtVEmpty = 0x201, kAtREmpty, kAtQEmpty, kAtOperands, kAtSFull, kAtPvDone };
 
-__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, uint32_t bar) {
+// A barrier that takes turns with others of its kind: parity of the phase that its use for tile i completes.
+__device__ __forceinline__ uint32_t turn_parity(int i) { return static_cast<uint32_t>(i / kTurns) & 1u; }
+
+// Copies for a whole warp, which comes here together: one lane issues.
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, int c1, int c2, int c3, uint32_t bar) {
   asm volatile(
-      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
-      "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(bar)
+      "{\n\t.reg .pred leader;\n\t"
+      "elect.sync _|leader, 0xffffffff;\n\t"
+      "@leader cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];\n\t}" ::"r"(dst),
+      "l"(map), "r"(0), "r"(c1), "r"(c2), "r"(c3), "r"(bar)
+      : "memory");
+}
+__device__ __forceinline__ void tma_load_5d(uint32_t dst, const CUtensorMap* map, int c1, int c2, int c3, int c4, uint32_t bar) {
+  asm volatile(
+      "{\n\t.reg .pred leader;\n\t"
+      "elect.sync _|leader, 0xffffffff;\n\t"
+      "@leader cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, %6}], [%7];\n\t}" ::"r"(dst),
+      "l"(map), "r"(0), "r"(c1), "r"(c2), "r"(c3), "r"(c4), "r"(bar)
+      : "memory");
+}
+// For one thread.
+__device__ __forceinline__ void tma_load_4d_own(uint32_t dst, const CUtensorMap* map, int c1, int c2, int c3, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
+      "l"(map), "r"(0), "r"(c1), "r"(c2), "r"(c3), "r"(bar)
       : "memory");
 }
 
@@ -268,19 +294,26 @@ __device__ __forceinline__ void tcgen05_fence_before() { asm volatile("tcgen05.f
 __device__ __forceinline__ void tcgen05_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
 // Matrix descriptors as 32-bit halves, as in the GEMM: low word address and leading offset, high word stride offset, version
-// and the 128-byte swizzle. Only the address changes between instructions.
-__device__ __forceinline__ void umma_f16(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t hi, uint32_t idesc, uint32_t accumulate) {
+// and the 128-byte swizzle. Only the address changes between instructions. The whole warp comes here and one lane of it, always
+// the same, issues.
+__device__ __forceinline__ void umma_f16(uint32_t d, uint32_t a_lo, uint32_t a_hi, uint32_t b_lo, uint32_t b_hi, uint32_t idesc,
+                                         uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
-      "mov.b64 da, {%1, %3};\n\t"
-      "mov.b64 db, {%2, %3};\n\t"
-      "setp.ne.b32 p, %5, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %4, p;\n\t}" ::"r"(d),
-      "r"(a_lo), "r"(b_lo), "r"(hi), "r"(idesc), "r"(accumulate)
+      "{\n\t.reg .pred p, leader;\n\t.reg .b64 da, db;\n\t"
+      "elect.sync _|leader, 0xffffffff;\n\t"
+      "mov.b64 da, {%1, %2};\n\t"
+      "mov.b64 db, {%3, %4};\n\t"
+      "setp.ne.b32 p, %6, 0;\n\t"
+      "@leader tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %5, p;\n\t}" ::"r"(d),
+      "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate)
       : "memory");
 }
 __device__ __forceinline__ void umma_commit(uint32_t bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+  asm volatile(
+      "{\n\t.reg .pred leader;\n\t"
+      "elect.sync _|leader, 0xffffffff;\n\t"
+      "@leader tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar)
+      : "memory");
 }
 
 // 16 lanes x 64 columns: thread t gets columns 8 i + 2 (t % 4) + {0, 1} of lane t / 4 in v[4 i + {0, 1}], of lane t / 4 + 8 in
@@ -349,8 +382,11 @@ __device__ __forceinline__ bool softmax_any(bool mine) {
 
 // What the roles of a CTA share, at the end of its shared memory.
 struct alignas(8) AttendShared {
-  uint64_t v_full[kMaxV], v_empty[kMaxV], r_full[kMaxR], r_empty[kMaxR];
-  uint64_t q_full, q_empty, s_full[2], s_free[2], p_full, pv_done, o_free, drained;
+  uint64_t v_full[kMaxV], r_full[kMaxR];  // a unit is there
+  uint64_t s_full[kTurns];   // a tile's first product is done: its elements behind the value are free
+  uint64_t pv_half[kTurns];  // the second product is done with the first half of the tile's value units
+  uint64_t pv_done[kTurns];  // and with all
+  uint64_t q_full, q_empty, s_free[2], p_full, o_free, drained;
   float factor[64];   // by which a head's accumulators are multiplied when its maximum is replaced
   float inverse[64];  // 1 / sum of weights
   float2 stat[64];
@@ -360,6 +396,7 @@ struct alignas(8) AttendShared {
   int expired, first_seq, first_tile;
 };
 static_assert(sizeof(AttendShared) <= kHeaderBytes, "the header is too small");
+static_assert(kTurns > kMaxV && kTurns > kMaxR, "a phase could be taken for one two turns before it");
 
 // A worker's walk over its share: segment after segment, each a run of tiles of one sequence.
 struct Walk {
@@ -395,50 +432,54 @@ struct Walk {
 // With the value's elements in the lanes, the accumulators of 64 heads take 256 of the 512 TMEM columns; with the heads in the
 // lanes, 128 heads would take them all and leave none for S. Fewer heads shrink N (16 or 32) and what Q takes of shared memory.
 //
-// One CTA per SM and worker: warp 4 copies (TMA, 128-byte swizzle; Q once per segment, rows in units of 128 value elements that
-// are freed one by one), warp 5 issues the products, warps 0 to 3 do the softmax (S comes as the 16 x 256-bit fragments: 4 threads
-// to a head) and the epilogue. S is double buffered; the next tile's first product runs under this tile's softmax. The running
-// maximum is replaced only when a logit exceeds it by 2^8: the weights stay below 2^8, which no type here minds, and rescaling the
-// accumulators is rare. Sums are kept in fp32, weights are rounded to the cache's type for the second product, as matrix operands
-// have to be.
+// A tile comes in units of 128 elements of the value (and one of what lies behind it), each in shared memory as [8 groups of
+// rows][chunk of 64 elements][8 rows x 128 bytes]: one stride from group to group for both operands, and one copy brings a unit of as
+// many rows as lie together in a page. The first product takes units as they come, the second one frees them half a tile at a time, so
+// that a slot is on its way to being filled again while the rest of its tile is still in use.
+//
+// One CTA per SM and worker: warp 4 copies, warp 5 issues the products, warps 0 to 3 do the softmax (S comes as 16 x 256-bit
+// fragments, 4 threads to a head) and the epilogue. S is double buffered; the next tile's first product runs under this tile's
+// softmax. The running maximum is replaced only when a logit exceeds it by 2^8: the weights stay below 2^8, which no type here
+// minds, and rescaling the accumulators is rare. Sums are kept in fp32, weights are rounded to the cache's type for the second
+// product, as matrix operands have to be.
 template <typename T, int HT>
 __global__ void __launch_bounds__(kAttendThreads, 1)
-attend_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap row_map, const __grid_constant__ AttendParams p) {
+attend_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap v_map, const __grid_constant__ CUtensorMap r_map,
+              const __grid_constant__ AttendParams p) {
   extern __shared__ __align__(1024) uint8_t smem[];
   const CacheView& c = p.cache;
-  const int chunks = 2 * p.v_units + p.r_chunks;
-  uint8_t* const q_smem = smem;
+  constexpr int kUnitBytes = 2 * kTile * kRowBytes;
+  const int chunks = 2 * p.v_units + p.r_chunks, r_bytes = p.r_chunks * kTile * kRowBytes;
+  uint8_t* const q_smem = smem;  // [chunk][HT rows x 128 bytes]; the first product reads 64 rows, those behind HT are never looked at
   uint8_t* const v_ring = q_smem + chunks * HT * kRowBytes;
   uint8_t* const r_ring = v_ring + p.v_slots * kUnitBytes;
-  uint8_t* const p_smem = r_ring + p.r_slots * p.r_chunks * kChunkBytes;
+  uint8_t* const p_smem = r_ring + p.r_slots * r_bytes;
   AttendShared& sh = *reinterpret_cast<AttendShared*>(p_smem + HT * kRowBytes);
   const int tid = static_cast<int>(threadIdx.x), warp = tid >> 5, lane = tid & 31;
   const int head_tile = static_cast<int>(blockIdx.x) % p.head_tiles, worker = static_cast<int>(blockIdx.x) / p.head_tiles;
   const int head0 = head_tile * HT;
   const Waits waits{&sh.expired, p.status};
   if (tid == 0) {
-    for (int i = 0; i < kMaxV; ++i) {
-      mbar_init(smem_u32(&sh.v_full[i]), 1);
-      mbar_init(smem_u32(&sh.v_empty[i]), 1);
-    }
-    for (int i = 0; i < kMaxR; ++i) {
-      mbar_init(smem_u32(&sh.r_full[i]), 1);
-      mbar_init(smem_u32(&sh.r_empty[i]), 1);
+    for (int i = 0; i < kMaxV; ++i) mbar_init(smem_u32(&sh.v_full[i]), 1);
+    for (int i = 0; i < kMaxR; ++i) mbar_init(smem_u32(&sh.r_full[i]), 1);
+    for (int i = 0; i < kTurns; ++i) {
+      mbar_init(smem_u32(&sh.s_full[i]), 1);
+      mbar_init(smem_u32(&sh.pv_half[i]), 1);
+      mbar_init(smem_u32(&sh.pv_done[i]), 1);
     }
     mbar_init(smem_u32(&sh.q_full), 1);
     mbar_init(smem_u32(&sh.q_empty), 1);
     for (int i = 0; i < 2; ++i) {
-      mbar_init(smem_u32(&sh.s_full[i]), 1);
       mbar_init(smem_u32(&sh.s_free[i]), 4);
     }
     mbar_init(smem_u32(&sh.p_full), 4);
-    mbar_init(smem_u32(&sh.pv_done), 1);
     mbar_init(smem_u32(&sh.o_free), 4);
     mbar_init(smem_u32(&sh.drained), 1);
     sh.expired = (smem_u32(smem) & 1023u) != 0;  // the swizzle needs it; never so with no static shared memory before it
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&q_map) : "memory");
-    asm volatile("prefetch.tensormap [%0];" ::"l"(&row_map) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&v_map) : "memory");
+    if (p.r_chunks > 0) asm volatile("prefetch.tensormap [%0];" ::"l"(&r_map) : "memory");
   }
   if (warp == 5) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem_base)), "r"(kTmemCols) : "memory");
@@ -496,175 +537,213 @@ attend_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__
   }
   __syncthreads();
 
+  const int n1 = p.v_units / 2;  // units of the first half
   if (warp == 4) {
-    // Copies. A lane takes the pieces (copy_rows rows of one page) lane, lane + 32 of a tile.
-    const int pieces = kTile / p.copy_rows, r_bytes = p.r_chunks * kChunkBytes;
-    int v = 0, r = 0, segment = 0;
-    uint32_t v_phase = 0, r_phase = 0;
-    bool ok = sh.expired == 0;
-    auto all_wait = [&](uint64_t* bar, uint32_t parity, int where) {
-      return __all_sync(0xffffffffu, waits.wait(smem_u32(bar), parity, where)) != 0;
-    };
+    // Copies. Lane l knows where pieces l and l + 32 (copy_rows rows each) of a tile come from.
+    const int pieces = kTile / p.copy_rows;
+    int v = 0, r = 0, segment = 0, i = 0;
+    int old_i = 0, old_u = -p.v_slots;  // the unit that was in the slot to be filled: none while negative
+    bool ok = __all_sync(0xffffffffu, sh.expired == 0);
     Walk walk(sh);
-    while (ok && walk.next(p)) {
+    while (ok && __all_sync(0xffffffffu, walk.next(p))) {
       const int* table = c.block_table + walk.b * c.table_stride;
-      // (page, slot) of this lane's pieces of a tile; rows behind the sequence come from a page behind the last, as zeros
-      auto place = [&](int tile, int k, int* page, int* slot) {
-        const int row = tile * kTile + (lane + 32 * k) * p.copy_rows;
-        *page = c.pages;
-        *slot = 0;
-        if (lane + 32 * k < pieces && tile < walk.t + walk.count && row < walk.rows) {
-          const int at = row / c.page_size;
-          *slot = row - at * c.page_size;
-          const int id = table[at];
-          *page = id < 0 || id > c.pages ? c.pages : id;
+      int page[2], slot[2];
+      // rows behind the sequence come from a page behind the last, as zeros
+      auto place = [&](int tile) {
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const int piece = lane + 32 * k, row = tile * kTile + piece * p.copy_rows;
+          page[k] = c.pages;
+          slot[k] = 0;
+          if (piece < pieces && tile < walk.t + walk.count && row < walk.rows) {
+            const int at = row / c.page_size;
+            slot[k] = row - at * c.page_size;
+            const int id = table[at];
+            page[k] = id < 0 || id > c.pages ? c.pages : id;
+          }
         }
       };
-      int page[2], slot[2];
-      for (int k = 0; k < 2; ++k) place(walk.t, k, &page[k], &slot[k]);
-      for (int tile = walk.t; ok && tile < walk.t + walk.count; ++tile) {
-        int next_page[2], next_slot[2];
-        for (int k = 0; k < 2; ++k) place(tile + 1, k, &next_page[k], &next_slot[k]);  // on their way during this tile's waits
-        auto copy = [&](uint8_t* dst, int chunk0, int n, uint64_t* full) {
-          if (lane == 0) mbar_expect_tx(smem_u32(full), n * kChunkBytes);
+      place(walk.t);
+      const int count = __shfl_sync(0xffffffffu, walk.count, 0);
+      for (int tile = 0; ok && tile < count; ++tile, ++i) {
+        // `n` chunks from `chunk` on of the tile's rows
+        auto copy = [&](uint32_t to, const CUtensorMap* map, int chunk, int n, uint32_t full) {
+          if (lane == 0) mbar_expect_tx(full, n * kTile * kRowBytes);
           __syncwarp();
-          for (int k = 0; k < 2; ++k) {
-            const int piece = lane + 32 * k;
-            if (piece >= pieces) break;
-            for (int i = 0; i < n; ++i)
-              tma_load_3d(smem_u32(dst) + i * kChunkBytes + piece * p.copy_rows * kRowBytes, &row_map, (chunk0 + i) * 64, slot[k], page[k],
-                          smem_u32(full));
+          if (p.copy_rows >= 8) {
+            for (int k = 0; k < pieces; ++k)
+              tma_load_5d(to + k * (p.copy_rows >> 3) * n * kGroupBytes, map, 0, chunk, __shfl_sync(0xffffffffu, slot[0], k) >> 3,
+                          __shfl_sync(0xffffffffu, page[0], k), full);
+          } else {
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              const int piece = lane + 32 * k, row = piece * p.copy_rows;
+              if (piece < pieces)
+                for (int m = 0; m < n; ++m)
+                  tma_load_4d_own(to + ((row >> 3) * n + m) * kGroupBytes + (row & 7) * kRowBytes, map, slot[k], chunk + m, page[k], full);
+            }
           }
         };
         if (p.r_chunks > 0) {
-          if (!(ok = all_wait(&sh.r_empty[r], r_phase ^ 1, kAtREmpty))) break;
-          copy(r_ring + r * r_bytes, 2 * p.v_units, p.r_chunks, &sh.r_full[r]);
-          if (++r == p.r_slots) r = 0, r_phase ^= 1;
+          const int old = i - p.r_slots;
+          if (old >= 0 && !(ok = waits.wait_all(smem_u32(&sh.s_full[old % kTurns]), turn_parity(old), kAtREmpty))) break;
+          copy(smem_u32(r_ring) + r * r_bytes, &r_map, 2 * p.v_units, p.r_chunks, smem_u32(&sh.r_full[r]));
+          if (++r == p.r_slots) r = 0;
         }
         for (int u = 0; u < p.v_units; ++u) {
-          if (!(ok = all_wait(&sh.v_empty[v], v_phase ^ 1, kAtVEmpty))) break;
-          copy(v_ring + v * kUnitBytes, 2 * u, 2, &sh.v_full[v]);
-          if (++v == p.v_slots) v = 0, v_phase ^= 1;
-        }
-        if (ok && tile == walk.t) {
-          // The queries of this segment, once the first products of the segment before are over.
-          if (segment > 0 && !(ok = all_wait(&sh.q_empty, (segment - 1) & 1, kAtQEmpty))) break;
-          if (lane == 0) {
-            mbar_expect_tx(smem_u32(&sh.q_full), chunks * HT * kRowBytes);
-            for (int i = 0; i < chunks; ++i)
-              tma_load_3d(smem_u32(q_smem) + i * HT * kRowBytes, &q_map, i * 64, head0, walk.b, smem_u32(&sh.q_full));
+          // (the first of the units that become free together, or of this tile, waits)
+          if (old_u >= 0 && (u == 0 || old_u == 0 || old_u == n1)) {
+            uint64_t* const freed = old_u < n1 ? &sh.pv_half[old_i % kTurns] : &sh.pv_done[old_i % kTurns];
+            if (!(ok = waits.wait_all(smem_u32(freed), turn_parity(old_i), kAtVEmpty))) break;
           }
+          if (++old_u == p.v_units) old_u = 0, ++old_i;
+          copy(smem_u32(v_ring) + v * kUnitBytes, &v_map, 2 * u, 2, smem_u32(&sh.v_full[v]));
+          if (++v == p.v_slots) v = 0;
         }
-        for (int k = 0; k < 2; ++k) page[k] = next_page[k], slot[k] = next_slot[k];
+        if (!ok) break;
+        if (tile == 0) {
+          // The queries of this segment, once the first products of the segment before are over.
+          if (segment > 0 && !(ok = waits.wait_all(smem_u32(&sh.q_empty), (segment - 1) & 1, kAtQEmpty))) break;
+          if (lane == 0) mbar_expect_tx(smem_u32(&sh.q_full), chunks * HT * kRowBytes);
+          __syncwarp();
+          tma_load_4d(smem_u32(q_smem), &q_map, head0, 0, walk.b, smem_u32(&sh.q_full));
+        }
+        place(walk.t + tile + 1);  // on its way during the waits
       }
       ++segment;
     }
-    if (sh.expired != 0 && lane == 0) {
-      // A wait has expired somewhere: no copy may still be in flight when the CTA ends. A slot's last copies belong to the phase
-      // that its barrier completed last or is in; waiting for the other parity returns at once where none are in flight.
-      auto drain = [&](uint64_t* bar, uint32_t parity) {
-        for (int i = 0; i < 1000 && !mbar_try_wait(smem_u32(bar), parity, 10000); ++i) {
-        }
+    if (__any_sync(0xffffffffu, sh.expired != 0) && lane == 0) {
+      // A wait has expired somewhere: no copy may still be in flight when the CTA ends. A phase that will not complete (a use that
+      // was not begun) runs out of its 10 ms.
+      auto drain = [&](uint64_t* bar) {
+        for (uint32_t parity = 0; parity < 2; ++parity)
+          for (int n = 0; n < 1000 && !mbar_try_wait(smem_u32(bar), parity, 10000); ++n) {
+          }
       };
-      for (int i = 0; i < p.v_slots; ++i) drain(&sh.v_full[i], i < v ? v_phase : v_phase ^ 1);
-      for (int i = 0; i < p.r_slots; ++i) drain(&sh.r_full[i], i < r ? r_phase : r_phase ^ 1);
-      for (uint32_t parity = 0; parity < 2; ++parity) drain(&sh.q_full, parity);
+      for (int n = 0; n < p.v_slots; ++n) drain(&sh.v_full[n]);
+      for (int n = 0; n < p.r_slots; ++n) drain(&sh.r_full[n]);
+      drain(&sh.q_full);
     }
     __syncwarp();
   } else if (warp == 5) {
-    if (lane == 0) {
-      constexpr uint32_t kType = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
-      constexpr uint32_t kIdesc = (1u << 4) | (kType << 7) | (kType << 10);
-      constexpr uint32_t kIdescS = kIdesc | (static_cast<uint32_t>(kTile >> 3) << 17) | (64u >> 4 << 24);
-      constexpr uint32_t kIdescO = kIdesc | (1u << 15) | (static_cast<uint32_t>(HT >> 3) << 17) | (128u >> 4 << 24);  // A is MN-major
-      constexpr uint32_t kHi = (1024u >> 4) | (1u << 14) | (2u << 29);
-      constexpr uint32_t kLoK = 1u << 16;                                             // K-major: no leading offset
-      constexpr uint32_t kLoV = static_cast<uint32_t>(kChunkBytes >> 4) << 16;        // MN-major: to the next 64 elements
-      const uint32_t q_lo = kLoK | (smem_u32(q_smem) >> 4), p_lo = kLoK | (smem_u32(p_smem) >> 4);
-      const uint32_t v_base = smem_u32(v_ring) >> 4, r_base = smem_u32(r_ring) >> 4;
-      int v = 0, r = 0, i = 0, segment = 0;
-      uint32_t v_phase = 0, r_phase = 0;
-      bool ok = sh.expired == 0;
-      // The second product that is still to be issued: of tile i - 1, whose value units begin at slot pv.
-      bool pending = false, pending_first = false;
-      int pv = 0, pv_segment = 0, pv_tile = 0;
-      auto second = [&]() {
-        pending = false;
-        if (pending_first && pv_segment > 0 && !(ok = waits.wait(smem_u32(&sh.o_free), (pv_segment - 1) & 1, kAtOFree))) return;
-        tcgen05_fence_after();
-        for (int u = 0; u < p.v_units; ++u) {
-          const uint32_t a = kLoV | (v_base + pv * (kUnitBytes >> 4));
+    // Products. All lanes walk along, and votes make the branches uniform: the operands of the instructions are then formed in
+    // uniform registers. With one lane walking alone, each instruction took 97 clocks to issue. (Two issuing warps, one for each
+    // product, were three times slower: the tensor core does not like the shapes to alternate.)
+    constexpr uint32_t kAll = 0xffffffffu;
+    constexpr uint32_t kType = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+    constexpr uint32_t kIdesc = (1u << 4) | (kType << 7) | (kType << 10);
+    constexpr uint32_t kIdescS = kIdesc | (static_cast<uint32_t>(kTile >> 3) << 17) | (64u >> 4 << 24);
+    constexpr uint32_t kIdescO = kIdesc | (1u << 15) | (static_cast<uint32_t>(HT >> 3) << 17) | (128u >> 4 << 24);  // A is MN-major
+    constexpr uint32_t kHi = (1u << 14) | (2u << 29);
+    constexpr uint32_t kHiDense = kHi | (kGroupBytes >> 4);      // queries and weights: groups of 8 rows one behind the other
+    constexpr uint32_t kHiValue = kHi | (2 * kGroupBytes >> 4);  // units of the value
+    constexpr uint32_t kLoK = 1u << 16;                                       // K-major: no leading offset
+    constexpr uint32_t kLoV = static_cast<uint32_t>(kGroupBytes >> 4) << 16;  // MN-major: to the next 64 elements
+    const uint32_t hi_rest = kHi | (p.r_chunks * kGroupBytes >> 4);
+    const uint32_t q_lo = kLoK | (smem_u32(q_smem) >> 4), p_lo = kLoK | (smem_u32(p_smem) >> 4);
+    const uint32_t v_at = smem_u32(v_ring) >> 4, r_at = smem_u32(r_ring) >> 4;
+    const uint32_t v_bar = smem_u32(&sh.v_full[0]), r_bar = smem_u32(&sh.r_full[0]), s_bar = smem_u32(&sh.s_free[0]);
+    int v = 0, r = 0, i = 0, segment = 0;
+    uint32_t v_phase = 0, r_phase = 0;
+    // The second product that is still to be issued, of the tile before, whose value units begin at slot pv.
+    bool pending = false, pending_first = false;
+    int pv = 0, pv_segment = 0;
+    // What the products need is looked at all at once, a barrier per lane: lanes 0 .. v_units - 1 the value units of the tile, lane 8
+    // the elements behind the value, 9 the buffer of S, 10 the queries, 30 and 31 what the pending second product needs (the
+    // accumulators read out, the weights). Both are issued as they can be, the second product first, because it frees the rings.
+    auto issue = [&](bool with_first, int tile) {
+      uint32_t bar = 0, parity = 0;
+      if (with_first) {
+        int slot = v + lane;
+        const bool wraps = slot >= p.v_slots;
+        slot = wraps ? slot - p.v_slots : slot;
+        bar = lane < p.v_units ? v_bar + 8 * slot : 0u;
+        parity = wraps ? v_phase ^ 1 : v_phase;
+        bar = lane == 8 && p.r_chunks > 0 ? r_bar + 8 * r : bar;
+        parity = lane == 8 ? r_phase : parity;
+        bar = lane == 9 ? s_bar + 8 * (i & 1) : bar;
+        parity = lane == 9 ? ((i >> 1) & 1) ^ 1 : parity;
+        bar = lane == 10 && tile == 0 ? smem_u32(&sh.q_full) : bar;
+        parity = lane == 10 ? segment & 1 : parity;
+      }
+      if (pending) {
+        bar = lane == 30 && pending_first && pv_segment > 0 ? smem_u32(&sh.o_free) : bar;
+        parity = lane == 30 ? (pv_segment - 1) & 1 : parity;
+        bar = lane == 31 ? smem_u32(&sh.p_full) : bar;
+        parity = lane == 31 ? (i - 1) & 1 : parity;
+      }
+      const uint32_t s = tmem + kTmemLogits + (i & 1) * kTile;
+      int u = with_first ? 0 : p.v_units;
+      bool began = false;
+      unsigned long long t0 = 0;  // (read late: reading the timer takes several hundred clocks)
+      for (uint32_t spins = 1; u < p.v_units || pending; ++spins) {
+        const uint32_t there = __ballot_sync(kAll, bar == 0 || mbar_test(bar, parity));
+        const uint32_t units = (there & 0x700u) == 0x700u && u < p.v_units ? there >> u & 1u : 0u;
+        if (pending && (there >> 30) == 3u) {
+          tcgen05_fence_after();
+          const int done = (i - 1) % kTurns;
+          for (int w = 0; w < p.v_units; ++w) {
+            const uint32_t a = kLoV | (v_at + pv * (kUnitBytes >> 4));
 #pragma unroll
-          for (int k = 0; k < kTile / 16; ++k)
-            umma_f16(tmem + u * HT, a + k * (16 * kRowBytes >> 4), p_lo + k * 2, kHi, kIdescO, !(pending_first && k == 0));
-          umma_commit(smem_u32(&sh.v_empty[pv]));
-          if (++pv == p.v_slots) pv = 0;
-        }
-        umma_commit(smem_u32(&sh.pv_done));
-      };
-      // Waits for `bar`; while it is not there, the second product goes out as soon as its weights are.
-      auto wait_or_second = [&](uint64_t* bar, uint32_t parity, int where) {
-        if (!pending) return waits.wait(smem_u32(bar), parity, where);
-        const unsigned long long t0 = global_ns();
-        for (uint32_t spins = 0; !mbar_test(smem_u32(bar), parity); ++spins) {
-          if (mbar_test(smem_u32(&sh.p_full), pv_tile & 1)) {
-            second();
-            return ok && waits.wait(smem_u32(bar), parity, where);
+            for (int k = 0; k < kTile / 16; ++k)
+              umma_f16(tmem + w * HT, a + k * (4 * kGroupBytes >> 4), kHiValue, p_lo + k * 2, kHiDense, kIdescO, k > 0 || !pending_first);
+            if (++pv == p.v_slots) pv = 0;
+            if (w + 1 == n1) umma_commit(smem_u32(&sh.pv_half[done]));
           }
-          if ((spins & 63u) == 63u && waits.give_up(t0, parity, where)) return false;
+          umma_commit(smem_u32(&sh.pv_done[done]));
+          pending = false;
+          bar = lane >= 30 ? 0u : bar;
+          spins = 0;
         }
-        return true;
-      };
-      Walk walk(sh);
-      while (ok && walk.next(p)) {
-        for (int tile = 0; ok && tile < walk.count; ++tile, ++i) {
-          const uint32_t s = tmem + kTmemLogits + (i & 1) * kTile;
-          if (!(ok = waits.wait(smem_u32(&sh.s_free[i & 1]), ((i >> 1) & 1) ^ 1, kAtSFree))) break;
-          if (tile == 0 && !(ok = wait_or_second(&sh.q_full, segment & 1, kAtQFull))) break;
-          uint32_t accumulate = 0;
-          auto first = [&](uint32_t rows, int chunk) {
-            const uint32_t a = q_lo + chunk * (HT * kRowBytes >> 4);
+        if (units != 0) {
+          tcgen05_fence_after();
+          if (!began) {
+            for (int n = 0; n < p.r_chunks; ++n) {
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              umma_f16(s, a + k * 2, (kLoK | rows) + k * 2, kHi, kIdescS, accumulate);
-              accumulate = 1;
+              for (int k = 0; k < 4; ++k)
+                umma_f16(s, q_lo + (2 * p.v_units + n) * (HT * kRowBytes >> 4) + k * 2, kHiDense,
+                         (kLoK | (r_at + r * (r_bytes >> 4))) + n * (kGroupBytes >> 4) + k * 2, hi_rest, kIdescS, n + k > 0);
             }
-          };
-          if (p.r_chunks > 0) {
-            if (!(ok = wait_or_second(&sh.r_full[r], r_phase, kAtRFull))) break;
-            tcgen05_fence_after();
-            for (int n = 0; n < p.r_chunks; ++n) first(r_base + (r * p.r_chunks + n) * (kChunkBytes >> 4), 2 * p.v_units + n);
-            umma_commit(smem_u32(&sh.r_empty[r]));
-            if (++r == p.r_slots) r = 0, r_phase ^= 1;
           }
-          const int v0 = v;
-          for (int u = 0; u < p.v_units; ++u) {
-            if (!(ok = wait_or_second(&sh.v_full[v], v_phase, kAtVFull))) break;
-            tcgen05_fence_after();
-            for (int n = 0; n < 2; ++n) first(v_base + v * (kUnitBytes >> 4) + n * (kChunkBytes >> 4), 2 * u + n);
+          for (; u < p.v_units && (there >> u & 1u) != 0; ++u) {
+            const uint32_t b = kLoK | (v_at + v * (kUnitBytes >> 4));
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+              umma_f16(s, q_lo + (2 * u + k / 4) * (HT * kRowBytes >> 4) + k % 4 * 2, kHiDense, b + k / 4 * (kGroupBytes >> 4) + k % 4 * 2,
+                       kHiValue, kIdescS, k > 0 || began || p.r_chunks > 0);
+            began = true;
             if (++v == p.v_slots) v = 0, v_phase ^= 1;
           }
-          if (!ok) break;
-          umma_commit(smem_u32(&sh.s_full[i & 1]));
-          if (tile == walk.count - 1) umma_commit(smem_u32(&sh.q_empty));
-          if (pending) {
-            if (!(ok = waits.wait(smem_u32(&sh.p_full), pv_tile & 1, kAtPFull))) break;
-            second();
-            if (!ok) break;
-          }
-          pending = true;
-          pending_first = tile == 0;
-          pv = v0;
-          pv_segment = segment;
-          pv_tile = i;
+          if (u == p.v_units) umma_commit(smem_u32(&sh.s_full[i % kTurns]));
+          spins = 0;
         }
-        ++segment;
+        if ((spins & 1023u) == 1023u) {
+          if (t0 == 0) t0 = global_ns();
+          if (__any_sync(kAll, waits.give_up(t0, static_cast<uint32_t>(i), kAtOperands))) return false;
+        }
       }
-      if (ok && pending && waits.wait(smem_u32(&sh.p_full), pv_tile & 1, kAtPFull)) second();
-      if (sh.expired != 0) {  // none in flight past here
-        umma_commit(smem_u32(&sh.drained));
-        for (int n = 0; n < 1000 && !mbar_try_wait(smem_u32(&sh.drained), 0, 10000); ++n) {
-        }
+      return true;
+    };
+    bool ok = __all_sync(kAll, sh.expired == 0);
+    Walk walk(sh);
+    while (ok && __all_sync(kAll, walk.next(p))) {
+      const int count = __shfl_sync(kAll, walk.count, 0);
+      for (int tile = 0; tile < count; ++tile, ++i) {
+        const int v0 = v;
+        if (!(ok = issue(true, tile))) break;
+        if (tile == count - 1) umma_commit(smem_u32(&sh.q_empty));
+        if (p.r_chunks > 0 && ++r == p.r_slots) r = 0, r_phase ^= 1;
+        pending = true;
+        pending_first = tile == 0;
+        pv = v0;
+        pv_segment = segment;
+      }
+      ++segment;
+    }
+    if (ok && pending) issue(false, 0);
+    if (__any_sync(kAll, sh.expired != 0)) {  // none in flight past here
+      umma_commit(smem_u32(&sh.drained));
+      for (int n = 0; n < 1000 && !mbar_try_wait(smem_u32(&sh.drained), 0, 10000); ++n) {
       }
     }
     __syncwarp();
@@ -685,7 +764,7 @@ attend_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__
     while (walk.next(p)) {
       float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
       for (int tile = 0; tile < walk.count; ++tile, ++i) {
-        wait(&sh.s_full[i & 1], (i >> 1) & 1, kAtSFull);
+        wait(&sh.s_full[i % kTurns], turn_parity(i), kAtSFull);
         tcgen05_fence_after();
         uint32_t x[32];
         if (active) tmem_ld_16x64(tmem + lanes + kTmemLogits + (i & 1) * kTile, x);
@@ -751,7 +830,7 @@ attend_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__
           }
         }
         // The weights before are read, and the accumulators at rest, once the second product of the tile before is over.
-        if (i > 0) wait(&sh.pv_done, (i - 1) & 1, kAtPvDone);
+        if (i > 0) wait(&sh.pv_done[(i - 1) % kTurns], turn_parity(i - 1), kAtPvDone);
         if (rescale) {
           softmax_sync();
           tcgen05_fence_after();
@@ -780,10 +859,11 @@ attend_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__
           // infinity or NaN would be NaN.
           int slot = v;
           for (int u = 0; u < p.v_units; ++u) {
-            for (int at = left * kRowBytes + tid * 16; at < kChunkBytes; at += kSoftmaxThreads * 16) {
-              uint8_t* to = v_ring + slot * kUnitBytes + at;
-              *reinterpret_cast<uint4*>(to) = make_uint4(0u, 0u, 0u, 0u);
-              *reinterpret_cast<uint4*>(to + kChunkBytes) = make_uint4(0u, 0u, 0u, 0u);
+            uint8_t* const unit = v_ring + slot * kUnitBytes;
+            for (int at = tid; at < (kTile - left) * 16; at += kSoftmaxThreads) {
+              const int row = left + at / 16, piece = at % 16;
+              *reinterpret_cast<uint4*>(unit + (row >> 3) * (2 * kGroupBytes) + (piece >> 3) * kGroupBytes + (row & 7) * kRowBytes + (piece & 7) * 16) =
+                  make_uint4(0u, 0u, 0u, 0u);
             }
             if (++slot == p.v_slots) slot = 0;
           }
@@ -809,7 +889,7 @@ attend_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__
         }
       }
       softmax_sync();
-      wait(&sh.pv_done, (i - 1) & 1, kAtPvDone);
+      wait(&sh.pv_done[(i - 1) % kTurns], turn_parity(i - 1), kAtPvDone);
       tcgen05_fence_after();
       const int heads = min(HT, p.heads - head0);
       if (walk.whole()) {
@@ -951,11 +1031,12 @@ __global__ void __launch_bounds__(kJoinThreads) attend_join_kernel(const __grid_
   }
 }
 
-// score_out = score + the weights of all heads, from the logits that the attention left: a CTA per tile, four groups of heads.
-constexpr int kScoreThreads = 4 * kTile;
+// score_out = score + the weights of all heads, from the logits that the attention left: a CTA per tile, a group of threads for every fourth head.
+constexpr int kScoreGroups = 4;
+constexpr int kScoreThreads = kScoreGroups * kTile;
 
 __global__ void __launch_bounds__(kScoreThreads) attend_score_kernel(const __grid_constant__ AttendParams p) {
-  __shared__ float sums[4][kTile];
+  __shared__ float sums[kScoreGroups][kTile];
   pdl_wait();
   pdl_launch_dependents();
   const int b = static_cast<int>(blockIdx.y), tile = static_cast<int>(blockIdx.x);
@@ -966,12 +1047,15 @@ __global__ void __launch_bounds__(kScoreThreads) attend_score_kernel(const __gri
   const float* lse2 = p.lse2 + static_cast<long long>(b) * p.heads;
   float sum = 0.f;
 #pragma unroll 4
-  for (int h = group; h < p.heads; h += 4) sum += exp2_fast(x[static_cast<long long>(h) * kTile] - lse2[h]);
+  for (int h = group; h < p.heads; h += kScoreGroups) sum += exp2_fast(x[static_cast<long long>(h) * kTile] - lse2[h]);
   sums[group][col] = sum;
   __syncthreads();
   const int j = tile * kTile + col;
-  if (group == 0 && j < rows)
-    p.score_out[b * p.score_out_stride + j] = p.score[b * p.score_stride + j] + ((sums[0][col] + sums[1][col]) + (sums[2][col] + sums[3][col]));
+  if (group == 0 && j < rows) {
+#pragma unroll
+    for (int k = 1; k < kScoreGroups; ++k) sum += sums[k][col];
+    p.score_out[b * p.score_out_stride + j] = p.score[b * p.score_stride + j] + sum;
+  }
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -1239,46 +1323,54 @@ AttendWorkspace attend_workspace(int batch, int heads, int dv, int max_len, bool
   return w;
 }
 
-// Ring slots: as many tiles as fit, the value in units that are freed one by one. Returns the shared memory of the CTA.
+// Ring slots: as many tiles as fit, and of the value's units whatever else does. Returns the shared memory of the CTA.
 size_t plan_rings(int ht, AttendParams* p) {
-  const int fixed = kHeaderBytes + (2 * p->v_units + p->r_chunks) * ht * kRowBytes + ht * kRowBytes;
-  const int r_bytes = p->r_chunks * kChunkBytes;
-  p->r_slots = p->r_chunks > 0 ? 2 : 0;
+  const int unit = 2 * kTile * kRowBytes, rest = p->r_chunks * kTile * kRowBytes;
+  const int fixed = kHeaderBytes + (2 * p->v_units + p->r_chunks + 1) * ht * kRowBytes;
   auto units = [&](int r) {
-    const int n = (kMaxSmem - fixed - r * r_bytes) / kUnitBytes;
+    const int n = (kMaxSmem - fixed - r * rest) / unit;
     return n < kMaxV ? n : kMaxV;
   };
-  while (p->r_chunks > 0 && p->r_slots < kMaxR && units(p->r_slots + 1) > p->v_units * p->r_slots) ++p->r_slots;
+  p->r_slots = rest > 0 ? 2 : 0;  // (two of the largest tiles fit next to 64 heads)
+  while (rest > 0 && p->r_slots < kMaxR && units(p->r_slots + 1) > p->v_units * p->r_slots) ++p->r_slots;
   p->v_slots = units(p->r_slots);
-  return static_cast<size_t>(fixed) + p->v_slots * kUnitBytes + p->r_slots * r_bytes;
+  return static_cast<size_t>(fixed) + p->v_slots * unit + p->r_slots * rest;
 }
 
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 
-// [outer][inner][d] of 16-bit elements, box: 64 elements of `rows` inner rows, 128-byte swizzle. What lies outside reads as 0.
-bool encode_rows(CUtensorMap* map, const void* base, bool bf16, int d, int inner, int outer, long long inner_stride, long long outer_stride,
-                 int rows) {
-  static const EncodeTiledFn fn = []() -> EncodeTiledFn {
-    void* ptr = nullptr;
-    cudaDriverEntryPointQueryResult found;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &found) != cudaSuccess || found != cudaDriverEntryPointSuccess) {
-      (void)cudaGetLastError();
-      return nullptr;
-    }
-    return reinterpret_cast<EncodeTiledFn>(ptr);
-  }();
-  if (fn == nullptr) return false;
-  const cuuint64_t dims[3] = {static_cast<cuuint64_t>(d), static_cast<cuuint64_t>(inner), static_cast<cuuint64_t>(outer)};
-  const cuuint64_t strides[2] = {static_cast<cuuint64_t>(inner_stride) * 2, static_cast<cuuint64_t>(outer_stride) * 2};
-  const cuuint32_t box[3] = {64, static_cast<cuuint32_t>(rows), 1}, steps[3] = {1, 1, 1};
-  return fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(base), dims, strides, box,
-            steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
+// A map of 16-bit elements, 128-byte swizzle, first dimension and box 64 elements. What lies outside reads as 0. Encoded for every
+// call: a map holds an address, and is not kept beyond the call that it was made for.
+struct MapDims {
+  int rank = 1;
+  cuuint64_t dims[5] = {64}, strides[4] = {};
+  cuuint32_t box[5] = {64};
+  void add(long long extent, long long stride, int box_extent) {
+    dims[rank] = static_cast<cuuint64_t>(extent);
+    strides[rank - 1] = static_cast<cuuint64_t>(stride) * 2;
+    box[rank++] = static_cast<cuuint32_t>(box_extent);
+  }
+  bool encode(CUtensorMap* map, const void* base, bool bf16) const {
+    static const EncodeTiledFn fn = []() -> EncodeTiledFn {
+      void* ptr = nullptr;
+      cudaDriverEntryPointQueryResult found;
+      if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &found) != cudaSuccess || found != cudaDriverEntryPointSuccess) {
+        (void)cudaGetLastError();
+        return nullptr;
+      }
+      return reinterpret_cast<EncodeTiledFn>(ptr);
+    }();
+    const cuuint32_t steps[5] = {1, 1, 1, 1, 1};
+    return fn != nullptr &&
+           fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, static_cast<cuuint32_t>(rank),
+              const_cast<void*>(base), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  }
+};
 
-typedef void (*AttendFn)(const CUtensorMap, const CUtensorMap, const AttendParams);
+typedef void (*AttendFn)(const CUtensorMap, const CUtensorMap, const CUtensorMap, const AttendParams);
 
 AttendFn attend_fn(bool bf16, int ht) {
   if (bf16) return ht == 16 ? attend_kernel<__nv_bfloat16, 16> : ht == 32 ? attend_kernel<__nv_bfloat16, 32> : attend_kernel<__nv_bfloat16, 64>;
@@ -1393,13 +1485,28 @@ int b200_mla_cache_attend(const b200_mla_cache* cache, const void* q, long long 
   p.status = device_status;
   const size_t smem = plan_rings(ht, &p);
   const bool bf16 = cache->dtype == B200_MLA_CACHE_BF16;
-  CUtensorMap q_map, row_map;
-  if (!encode_rows(&q_map, q, bf16, p.cache.d, heads, cache->batch, q_sh, q_sb, ht) ||
-      !encode_rows(&row_map, cache->data, bf16, p.cache.d, cache->page_size, cache->pages, cache->slot_stride, cache->page_stride, p.copy_rows))
-    return B200_FP8_MM_ERR_DRIVER;
+  CUtensorMap q_map, v_map, r_map;
+  const int chunks = p.cache.d / 64;
+  MapDims q_dims;
+  q_dims.add(heads, q_sh, ht);
+  q_dims.add(chunks, 64, chunks);
+  q_dims.add(cache->batch, q_sb, 1);
+  // Copies of whole groups of 8 rows bring all chunks of a unit; shorter ones (pages that no 8 divides) a chunk each.
+  auto row_dims = [&](int unit_chunks) {
+    const bool groups = p.copy_rows >= 8;
+    MapDims m;
+    m.add(groups ? 8 : cache->page_size, cache->slot_stride, groups ? 8 : p.copy_rows);
+    m.add(chunks, 64, groups ? unit_chunks : 1);
+    if (groups) m.add(cache->page_size / 8, 8 * cache->slot_stride, p.copy_rows / 8);
+    m.add(cache->pages, cache->page_stride, 1);
+    return m;
+  };
+  if (!q_dims.encode(&q_map, q, bf16) || !row_dims(2).encode(&v_map, cache->data, bf16)) return B200_FP8_MM_ERR_DRIVER;
+  r_map = v_map;
+  if (p.r_chunks != 0 && p.r_chunks != 2 && p.copy_rows >= 8 && !row_dims(p.r_chunks).encode(&r_map, cache->data, bf16)) return B200_FP8_MM_ERR_DRIVER;
   const AttendFn fn = attend_fn(bf16, ht);
   if (!opt_in(fn, bf16, ht, device)) return B200_FP8_MM_ERR_DRIVER;
-  rc = launch_pdl(fn, dim3(static_cast<unsigned>(p.workers) * p.head_tiles), kAttendThreads, smem, stream, q_map, row_map, p);
+  rc = launch_pdl(fn, dim3(static_cast<unsigned>(p.workers) * p.head_tiles), kAttendThreads, smem, stream, q_map, v_map, r_map, p);
   if (rc != B200_FP8_MM_OK) return rc;
   // CTAs for every SM a few times over, however few sequences there are; those of a sequence share its heads.
   const int each = (4 * sms + cache->batch - 1) / cache->batch;
