@@ -153,9 +153,7 @@ constexpr int kMaxD = 576;
 constexpr int kTile = cache_walk::kTileRows;   // rows of the cache per tile
 constexpr int kRowBytes = 128;                 // of a row that lie together under the 128-byte swizzle: a chunk of 64 elements
 constexpr int kGroupBytes = 8 * kRowBytes;     // 8 rows of a chunk, the swizzle's period
-constexpr int kMaxV = 15, kMaxR = 8;           // ring slots
-constexpr int kTurns = 16;                     // barriers of the products, one per tile in turn: a wait tells a phase's parity only,
-                                               // so there are more of them than tiles can be in the rings
+constexpr int kMaxStages = 12;
 constexpr int kSoftmaxThreads = 128;
 constexpr int kAttendThreads = kSoftmaxThreads + 64;
 constexpr int kHeaderBytes = 2048;             // barriers and small arrays, behind the rings
@@ -175,8 +173,8 @@ struct AttendParams {
   int heads, head_tiles, max_len, batch;
   int workers, least;      // workers per head tile, and the least tiles worth one
   int copy_rows;           // cache_walk::copy_rows(page_size)
-  int v_slots, r_slots;    // ring slots of a unit each: 128 elements of the value; all elements behind the value
-  int v_units, r_chunks;   // units of a tile; chunks behind the value
+  int stages;              // tiles of the ring
+  int v_units, chunks;     // 128-element units of the value; 64-element chunks of a row
   float scale_log2;        // scale * log2(e)
   // Workspace
   long long* first_tile;   // [batch + 1]: tiles before each sequence, and all
@@ -254,16 +252,18 @@ struct Waits {
   __device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, int where) const {
     return mbar_try_wait(bar, parity, 200000) || slow(bar, parity, where);
   }
-  // For a whole warp, which leaves together.
+  // For a whole warp, which leaves together: every lane has a barrier of its own (0: none).
+  __device__ __forceinline__ bool wait_lanes(uint32_t bar, uint32_t parity, int where) const {
+    if (__all_sync(0xffffffffu, bar == 0 || mbar_try_wait(bar, parity, 200000))) return true;
+    return __all_sync(0xffffffffu, bar == 0 || slow(bar, parity, where)) != 0;
+  }
+  // The same barrier for all.
   __device__ __forceinline__ bool wait_all(uint32_t bar, uint32_t parity, int where) const {
     return __all_sync(0xffffffffu, wait(bar, parity, where)) != 0;
   }
 };
 
-enum Where { kAtVEmpty = 0x201, kAtREmpty, kAtQEmpty, kAtOperands, kAtSFull, kAtPvDone };
-
-// A barrier that takes turns with others of its kind: parity of the phase that its use for tile i completes.
-__device__ __forceinline__ uint32_t turn_parity(int i) { return static_cast<uint32_t>(i / kTurns) & 1u; }
+enum Where { kAtFree = 0x201, kAtQEmpty, kAtOperands, kAtWeights, kAtSFull, kAtPvDone };
 
 // Copies for a whole warp, which comes here together: one lane issues.
 __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, int c1, int c2, int c3, uint32_t bar) {
@@ -293,21 +293,31 @@ __device__ __forceinline__ void tma_load_4d_own(uint32_t dst, const CUtensorMap*
 __device__ __forceinline__ void tcgen05_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tcgen05_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
-// Matrix descriptors as 32-bit halves, as in the GEMM: low word address and leading offset, high word stride offset, version
-// and the 128-byte swizzle. Only the address changes between instructions. The whole warp comes here and one lane of it, always
-// the same, issues.
-__device__ __forceinline__ void umma_f16(uint32_t d, uint32_t a_lo, uint32_t a_hi, uint32_t b_lo, uint32_t b_hi, uint32_t idesc,
-                                         uint32_t accumulate) {
+// Four products along K into one accumulator, a_step (of 16 bytes) of A and 32 bytes of B from one to the next. Matrix descriptors as
+// 32-bit halves, as in the GEMM: low word address and leading offset, high word stride offset, version and the 128-byte swizzle.
+// The whole warp comes here and one lane of it, always the same, issues. One statement for four, and rolled loops around it: a warp
+// that issues from unrolled code is held up by its instruction fetch (56 clocks a product against 30).
+__device__ __forceinline__ void umma_f16_x4(uint32_t d, uint32_t a_lo, uint32_t a_hi, uint32_t a_step, uint32_t b_lo, uint32_t b_hi,
+                                            uint32_t idesc, uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p, leader;\n\t.reg .b64 da, db;\n\t"
+      "{\n\t.reg .pred p, leader, yes;\n\t.reg .b64 da, db;\n\t.reg .b32 la, lb;\n\t"
       "elect.sync _|leader, 0xffffffff;\n\t"
+      "setp.ne.b32 p, %6, 0;\n\t"
+      "setp.eq.b32 yes, 0, 0;\n\t"
       "mov.b64 da, {%1, %2};\n\t"
       "mov.b64 db, {%3, %4};\n\t"
-      "setp.ne.b32 p, %6, 0;\n\t"
-      "@leader tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %5, p;\n\t}" ::"r"(d),
-      "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate)
+      "@leader tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %5, p;\n\t"
+      "add.u32 la, %1, %7;\n\tadd.u32 lb, %3, 2;\n\tmov.b64 da, {la, %2};\n\tmov.b64 db, {lb, %4};\n\t"
+      "@leader tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %5, yes;\n\t"
+      "add.u32 la, la, %7;\n\tadd.u32 lb, %3, 4;\n\tmov.b64 da, {la, %2};\n\tmov.b64 db, {lb, %4};\n\t"
+      "@leader tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %5, yes;\n\t"
+      "add.u32 la, la, %7;\n\tadd.u32 lb, %3, 6;\n\tmov.b64 da, {la, %2};\n\tmov.b64 db, {lb, %4};\n\t"
+      "@leader tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %5, yes;\n\t}" ::"r"(d),
+      "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate), "r"(a_step)
       : "memory");
 }
+static_assert(kTile == 64, "four products along a tile's rows");
+
 __device__ __forceinline__ void umma_commit(uint32_t bar) {
   asm volatile(
       "{\n\t.reg .pred leader;\n\t"
@@ -339,6 +349,21 @@ __device__ __forceinline__ void tmem_ld_32x16(uint32_t taddr, uint32_t (&v)[16])
       "tcgen05.wait::ld.sync.aligned;"
       : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
         "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_ld_32(uint32_t taddr, uint32_t (&v)[16]) { tmem_ld_32x16(taddr, v); }
+// 32 lanes x 32 columns.
+__device__ __forceinline__ void tmem_ld_32(uint32_t taddr, uint32_t (&v)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
+        "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]),
+        "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]),
+        "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
       : "r"(taddr)
       : "memory");
 }
@@ -382,21 +407,17 @@ __device__ __forceinline__ bool softmax_any(bool mine) {
 
 // What the roles of a CTA share, at the end of its shared memory.
 struct alignas(8) AttendShared {
-  uint64_t v_full[kMaxV], r_full[kMaxR];  // a unit is there
-  uint64_t s_full[kTurns];   // a tile's first product is done: its elements behind the value are free
-  uint64_t pv_half[kTurns];  // the second product is done with the first half of the tile's value units
-  uint64_t pv_done[kTurns];  // and with all
-  uint64_t q_full, q_empty, s_free[2], p_full, o_free, drained;
-  float factor[64];   // by which a head's accumulators are multiplied when its maximum is replaced
-  float inverse[64];  // 1 / sum of weights
-  float2 stat[64];
+  uint64_t full[kMaxStages], pv_done[kMaxStages];  // a tile is there; the second product is done with it
+  uint64_t s_full[2], s_free[2], p_full, q_full, q_empty, o_free, drained;
+  float factor[2][64];  // by which a head's accumulators are multiplied when its maximum is replaced; tiles take turns
+  float2 stat[64];      // maximum and sum of weights of a head
+  float inverse[64];    // 1 / sum
   long long sums[kAttendThreads / 32];
   long long share, share_end;
   uint32_t tmem_base;
   int expired, first_seq, first_tile;
 };
 static_assert(sizeof(AttendShared) <= kHeaderBytes, "the header is too small");
-static_assert(kTurns > kMaxV && kTurns > kMaxR, "a phase could be taken for one two turns before it");
 
 // A worker's walk over its share: segment after segment, each a run of tiles of one sequence.
 struct Walk {
@@ -432,10 +453,11 @@ struct Walk {
 // With the value's elements in the lanes, the accumulators of 64 heads take 256 of the 512 TMEM columns; with the heads in the
 // lanes, 128 heads would take them all and leave none for S. Fewer heads shrink N (16 or 32) and what Q takes of shared memory.
 //
-// A tile comes in units of 128 elements of the value (and one of what lies behind it), each in shared memory as [8 groups of
-// rows][chunk of 64 elements][8 rows x 128 bytes]: one stride from group to group for both operands, and one copy brings a unit of as
-// many rows as lie together in a page. The first product takes units as they come, the second one frees them half a tile at a time, so
-// that a slot is on its way to being filled again while the rest of its tile is still in use.
+// A tile lies in shared memory as [8 groups of rows][chunk of 64 elements][8 rows x 128 bytes]: one stride from group to group and one
+// from chunk to chunk for both operands, and one copy brings all chunks of as many rows as lie together in a page, up to half a tile.
+// What bounds the loop is how long a tile stays, from its copy's way through memory over both products and the softmax between them,
+// and what fits next to Q; so the second product goes by halves of the rows and frees each for its next copy. (Tiles of 32 rows, more
+// of them in flight, are slower: an MMA takes 27 clocks to issue however small it is.)
 //
 // One CTA per SM and worker: warp 4 copies, warp 5 issues the products, warps 0 to 3 do the softmax (S comes as 16 x 256-bit
 // fragments, 4 threads to a head) and the epilogue. S is double buffered; the next tile's first product runs under this tile's
@@ -444,32 +466,27 @@ struct Walk {
 // product, as matrix operands have to be.
 template <typename T, int HT>
 __global__ void __launch_bounds__(kAttendThreads, 1)
-attend_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap v_map, const __grid_constant__ CUtensorMap r_map,
-              const __grid_constant__ AttendParams p) {
+attend_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap row_map, const __grid_constant__ AttendParams p) {
   extern __shared__ __align__(1024) uint8_t smem[];
   const CacheView& c = p.cache;
-  constexpr int kUnitBytes = 2 * kTile * kRowBytes;
-  const int chunks = 2 * p.v_units + p.r_chunks, r_bytes = p.r_chunks * kTile * kRowBytes;
+  const int group_bytes = p.chunks * kGroupBytes, tile_bytes = kTile / 8 * group_bytes;
   uint8_t* const q_smem = smem;  // [chunk][HT rows x 128 bytes]; the first product reads 64 rows, those behind HT are never looked at
-  uint8_t* const v_ring = q_smem + chunks * HT * kRowBytes;
-  uint8_t* const r_ring = v_ring + p.v_slots * kUnitBytes;
-  uint8_t* const p_smem = r_ring + p.r_slots * r_bytes;
+  uint8_t* const ring = q_smem + p.chunks * HT * kRowBytes;
+  uint8_t* const p_smem = ring + p.stages * tile_bytes;
   AttendShared& sh = *reinterpret_cast<AttendShared*>(p_smem + HT * kRowBytes);
   const int tid = static_cast<int>(threadIdx.x), warp = tid >> 5, lane = tid & 31;
   const int head_tile = static_cast<int>(blockIdx.x) % p.head_tiles, worker = static_cast<int>(blockIdx.x) / p.head_tiles;
   const int head0 = head_tile * HT;
   const Waits waits{&sh.expired, p.status};
   if (tid == 0) {
-    for (int i = 0; i < kMaxV; ++i) mbar_init(smem_u32(&sh.v_full[i]), 1);
-    for (int i = 0; i < kMaxR; ++i) mbar_init(smem_u32(&sh.r_full[i]), 1);
-    for (int i = 0; i < kTurns; ++i) {
-      mbar_init(smem_u32(&sh.s_full[i]), 1);
-      mbar_init(smem_u32(&sh.pv_half[i]), 1);
+    for (int i = 0; i < kMaxStages; ++i) {
+      mbar_init(smem_u32(&sh.full[i]), 1);
       mbar_init(smem_u32(&sh.pv_done[i]), 1);
     }
     mbar_init(smem_u32(&sh.q_full), 1);
     mbar_init(smem_u32(&sh.q_empty), 1);
     for (int i = 0; i < 2; ++i) {
+      mbar_init(smem_u32(&sh.s_full[i]), 1);
       mbar_init(smem_u32(&sh.s_free[i]), 4);
     }
     mbar_init(smem_u32(&sh.p_full), 4);
@@ -478,8 +495,7 @@ attend_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__
     sh.expired = (smem_u32(smem) & 1023u) != 0;  // the swizzle needs it; never so with no static shared memory before it
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&q_map) : "memory");
-    asm volatile("prefetch.tensormap [%0];" ::"l"(&v_map) : "memory");
-    if (p.r_chunks > 0) asm volatile("prefetch.tensormap [%0];" ::"l"(&r_map) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&row_map) : "memory");
   }
   if (warp == 5) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem_base)), "r"(kTmemCols) : "memory");
@@ -502,7 +518,8 @@ attend_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__
   tcgen05_fence_before();
   __syncthreads();
   tcgen05_fence_after();
-  const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(&sh.tmem_base);
+  constexpr uint32_t tmem = 0;  // all columns are this CTA's, so they begin at the first (checked below)
+  if (tid == 0 && sh.tmem_base != tmem) sh.expired = 1;
   {
     long long before = upto - mine, tiles = 0;
     for (int w = 0; w < kAttendThreads / 32; ++w) {
@@ -537,13 +554,12 @@ attend_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__
   }
   __syncthreads();
 
-  const int n1 = p.v_units / 2;  // units of the first half
   if (warp == 4) {
     // Copies. Lane l knows where pieces l and l + 32 (copy_rows rows each) of a tile come from.
     const int pieces = kTile / p.copy_rows;
-    int v = 0, r = 0, segment = 0, i = 0;
-    int old_i = 0, old_u = -p.v_slots;  // the unit that was in the slot to be filled: none while negative
-    bool ok = __all_sync(0xffffffffu, sh.expired == 0);
+    int stage = 0, segment = 0;
+    uint32_t lap = 0;  // parity of the ring's current use
+    bool first_lap = true, ok = __all_sync(0xffffffffu, sh.expired == 0);
     Walk walk(sh);
     while (ok && __all_sync(0xffffffffu, walk.next(p))) {
       const int* table = c.block_table + walk.b * c.table_stride;
@@ -565,46 +581,29 @@ attend_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__
       };
       place(walk.t);
       const int count = __shfl_sync(0xffffffffu, walk.count, 0);
-      for (int tile = 0; ok && tile < count; ++tile, ++i) {
-        // `n` chunks from `chunk` on of the tile's rows
-        auto copy = [&](uint32_t to, const CUtensorMap* map, int chunk, int n, uint32_t full) {
-          if (lane == 0) mbar_expect_tx(full, n * kTile * kRowBytes);
-          __syncwarp();
-          if (p.copy_rows >= 8) {
-            for (int k = 0; k < pieces; ++k)
-              tma_load_5d(to + k * (p.copy_rows >> 3) * n * kGroupBytes, map, 0, chunk, __shfl_sync(0xffffffffu, slot[0], k) >> 3,
-                          __shfl_sync(0xffffffffu, page[0], k), full);
-          } else {
+      for (int tile = 0; ok && tile < count; ++tile) {
+        const uint32_t full = smem_u32(&sh.full[stage]), to = smem_u32(ring) + stage * tile_bytes;
+        if (!first_lap && !(ok = waits.wait_all(smem_u32(&sh.pv_done[stage]), lap ^ 1, kAtFree))) break;
+        if (lane == 0) mbar_expect_tx(full, tile_bytes);
+        __syncwarp();
+        if (p.copy_rows >= 8) {
+          for (int i = 0; i < pieces; ++i)
+            tma_load_5d(to + i * (p.copy_rows >> 3) * group_bytes, &row_map, 0, 0, __shfl_sync(0xffffffffu, slot[0], i) >> 3,
+                        __shfl_sync(0xffffffffu, page[0], i), full);
+        } else {
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
-              const int piece = lane + 32 * k, row = piece * p.copy_rows;
-              if (piece < pieces)
-                for (int m = 0; m < n; ++m)
-                  tma_load_4d_own(to + ((row >> 3) * n + m) * kGroupBytes + (row & 7) * kRowBytes, map, slot[k], chunk + m, page[k], full);
-            }
+          for (int k = 0; k < 2; ++k) {
+            const int piece = lane + 32 * k, row = piece * p.copy_rows;
+            if (piece < pieces)
+              for (int i = 0; i < p.chunks; ++i)
+                tma_load_4d_own(to + (row >> 3) * group_bytes + i * kGroupBytes + (row & 7) * kRowBytes, &row_map, slot[k], i, page[k], full);
           }
-        };
-        if (p.r_chunks > 0) {
-          const int old = i - p.r_slots;
-          if (old >= 0 && !(ok = waits.wait_all(smem_u32(&sh.s_full[old % kTurns]), turn_parity(old), kAtREmpty))) break;
-          copy(smem_u32(r_ring) + r * r_bytes, &r_map, 2 * p.v_units, p.r_chunks, smem_u32(&sh.r_full[r]));
-          if (++r == p.r_slots) r = 0;
         }
-        for (int u = 0; u < p.v_units; ++u) {
-          // (the first of the units that become free together, or of this tile, waits)
-          if (old_u >= 0 && (u == 0 || old_u == 0 || old_u == n1)) {
-            uint64_t* const freed = old_u < n1 ? &sh.pv_half[old_i % kTurns] : &sh.pv_done[old_i % kTurns];
-            if (!(ok = waits.wait_all(smem_u32(freed), turn_parity(old_i), kAtVEmpty))) break;
-          }
-          if (++old_u == p.v_units) old_u = 0, ++old_i;
-          copy(smem_u32(v_ring) + v * kUnitBytes, &v_map, 2 * u, 2, smem_u32(&sh.v_full[v]));
-          if (++v == p.v_slots) v = 0;
-        }
-        if (!ok) break;
+        if (++stage == p.stages) stage = 0, lap ^= 1, first_lap = false;
         if (tile == 0) {
           // The queries of this segment, once the first products of the segment before are over.
           if (segment > 0 && !(ok = waits.wait_all(smem_u32(&sh.q_empty), (segment - 1) & 1, kAtQEmpty))) break;
-          if (lane == 0) mbar_expect_tx(smem_u32(&sh.q_full), chunks * HT * kRowBytes);
+          if (lane == 0) mbar_expect_tx(smem_u32(&sh.q_full), p.chunks * HT * kRowBytes);
           __syncwarp();
           tma_load_4d(smem_u32(q_smem), &q_map, head0, 0, walk.b, smem_u32(&sh.q_full));
         }
@@ -620,8 +619,7 @@ attend_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__
           for (int n = 0; n < 1000 && !mbar_try_wait(smem_u32(bar), parity, 10000); ++n) {
           }
       };
-      for (int n = 0; n < p.v_slots; ++n) drain(&sh.v_full[n]);
-      for (int n = 0; n < p.r_slots; ++n) drain(&sh.r_full[n]);
+      for (int n = 0; n < p.stages; ++n) drain(&sh.full[n]);
       drain(&sh.q_full);
     }
     __syncwarp();
@@ -636,111 +634,83 @@ attend_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__
     constexpr uint32_t kIdescO = kIdesc | (1u << 15) | (static_cast<uint32_t>(HT >> 3) << 17) | (128u >> 4 << 24);  // A is MN-major
     constexpr uint32_t kHi = (1u << 14) | (2u << 29);
     constexpr uint32_t kHiDense = kHi | (kGroupBytes >> 4);      // queries and weights: groups of 8 rows one behind the other
-    constexpr uint32_t kHiValue = kHi | (2 * kGroupBytes >> 4);  // units of the value
     constexpr uint32_t kLoK = 1u << 16;                                       // K-major: no leading offset
     constexpr uint32_t kLoV = static_cast<uint32_t>(kGroupBytes >> 4) << 16;  // MN-major: to the next 64 elements
-    const uint32_t hi_rest = kHi | (p.r_chunks * kGroupBytes >> 4);
-    const uint32_t q_lo = kLoK | (smem_u32(q_smem) >> 4), p_lo = kLoK | (smem_u32(p_smem) >> 4);
-    const uint32_t v_at = smem_u32(v_ring) >> 4, r_at = smem_u32(r_ring) >> 4;
-    const uint32_t v_bar = smem_u32(&sh.v_full[0]), r_bar = smem_u32(&sh.r_full[0]), s_bar = smem_u32(&sh.s_free[0]);
-    int v = 0, r = 0, i = 0, segment = 0;
-    uint32_t v_phase = 0, r_phase = 0;
-    // The second product that is still to be issued, of the tile before, whose value units begin at slot pv.
+    const uint32_t hi_rows = kHi | (group_bytes >> 4);
+    const uint32_t q_lo = kLoK | (smem_u32(q_smem) >> 4), p_lo = kLoK | (smem_u32(p_smem) >> 4), ring_at = smem_u32(ring) >> 4;
+    // One value for the warp, in a uniform register.
+    auto uniform = [](uint32_t v) { return __reduce_max_sync(kAll, v); };
+    int stage = 0, i = 0, segment = 0;
+    uint32_t lap = 0;
+    // The second product that is still to be issued, of the tile before.
     bool pending = false, pending_first = false;
-    int pv = 0, pv_segment = 0;
-    // What the products need is looked at all at once, a barrier per lane: lanes 0 .. v_units - 1 the value units of the tile, lane 8
-    // the elements behind the value, 9 the buffer of S, 10 the queries, 30 and 31 what the pending second product needs (the
-    // accumulators read out, the weights). Both are issued as they can be, the second product first, because it frees the rings.
-    auto issue = [&](bool with_first, int tile) {
-      uint32_t bar = 0, parity = 0;
-      if (with_first) {
-        int slot = v + lane;
-        const bool wraps = slot >= p.v_slots;
-        slot = wraps ? slot - p.v_slots : slot;
-        bar = lane < p.v_units ? v_bar + 8 * slot : 0u;
-        parity = wraps ? v_phase ^ 1 : v_phase;
-        bar = lane == 8 && p.r_chunks > 0 ? r_bar + 8 * r : bar;
-        parity = lane == 8 ? r_phase : parity;
-        bar = lane == 9 ? s_bar + 8 * (i & 1) : bar;
-        parity = lane == 9 ? ((i >> 1) & 1) ^ 1 : parity;
-        bar = lane == 10 && tile == 0 ? smem_u32(&sh.q_full) : bar;
-        parity = lane == 10 ? segment & 1 : parity;
+    int pv_stage = 0, pv_segment = 0;
+    auto second = [&]() {
+      tcgen05_fence_after();
+      uint32_t values = uniform(kLoV | (ring_at + pv_stage * (tile_bytes >> 4))), o = tmem;
+#pragma unroll 1
+      for (int u = 0; u < p.v_units; ++u, values += 2 * kGroupBytes >> 4, o += HT)
+        umma_f16_x4(o, values, hi_rows, 2 * group_bytes >> 4, p_lo, kHiDense, kIdescO, pending_first ? 0u : 1u);
+      umma_commit(smem_u32(&sh.pv_done[pv_stage]));
+      pending = false;
+    };
+    // Waits for what the next products need, a barrier per lane: the first product of this tile for its rows (lane 0), a buffer of S (1)
+    // and the queries (2), the second product of the tile before for the weights (3) and, where it begins a segment, for the
+    // accumulators of the one before to have been read (4). Issues the second one if it can go and the first cannot; returns when
+    // the first can.
+    auto ready = [&](int tile) {
+      const bool fresh = pending_first && pv_segment > 0;
+      uint32_t bar = lane == 0 ? smem_u32(&sh.full[stage])
+                     : lane == 1 ? smem_u32(&sh.s_free[i & 1])
+                     : lane == 2 && tile == 0 ? smem_u32(&sh.q_full) : 0u;
+      uint32_t parity = lane == 0 ? lap : lane == 1 ? ((i >> 1) & 1) ^ 1 : segment & 1;
+      if (pending && lane >= 3) {
+        bar = lane == 3 ? smem_u32(&sh.p_full) : lane == 4 && fresh ? smem_u32(&sh.o_free) : 0u;
+        parity = static_cast<uint32_t>(lane == 3 ? i - 1 : pv_segment - 1) & 1u;
       }
-      if (pending) {
-        bar = lane == 30 && pending_first && pv_segment > 0 ? smem_u32(&sh.o_free) : bar;
-        parity = lane == 30 ? (pv_segment - 1) & 1 : parity;
-        bar = lane == 31 ? smem_u32(&sh.p_full) : bar;
-        parity = lane == 31 ? (i - 1) & 1 : parity;
-      }
-      const uint32_t s = tmem + kTmemLogits + (i & 1) * kTile;
-      int u = with_first ? 0 : p.v_units;
-      bool began = false;
       unsigned long long t0 = 0;  // (read late: reading the timer takes several hundred clocks)
-      for (uint32_t spins = 1; u < p.v_units || pending; ++spins) {
+      for (uint32_t spins = 1;; ++spins) {
         const uint32_t there = __ballot_sync(kAll, bar == 0 || mbar_test(bar, parity));
-        const uint32_t units = (there & 0x700u) == 0x700u && u < p.v_units ? there >> u & 1u : 0u;
-        if (pending && (there >> 30) == 3u) {
-          tcgen05_fence_after();
-          const int done = (i - 1) % kTurns;
-          for (int w = 0; w < p.v_units; ++w) {
-            const uint32_t a = kLoV | (v_at + pv * (kUnitBytes >> 4));
-#pragma unroll
-            for (int k = 0; k < kTile / 16; ++k)
-              umma_f16(tmem + w * HT, a + k * (4 * kGroupBytes >> 4), kHiValue, p_lo + k * 2, kHiDense, kIdescO, k > 0 || !pending_first);
-            if (++pv == p.v_slots) pv = 0;
-            if (w + 1 == n1) umma_commit(smem_u32(&sh.pv_half[done]));
-          }
-          umma_commit(smem_u32(&sh.pv_done[done]));
-          pending = false;
-          bar = lane >= 30 ? 0u : bar;
-          spins = 0;
-        }
-        if (units != 0) {
-          tcgen05_fence_after();
-          if (!began) {
-            for (int n = 0; n < p.r_chunks; ++n) {
-#pragma unroll
-              for (int k = 0; k < 4; ++k)
-                umma_f16(s, q_lo + (2 * p.v_units + n) * (HT * kRowBytes >> 4) + k * 2, kHiDense,
-                         (kLoK | (r_at + r * (r_bytes >> 4))) + n * (kGroupBytes >> 4) + k * 2, hi_rest, kIdescS, n + k > 0);
-            }
-          }
-          for (; u < p.v_units && (there >> u & 1u) != 0; ++u) {
-            const uint32_t b = kLoK | (v_at + v * (kUnitBytes >> 4));
-#pragma unroll
-            for (int k = 0; k < 8; ++k)
-              umma_f16(s, q_lo + (2 * u + k / 4) * (HT * kRowBytes >> 4) + k % 4 * 2, kHiDense, b + k / 4 * (kGroupBytes >> 4) + k % 4 * 2,
-                       kHiValue, kIdescS, k > 0 || began || p.r_chunks > 0);
-            began = true;
-            if (++v == p.v_slots) v = 0, v_phase ^= 1;
-          }
-          if (u == p.v_units) umma_commit(smem_u32(&sh.s_full[i % kTurns]));
-          spins = 0;
-        }
-        if ((spins & 1023u) == 1023u) {
+        if ((there & 7u) == 7u) return true;
+        if (pending && (there & 0x18u) == 0x18u) second();
+        if ((spins & 255u) == 0) {
           if (t0 == 0) t0 = global_ns();
-          if (__any_sync(kAll, waits.give_up(t0, static_cast<uint32_t>(i), kAtOperands))) return false;
+          if (__any_sync(kAll, waits.give_up(t0, parity, kAtOperands))) return false;
         }
       }
-      return true;
+    };
+    auto weights = [&]() {
+      const uint32_t bar = lane == 0 ? smem_u32(&sh.p_full) : lane == 1 && pending_first && pv_segment > 0 ? smem_u32(&sh.o_free) : 0u;
+      return waits.wait_lanes(bar, static_cast<uint32_t>(lane == 0 ? i - 1 : pv_segment - 1) & 1u, kAtWeights);
     };
     bool ok = __all_sync(kAll, sh.expired == 0);
     Walk walk(sh);
     while (ok && __all_sync(kAll, walk.next(p))) {
       const int count = __shfl_sync(kAll, walk.count, 0);
-      for (int tile = 0; tile < count; ++tile, ++i) {
-        const int v0 = v;
-        if (!(ok = issue(true, tile))) break;
+      for (int tile = 0; tile < count; ++tile) {
+        if (!(ok = ready(tile))) break;
+        tcgen05_fence_after();
+        const uint32_t s = uniform(tmem + kTmemLogits + (i & 1) * kTile);
+        uint32_t rows = uniform(kLoK | (ring_at + stage * (tile_bytes >> 4))), q_at = q_lo;
+#pragma unroll 1
+        for (int n = 0; n < p.chunks; ++n, q_at += HT * kRowBytes >> 4, rows += kGroupBytes >> 4)
+          umma_f16_x4(s, q_at, kHiDense, 2, rows, hi_rows, kIdescS, n > 0);
+        umma_commit(smem_u32(&sh.s_full[i & 1]));
         if (tile == count - 1) umma_commit(smem_u32(&sh.q_empty));
-        if (p.r_chunks > 0 && ++r == p.r_slots) r = 0, r_phase ^= 1;
+        if (pending) {
+          if (!(ok = weights())) break;
+          second();
+        }
+        ++i;
         pending = true;
         pending_first = tile == 0;
-        pv = v0;
+        pv_stage = stage;
         pv_segment = segment;
+        if (++stage == p.stages) stage = 0, lap ^= 1;
       }
       ++segment;
     }
-    if (ok && pending) issue(false, 0);
+    if (ok && pending && weights()) second();
     if (__any_sync(kAll, sh.expired != 0)) {  // none in flight past here
       umma_commit(smem_u32(&sh.drained));
       for (int n = 0; n < 1000 && !mbar_try_wait(smem_u32(&sh.drained), 0, 10000); ++n) {
@@ -752,7 +722,12 @@ attend_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__
     const bool active = 16 * warp < HT;
     const int row0 = 16 * warp + lane / 4, row1 = row0 + 8;
     const uint32_t lanes = static_cast<uint32_t>(32 * warp) << 16;
-    int i = 0, v = 0;
+    // The tile's place in the ring, and that of the tile before it, whose second product is waited for.
+    struct Place {
+      int stage;
+      uint32_t lap;
+    } here = {0, 0}, before = {0, 0};
+    int i = 0;
     bool ok = sh.expired == 0;
     // A wait that has expired does not end this role, because the other warps meet it at the barriers below: the rest of the walk
     // goes by without waiting, over whatever is there.
@@ -764,7 +739,7 @@ attend_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__
     while (walk.next(p)) {
       float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
       for (int tile = 0; tile < walk.count; ++tile, ++i) {
-        wait(&sh.s_full[i % kTurns], turn_parity(i), kAtSFull);
+        wait(&sh.s_full[i & 1], (i >> 1) & 1, kAtSFull);
         tcgen05_fence_after();
         uint32_t x[32];
         if (active) tmem_ld_16x64(tmem + lanes + kTmemLogits + (i & 1) * kTile, x);
@@ -773,13 +748,21 @@ attend_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__
         if (lane == 0) mbar_arrive(smem_u32(&sh.s_free[i & 1]));
         const int left = walk.rows - (walk.t + tile) * kTile;  // rows that exist from this tile on
         float t0 = -INFINITY, t1 = -INFINITY;
+        bool up = false;
         if (active) {
+          if (left >= kTile) {
+#pragma unroll
+            for (int n = 0; n < 32; ++n) x[n] = __float_as_uint(__uint_as_float(x[n]) * p.scale_log2);
+          } else {
+#pragma unroll
+            for (int n = 0; n < 32; ++n) {
+              const int col = 8 * (n / 4) + 2 * (lane % 4) + (n & 1);
+              x[n] = __float_as_uint(col < left ? __uint_as_float(x[n]) * p.scale_log2 : -INFINITY);
+            }
+          }
 #pragma unroll
           for (int n = 0; n < 32; ++n) {
-            const int col = 8 * (n / 4) + 2 * (lane % 4) + (n & 1);
-            const float xs = col < left ? __uint_as_float(x[n]) * p.scale_log2 : -INFINITY;
-            x[n] = __float_as_uint(xs);
-            if (n & 2) t1 = fmaxf(t1, xs); else t0 = fmaxf(t0, xs);
+            if (n & 2) t1 = fmaxf(t1, __uint_as_float(x[n])); else t0 = fmaxf(t0, __uint_as_float(x[n]));
           }
           if (p.logits != nullptr) {
             float* to = p.logits + ((static_cast<long long>(walk.b) * p.logit_tiles + walk.t + tile) * p.heads + head0) * kTile + 2 * (lane % 4);
@@ -796,29 +779,23 @@ attend_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__
             t0 = fmaxf(t0, __shfl_xor_sync(0xffffffffu, t0, o));
             t1 = fmaxf(t1, __shfl_xor_sync(0xffffffffu, t1, o));
           }
-        }
-        bool rescale = false;
-        __syncwarp();
-        if (tile == 0) {
-          m0 = t0;
-          m1 = t1;
-        } else {
-          const bool up0 = active && t0 > m0 + kRescaleAbove, up1 = active && t1 > m1 + kRescaleAbove;
-          rescale = softmax_any(up0 || up1);
-          if (rescale && active) {
-            const float f0 = up0 ? exp2_fast(m0 - t0) : 1.f, f1 = up1 ? exp2_fast(m1 - t1) : 1.f;
-            if (up0) m0 = t0;
-            if (up1) m1 = t1;
+          float f0 = 1.f, f1 = 1.f;
+          if (tile == 0) {
+            m0 = t0;
+            m1 = t1;
+          } else {
+            const bool up0 = t0 > m0 + kRescaleAbove, up1 = t1 > m1 + kRescaleAbove;
+            up = up0 || up1;
+            if (up0) f0 = exp2_fast(m0 - t0), m0 = t0;
+            if (up1) f1 = exp2_fast(m1 - t1), m1 = t1;
             l0 *= f0;
             l1 *= f1;
-            if (lane % 4 == 0) {
-              sh.factor[row0] = f0;
-              sh.factor[row1] = f1;
-            }
           }
-        }
-        const float z0 = m0 == -INFINITY ? 0.f : m0, z1 = m1 == -INFINITY ? 0.f : m1;
-        if (active) {
+          if (lane % 4 == 0) {
+            sh.factor[i & 1][row0] = f0;
+            sh.factor[i & 1][row1] = f1;
+          }
+          const float z0 = m0 == -INFINITY ? 0.f : m0, z1 = m1 == -INFINITY ? 0.f : m1;
 #pragma unroll
           for (int n = 0; n < 8; ++n) {
             const float a = exp2_fast(__uint_as_float(x[4 * n]) - z0), b = exp2_fast(__uint_as_float(x[4 * n + 1]) - z0);
@@ -829,16 +806,16 @@ attend_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__
             x[2 * n + 1] = pack2(e, f, T());
           }
         }
+        const bool rescale = tile > 0 && softmax_any(up);
         // The weights before are read, and the accumulators at rest, once the second product of the tile before is over.
-        if (i > 0) wait(&sh.pv_done[(i - 1) % kTurns], turn_parity(i - 1), kAtPvDone);
+        if (i > 0) wait(&sh.pv_done[before.stage], before.lap, kAtPvDone);
         if (rescale) {
-          softmax_sync();
           tcgen05_fence_after();
           for (int col = 0; col < p.v_units * HT; col += 16) {
             uint32_t o[16];
             tmem_ld_32x16(tmem + lanes + col, o);
 #pragma unroll
-            for (int n = 0; n < 16; ++n) o[n] = __float_as_uint(__uint_as_float(o[n]) * sh.factor[col % HT + n]);
+            for (int n = 0; n < 16; ++n) o[n] = __float_as_uint(__uint_as_float(o[n]) * sh.factor[i & 1][col % HT + n]);
             tmem_st_32x16(tmem + lanes + col, o);
           }
           asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
@@ -857,19 +834,16 @@ attend_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__
         if (left < kTile) {
           // What lies behind the sequence in its last page may be anything: as values it has to be 0, because 0 weights times
           // infinity or NaN would be NaN.
-          int slot = v;
-          for (int u = 0; u < p.v_units; ++u) {
-            uint8_t* const unit = v_ring + slot * kUnitBytes;
-            for (int at = tid; at < (kTile - left) * 16; at += kSoftmaxThreads) {
-              const int row = left + at / 16, piece = at % 16;
-              *reinterpret_cast<uint4*>(unit + (row >> 3) * (2 * kGroupBytes) + (piece >> 3) * kGroupBytes + (row & 7) * kRowBytes + (piece & 7) * 16) =
-                  make_uint4(0u, 0u, 0u, 0u);
-            }
-            if (++slot == p.v_slots) slot = 0;
+          uint8_t* const tile_at = ring + here.stage * tile_bytes;
+          const int pieces = 2 * p.v_units * (kRowBytes / 16);  // of a row's value
+          for (int at = tid; at < (kTile - left) * pieces; at += kSoftmaxThreads) {
+            const int row = left + at / pieces, piece = at % pieces;
+            *reinterpret_cast<uint4*>(tile_at + (row >> 3) * group_bytes + (piece >> 3) * kGroupBytes + (row & 7) * kRowBytes + (piece & 7) * 16) =
+                make_uint4(0u, 0u, 0u, 0u);
           }
         }
-        v += p.v_units;
-        if (v >= p.v_slots) v -= p.v_slots;
+        before = here;
+        if (++here.stage == p.stages) here.stage = 0, here.lap ^= 1;
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&sh.p_full));
@@ -889,22 +863,35 @@ attend_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__
         }
       }
       softmax_sync();
-      wait(&sh.pv_done[(i - 1) % kTurns], turn_parity(i - 1), kAtPvDone);
+      wait(&sh.pv_done[before.stage], before.lap, kAtPvDone);
       tcgen05_fence_after();
       const int heads = min(HT, p.heads - head0);
-      if (walk.whole()) {
-        T* out = static_cast<T*>(p.out) + walk.b * p.out_sb + head0 * p.out_sh + tid;
-        for (int u = 0; u < p.v_units; ++u) {
-          for (int h0 = 0; h0 < HT; h0 += 16) {
-            uint32_t o[16];
-            tmem_ld_32x16(tmem + lanes + u * HT + h0, o);
+      const bool whole = walk.whole();
+      const long long part = (static_cast<long long>(worker) * p.head_tiles + head_tile) * 2 + (first_segment ? 0 : 1);
+      // kCols heads of 128 value elements at a time: a warp writes 32 elements of a head at once
+      constexpr int kCols = HT < 32 ? HT : 32;
+      for (int u = 0; u < p.v_units; ++u) {
 #pragma unroll
-            for (int n = 0; n < 16; ++n) {
-              const int h = h0 + n;
-              if (h < heads) from_float(__uint_as_float(o[n]) * sh.inverse[h], out + h * p.out_sh + u * 128);
-            }
+        for (int h0 = 0; h0 < HT; h0 += kCols) {
+          uint32_t o[kCols];
+          tmem_ld_32(tmem + lanes + u * HT + h0, o);
+          if (whole) {
+            T* out = static_cast<T*>(p.out) + walk.b * p.out_sb + (head0 + h0) * p.out_sh + u * 128 + tid;
+#pragma unroll
+            for (int n = 0; n < kCols; ++n, out += p.out_sh)
+              if (h0 + n < heads) from_float(__uint_as_float(o[n]) * sh.inverse[h0 + n], out);
+          } else {
+            float* const out = p.part_out + (part * HT + h0) * c.dv + u * 128 + tid;
+#pragma unroll
+            for (int n = 0; n < kCols; ++n)
+              if (h0 + n < heads) out[n * c.dv] = __uint_as_float(o[n]);
           }
         }
+      }
+      tcgen05_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&sh.o_free));
+      if (whole) {
         if (tid < heads) {
           const float2 st = sh.stat[tid];
           const float lse2 = (st.x == -INFINITY ? 0.f : st.x) + log2f(st.y);
@@ -912,24 +899,10 @@ attend_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__
           p.lse2[at] = lse2;
           if (p.lse != nullptr) p.lse[at] = lse2 * kLn2;
         }
-      } else {
-        const long long part = (static_cast<long long>(worker) * p.head_tiles + head_tile) * 2 + (first_segment ? 0 : 1);
-        float* out = p.part_out + part * HT * c.dv + tid;
-        for (int u = 0; u < p.v_units; ++u) {
-          for (int h0 = 0; h0 < HT; h0 += 16) {
-            uint32_t o[16];
-            tmem_ld_32x16(tmem + lanes + u * HT + h0, o);
-#pragma unroll
-            for (int n = 0; n < 16; ++n)
-              if (h0 + n < heads) out[(h0 + n) * c.dv + u * 128] = __uint_as_float(o[n]);
-          }
-        }
-        if (tid < heads) p.part_stat[part * HT + tid] = sh.stat[tid];
+      } else if (tid < heads) {
+        p.part_stat[part * HT + tid] = sh.stat[tid];
       }
       first_segment = false;
-      tcgen05_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&sh.o_free));
     }
   }
   tcgen05_fence_before();
@@ -940,94 +913,86 @@ attend_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__
   }
 }
 
-// Joins the parts of split sequences, in the order of their rows, and writes what sequences without rows get. A group of dv / 4
-// threads takes every fourth part of a head.
-constexpr int kJoinGroups = 4;
-constexpr int kJoinThreads = kJoinGroups * 128;
-
-template <typename T>
-__global__ void __launch_bounds__(kJoinThreads) attend_join_kernel(const __grid_constant__ AttendParams p, int tile_heads) {
-  __shared__ float4 sums[kJoinGroups][128];
-  __shared__ float2 stats[512];
-  __shared__ float scratch[2][kJoinThreads / 32];
+// Joins the parts of split sequences, in the order of their rows, and writes what sequences without rows get: a CTA per head and
+// sequence, GROUPS groups of a thread for every 4 value elements that share the parts. It reads what the attention left in L2; what
+// it costs is a chain of loads (where the sequence's parts are, their statistics, the parts), so every thread looks up all of it
+// for itself and only the groups' sums go through shared memory.
+template <typename T, int GROUPS>
+__global__ void __launch_bounds__(128 * GROUPS) attend_join_kernel(const __grid_constant__ AttendParams p, int tile_heads) {
+  __shared__ float4 sums[GROUPS][128];
   pdl_wait();
   pdl_launch_dependents();
-  const int b = static_cast<int>(blockIdx.y), tid = static_cast<int>(threadIdx.x);
+  const int h = static_cast<int>(blockIdx.x), b = static_cast<int>(blockIdx.y), tid = static_cast<int>(threadIdx.x);
   const long long tiles = p.first_tile[p.batch], begin = p.first_tile[b], end = p.first_tile[b + 1];
-  const int lanes = p.cache.dv / 4, group = tid >> 7, e = tid & 127;
-  int g0 = 0, parts = 0, workers = 1;
-  if (begin < end) {
-    workers = cache_walk::workers_of(tiles, p.workers, p.least);
-    g0 = cache_walk::worker_of(tiles, workers, begin);
-    parts = cache_walk::worker_of(tiles, workers, end - 1) - g0 + 1;
-    if (parts == 1) return;  // written by its worker
-  }
-  for (int h = static_cast<int>(blockIdx.x); h < p.heads; h += static_cast<int>(gridDim.x)) {
-    T* out = static_cast<T*>(p.out) + b * p.out_sb + h * p.out_sh;
-    const long long at = static_cast<long long>(b) * p.heads + h;
-    if (parts == 0) {
-      for (int i = tid; i < p.cache.dv; i += kJoinThreads) from_float(0.f, out + i);
-      if (tid == 0) {
-        p.lse2[at] = -INFINITY;
-        if (p.lse != nullptr) p.lse[at] = -INFINITY;
-      }
-      continue;
-    }
-    const int head_tile = h / tile_heads;
-    auto part_of = [&](int i) {
-      const int g = g0 + i;
-      const int slot = cache_walk::part_slot(cache_walk::share_begin(tiles, workers, g), begin);
-      return ((static_cast<long long>(g) * p.head_tiles + head_tile) * 2 + slot) * tile_heads + (h - head_tile * tile_heads);
-    };
-    // The largest maximum; parts fit the array because there are no more than workers (checked by the launch).
-    __syncthreads();
-    float top = -INFINITY;
-    for (int i = tid; i < parts; i += kJoinThreads) {
-      stats[i] = p.part_stat[part_of(i)];
-      top = fmaxf(top, stats[i].x);
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    if ((tid & 31) == 0) scratch[0][tid >> 5] = top;
-    __syncthreads();
-    for (int w = 0; w < kJoinThreads / 32; ++w) top = fmaxf(top, scratch[0][w]);
-    const float base = top == -INFINITY ? 0.f : top;
-    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-    float total = 0.f;
-    for (int i = 0; i < parts; ++i) total += stats[i].y * exp2_fast(stats[i].x - base);
-    if (e < lanes) {
-#pragma unroll 4
-      for (int i = group; i < parts; i += kJoinGroups) {
-        const float w = exp2_fast(stats[i].x - base);
-        const float4 v = *reinterpret_cast<const float4*>(p.part_out + part_of(i) * p.cache.dv + 4 * e);
-        sum.x += w * v.x;
-        sum.y += w * v.y;
-        sum.z += w * v.z;
-        sum.w += w * v.w;
-      }
-      sums[group][e] = sum;
-    }
-    __syncthreads();
-    if (group == 0 && e < lanes) {
-#pragma unroll
-      for (int k = 1; k < kJoinGroups; ++k) {
-        const float4 v = sums[k][e];
-        sum.x += v.x;
-        sum.y += v.y;
-        sum.z += v.z;
-        sum.w += v.w;
-      }
-      const float inverse = 1.f / total;
-      from_float(sum.x * inverse, out + 4 * e);
-      from_float(sum.y * inverse, out + 4 * e + 1);
-      from_float(sum.z * inverse, out + 4 * e + 2);
-      from_float(sum.w * inverse, out + 4 * e + 3);
-    }
+  const int dv = p.cache.dv, group = tid >> 7, e = tid & 127, lane = tid & 31;
+  T* const out = static_cast<T*>(p.out) + b * p.out_sb + h * p.out_sh;
+  const long long at = static_cast<long long>(b) * p.heads + h;
+  if (begin == end) {
+    for (int i = tid; i < dv; i += 128 * GROUPS) from_float(0.f, out + i);
     if (tid == 0) {
-      const float lse2 = base + log2f(total);
-      p.lse2[at] = lse2;
-      if (p.lse != nullptr) p.lse[at] = lse2 * kLn2;
+      p.lse2[at] = -INFINITY;
+      if (p.lse != nullptr) p.lse[at] = -INFINITY;
     }
+    return;
+  }
+  const int workers = cache_walk::workers_of(tiles, p.workers, p.least);
+  const int g0 = cache_walk::worker_of(tiles, workers, begin), parts = cache_walk::worker_of(tiles, workers, end - 1) - g0 + 1;
+  if (parts == 1) return;  // written by its worker
+  const int head_tile = h / tile_heads, in_tile = h - head_tile * tile_heads;
+  // Only the first part can lie behind another sequence's in its worker's share.
+  const int slot0 = cache_walk::part_slot(cache_walk::share_begin(tiles, workers, g0), begin);
+  auto part_of = [&](int i) {
+    return ((static_cast<long long>(g0 + i) * p.head_tiles + head_tile) * 2 + (i == 0 ? slot0 : 0)) * tile_heads + in_tile;
+  };
+  float top = -INFINITY;
+  for (int i = lane; i < parts; i += 32) top = fmaxf(top, p.part_stat[part_of(i)].x);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  const float base = top == -INFINITY ? 0.f : top;
+  float total = 0.f;
+  for (int i = lane; i < parts; i += 32) {
+    const float2 s = p.part_stat[part_of(i)];
+    total += s.y * exp2_fast(s.x - base);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+  float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (4 * e < dv) {
+#pragma unroll 4
+    for (int i = group; i < parts; i += GROUPS) {
+      const long long at_part = part_of(i);
+      const float w = exp2_fast(p.part_stat[at_part].x - base);
+      const float4 v = *reinterpret_cast<const float4*>(p.part_out + at_part * dv + 4 * e);
+      sum.x += w * v.x;
+      sum.y += w * v.y;
+      sum.z += w * v.z;
+      sum.w += w * v.w;
+    }
+  }
+  if constexpr (GROUPS > 1) {
+    sums[group][e] = sum;
+    __syncthreads();
+    if (group > 0) return;
+#pragma unroll
+    for (int k = 1; k < GROUPS; ++k) {
+      const float4 v = sums[k][e];
+      sum.x += v.x;
+      sum.y += v.y;
+      sum.z += v.z;
+      sum.w += v.w;
+    }
+  }
+  if (4 * e < dv) {
+    const float inverse = 1.f / total;
+    from_float(sum.x * inverse, out + 4 * e);
+    from_float(sum.y * inverse, out + 4 * e + 1);
+    from_float(sum.z * inverse, out + 4 * e + 2);
+    from_float(sum.w * inverse, out + 4 * e + 3);
+  }
+  if (tid == 0) {
+    const float lse2 = base + log2f(total);
+    p.lse2[at] = lse2;
+    if (p.lse != nullptr) p.lse[at] = lse2 * kLn2;
   }
 }
 
@@ -1303,7 +1268,7 @@ int tile_heads_for(int heads) { return heads <= 16 ? 16 : heads <= 32 ? 32 : 64;
 int attend_workers(int heads, int sms) {
   const int ht = tile_heads_for(heads), tiles = (heads + ht - 1) / ht;
   const int n = sms / tiles;
-  return n < 1 ? 1 : n < 512 ? n : 512;  // (the join holds the statistics of 512 parts)
+  return n < 1 ? 1 : n;
 }
 
 struct AttendWorkspace {
@@ -1323,18 +1288,12 @@ AttendWorkspace attend_workspace(int batch, int heads, int dv, int max_len, bool
   return w;
 }
 
-// Ring slots: as many tiles as fit, and of the value's units whatever else does. Returns the shared memory of the CTA.
-size_t plan_rings(int ht, AttendParams* p) {
-  const int unit = 2 * kTile * kRowBytes, rest = p->r_chunks * kTile * kRowBytes;
-  const int fixed = kHeaderBytes + (2 * p->v_units + p->r_chunks + 1) * ht * kRowBytes;
-  auto units = [&](int r) {
-    const int n = (kMaxSmem - fixed - r * rest) / unit;
-    return n < kMaxV ? n : kMaxV;
-  };
-  p->r_slots = rest > 0 ? 2 : 0;  // (two of the largest tiles fit next to 64 heads)
-  while (rest > 0 && p->r_slots < kMaxR && units(p->r_slots + 1) > p->v_units * p->r_slots) ++p->r_slots;
-  p->v_slots = units(p->r_slots);
-  return static_cast<size_t>(fixed) + p->v_slots * unit + p->r_slots * rest;
+// Tiles in the ring: as many as fit, two of the largest next to 64 heads. Returns the shared memory of the CTA.
+size_t plan_ring(int ht, AttendParams* p) {
+  const int fixed = kHeaderBytes + (p->chunks + 1) * ht * kRowBytes, tile = p->chunks * kTile * kRowBytes;
+  const int fit = (kMaxSmem - fixed) / tile;
+  p->stages = fit < kMaxStages ? fit : kMaxStages;
+  return static_cast<size_t>(fixed) + p->stages * tile;
 }
 
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
@@ -1370,7 +1329,7 @@ struct MapDims {
   }
 };
 
-typedef void (*AttendFn)(const CUtensorMap, const CUtensorMap, const CUtensorMap, const AttendParams);
+typedef void (*AttendFn)(const CUtensorMap, const CUtensorMap, const AttendParams);
 
 AttendFn attend_fn(bool bf16, int ht) {
   if (bf16) return ht == 16 ? attend_kernel<__nv_bfloat16, 16> : ht == 32 ? attend_kernel<__nv_bfloat16, 32> : attend_kernel<__nv_bfloat16, 64>;
@@ -1474,7 +1433,7 @@ int b200_mla_cache_attend(const b200_mla_cache* cache, const void* q, long long 
   p.least = kLeastTiles;
   p.copy_rows = cache_walk::copy_rows(cache->page_size);
   p.v_units = cache->dv / 128;
-  p.r_chunks = cache->dr / 64;
+  p.chunks = p.cache.d / 64;
   p.scale_log2 = scale * kLog2E;
   p.first_tile = reinterpret_cast<long long*>(ws);
   p.lse2 = reinterpret_cast<float*>(ws + w.lse2);
@@ -1483,35 +1442,30 @@ int b200_mla_cache_attend(const b200_mla_cache* cache, const void* q, long long 
   p.logits = score_out != nullptr ? reinterpret_cast<float*>(ws + w.logits) : nullptr;
   p.logit_tiles = cache_walk::tiles_of(max_len);
   p.status = device_status;
-  const size_t smem = plan_rings(ht, &p);
+  const size_t smem = plan_ring(ht, &p);
   const bool bf16 = cache->dtype == B200_MLA_CACHE_BF16;
-  CUtensorMap q_map, v_map, r_map;
-  const int chunks = p.cache.d / 64;
-  MapDims q_dims;
+  CUtensorMap q_map, row_map;
+  MapDims q_dims, row_dims;
   q_dims.add(heads, q_sh, ht);
-  q_dims.add(chunks, 64, chunks);
+  q_dims.add(p.chunks, 64, p.chunks);
   q_dims.add(cache->batch, q_sb, 1);
-  // Copies of whole groups of 8 rows bring all chunks of a unit; shorter ones (pages that no 8 divides) a chunk each.
-  auto row_dims = [&](int unit_chunks) {
-    const bool groups = p.copy_rows >= 8;
-    MapDims m;
-    m.add(groups ? 8 : cache->page_size, cache->slot_stride, groups ? 8 : p.copy_rows);
-    m.add(chunks, 64, groups ? unit_chunks : 1);
-    if (groups) m.add(cache->page_size / 8, 8 * cache->slot_stride, p.copy_rows / 8);
-    m.add(cache->pages, cache->page_stride, 1);
-    return m;
-  };
-  if (!q_dims.encode(&q_map, q, bf16) || !row_dims(2).encode(&v_map, cache->data, bf16)) return B200_FP8_MM_ERR_DRIVER;
-  r_map = v_map;
-  if (p.r_chunks != 0 && p.r_chunks != 2 && p.copy_rows >= 8 && !row_dims(p.r_chunks).encode(&r_map, cache->data, bf16)) return B200_FP8_MM_ERR_DRIVER;
+  // Copies of whole groups of 8 rows bring all chunks; shorter ones (pages that no 8 divides) a chunk each.
+  const bool groups = p.copy_rows >= 8;
+  row_dims.add(groups ? 8 : cache->page_size, cache->slot_stride, groups ? 8 : p.copy_rows);
+  row_dims.add(p.chunks, 64, groups ? p.chunks : 1);
+  if (groups) row_dims.add(cache->page_size / 8, 8 * cache->slot_stride, p.copy_rows / 8);
+  row_dims.add(cache->pages, cache->page_stride, 1);
+  if (!q_dims.encode(&q_map, q, bf16) || !row_dims.encode(&row_map, cache->data, bf16)) return B200_FP8_MM_ERR_DRIVER;
   const AttendFn fn = attend_fn(bf16, ht);
   if (!opt_in(fn, bf16, ht, device)) return B200_FP8_MM_ERR_DRIVER;
-  rc = launch_pdl(fn, dim3(static_cast<unsigned>(p.workers) * p.head_tiles), kAttendThreads, smem, stream, q_map, v_map, r_map, p);
+  rc = launch_pdl(fn, dim3(static_cast<unsigned>(p.workers) * p.head_tiles), kAttendThreads, smem, stream, q_map, row_map, p);
   if (rc != B200_FP8_MM_OK) return rc;
-  // CTAs for every SM a few times over, however few sequences there are; those of a sequence share its heads.
-  const int each = (4 * sms + cache->batch - 1) / cache->batch;
-  const dim3 joins(static_cast<unsigned>(each < heads ? each : heads), static_cast<unsigned>(cache->batch));
-  rc = launch_pdl(bf16 ? attend_join_kernel<__nv_bfloat16> : attend_join_kernel<__half>, joins, kJoinThreads, 0, stream, p, ht);
+  // Eight groups where a sequence has eight parts and more on average, one where most have one or two.
+  const dim3 joins(static_cast<unsigned>(heads), static_cast<unsigned>(cache->batch));
+  if (p.workers / cache->batch >= 8)
+    rc = launch_pdl(bf16 ? attend_join_kernel<__nv_bfloat16, 8> : attend_join_kernel<__half, 8>, joins, 1024, 0, stream, p, ht);
+  else
+    rc = launch_pdl(bf16 ? attend_join_kernel<__nv_bfloat16, 1> : attend_join_kernel<__half, 1>, joins, 128, 0, stream, p, ht);
   if (rc != B200_FP8_MM_OK || score_out == nullptr) return rc;
   return launch_pdl(attend_score_kernel, dim3(static_cast<unsigned>(p.logit_tiles), static_cast<unsigned>(cache->batch)), kScoreThreads, 0, stream, p);
 }
