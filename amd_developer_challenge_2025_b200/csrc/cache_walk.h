@@ -1,8 +1,9 @@
 // How the tiles of a batch of cached sequences are shared out, for the kernels of mla_cache_sm100.cu and a host test.
 //
-// A sequence of n rows has ceil(n / 64) tiles; the tiles of all sequences lie one behind the other, and worker g of `workers`
-// takes [share_begin(g), share_begin(g + 1)) of them, whatever sequences these belong to: shares differ by one tile at most,
-// however ragged the batch is. A sequence that lies in the shares of several workers leaves a part with each of them.
+// A sequence of n rows has ceil(n / 64) tiles, and costs `extra` tiles more to begin and end. On a line, every sequence that has
+// rows takes its extra places and then one for each tile, and worker g of `workers` takes the places [share_begin(g), share_begin(g +
+// 1)), whatever sequences these belong to: shares differ by one place at most, however ragged the batch is. A sequence whose tiles lie
+// in the shares of several workers leaves a part with each of them; a border among the extra places splits nothing.
 #ifndef B200_CACHE_WALK_H_
 #define B200_CACHE_WALK_H_
 
@@ -18,21 +19,32 @@ constexpr int kTileRows = 64;
 
 CACHE_WALK_FN int tiles_of(int rows) { return (rows + kTileRows - 1) / kTileRows; }
 
-// Workers that get tiles: as many as there are, but each with `least` tiles where the batch has that many.
-CACHE_WALK_FN int workers_of(long long tiles, int most, int least) {
-  const long long want = (tiles + least - 1) / least;
+// Places on the line of a sequence.
+CACHE_WALK_FN int places_of(int rows, int extra) { return rows > 0 ? tiles_of(rows) + extra : 0; }
+
+// Workers that get a share: as many as there are, but each with `least` places where the batch has that many.
+CACHE_WALK_FN int workers_of(long long places, int most, int least) {
+  const long long want = (places + least - 1) / least;
   return want < 1 ? 1 : want < most ? static_cast<int>(want) : most;
 }
 
-CACHE_WALK_FN long long share_begin(long long tiles, int workers, int g) { return tiles * g / workers; }
+CACHE_WALK_FN long long share_begin(long long places, int workers, int g) { return places * g / workers; }
 
-// The worker in whose share tile t lies (0 <= t < tiles).
-CACHE_WALK_FN int worker_of(long long tiles, int workers, long long t) {
-  return static_cast<int>(((t + 1) * workers - 1) / tiles);
+// The worker in whose share place t lies (0 <= t < places).
+CACHE_WALK_FN int worker_of(long long places, int workers, long long t) {
+  return static_cast<int>(((t + 1) * workers - 1) / places);
+}
+
+// The tiles [*first, *first + return value) of a sequence, whose places begin at `begin`, that lie in the share [from, to).
+CACHE_WALK_FN int tiles_in(long long begin, int tiles, int extra, long long from, long long to, int* first) {
+  const long long t0 = begin + extra, t1 = t0 + tiles;
+  const long long a = from > t0 ? from : t0, b = to < t1 ? to : t1;
+  *first = static_cast<int>(a - t0);
+  return b > a ? static_cast<int>(b - a) : 0;
 }
 
 // A worker's parts of split sequences: 0 for the one its share begins with, 1 for one that begins inside its share.
-CACHE_WALK_FN int part_slot(long long share, long long first_tile_of_sequence) { return share >= first_tile_of_sequence ? 0 : 1; }
+CACHE_WALK_FN int part_slot(long long share, long long begin_of_sequence) { return share >= begin_of_sequence ? 0 : 1; }
 
 // Rows that one copy can bring: the largest power of two, at most a tile's, that divides the page, so that no copy crosses a
 // page's end and every copy of a tile begins at a multiple of it.

@@ -171,16 +171,17 @@ struct AttendParams {
   float* score_out;
   long long out_sb, out_sh, score_stride, score_out_stride;
   int heads, head_tiles, max_len, batch;
-  int workers, least;      // workers per head tile, and the least tiles worth one
+  int workers, least;      // workers per head tile, and the least places worth one
+  int extra;               // see cache_walk.h
   int copy_rows;           // cache_walk::copy_rows(page_size)
   int stages;              // tiles of the ring
   int v_units, chunks;     // 128-element units of the value; 64-element chunks of a row
   float scale_log2;        // scale * log2(e)
   // Workspace
-  long long* first_tile;   // [batch + 1]: tiles before each sequence, and all
+  long long* begins;       // [batch + 1]: places before each sequence, and all
   float* lse2;             // [batch][heads]: log2 of the sum of 2^x
   float2* part_stat;       // [worker][head tile][2][heads of a tile]: maximum and sum
-  float* part_out;         // the same, times dv
+  float* part_out;         // [worker][head tile][2][128-element unit of the value][heads of a tile][128]
   float* logits;           // [batch][tile][heads][rows of a tile] in log2, or null
   int logit_tiles;
   int* status;             // may be null
@@ -413,36 +414,30 @@ struct alignas(8) AttendShared {
   float2 stat[64];      // maximum and sum of weights of a head
   float inverse[64];    // 1 / sum
   long long sums[kAttendThreads / 32];
-  long long share, share_end;
+  long long share, share_end;  // this worker's places
+  long long first_begin;       // where those of the sequence that the share begins in begin
   uint32_t tmem_base;
-  int expired, first_seq, first_tile;
+  int expired, first_seq;
 };
 static_assert(sizeof(AttendShared) <= kHeaderBytes, "the header is too small");
 
 // A worker's walk over its share: segment after segment, each a run of tiles of one sequence.
 struct Walk {
-  int b, t;        // sequence, first tile of the segment
-  int rows, count; // rows of the sequence, tiles of the segment
-  long long left;
+  int b, t, rows, count;   // sequence and first tile of the segment, rows of the sequence, tiles of the segment
+  long long begin, from, to;
 
-  __device__ __forceinline__ Walk(const AttendShared& sh) : b(sh.first_seq), t(sh.first_tile), rows(0), count(0), left(sh.share_end - sh.share) {}
+  __device__ __forceinline__ Walk(const AttendShared& sh) : b(sh.first_seq - 1), t(0), rows(0), count(0), begin(sh.first_begin), from(sh.share), to(sh.share_end) {}
   __device__ __forceinline__ bool next(const AttendParams& p) {
-    t += count;
-    count = 0;
-    while (left > 0) {
-      rows = rows_of(p.cache, b, p.max_len);
-      const int tiles = cache_walk::tiles_of(rows);
-      if (t < tiles) {
-        count = static_cast<int>(min(static_cast<long long>(tiles - t), left));
-        left -= count;
-        return true;
-      }
+    while (begin < to) {
       ++b;
-      t = 0;
+      rows = rows_of(p.cache, b, p.max_len);
+      count = cache_walk::tiles_in(begin, cache_walk::tiles_of(rows), p.extra, from, to, &t);
+      begin += cache_walk::places_of(rows, p.extra);
+      if (rows > 0 && count > 0) return true;
     }
     return false;
   }
-  __device__ __forceinline__ bool whole() const { return t == 0 && count == cache_walk::tiles_of(rows); }
+  __device__ __forceinline__ bool whole() const { return count == cache_walk::tiles_of(rows); }
 };
 
 // Flash attention of one token per sequence over a latent cache: heads x rows x (d + dv) products per row of d elements read.
@@ -468,11 +463,16 @@ template <typename T, int HT>
 __global__ void __launch_bounds__(kAttendThreads, 1)
 attend_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap row_map, const __grid_constant__ AttendParams p) {
   extern __shared__ __align__(1024) uint8_t smem[];
-  const CacheView& c = p.cache;
-  const int group_bytes = p.chunks * kGroupBytes, tile_bytes = kTile / 8 * group_bytes;
+  // The loops below are full of statements that touch memory, behind each of which a parameter would be read anew.
+  const CacheView c = p.cache;
+  const int v_units = p.v_units, chunks = p.chunks, stages = p.stages, copy_rows = p.copy_rows, heads_all = p.heads;
+  const float scale_log2 = p.scale_log2;
+  const long long out_sb = p.out_sb, out_sh = p.out_sh;
+  float *const logits = p.logits, *const part_out = p.part_out;
+  const int group_bytes = chunks * kGroupBytes, tile_bytes = kTile / 8 * group_bytes;
   uint8_t* const q_smem = smem;  // [chunk][HT rows x 128 bytes]; the first product reads 64 rows, those behind HT are never looked at
-  uint8_t* const ring = q_smem + p.chunks * HT * kRowBytes;
-  uint8_t* const p_smem = ring + p.stages * tile_bytes;
+  uint8_t* const ring = q_smem + chunks * HT * kRowBytes;
+  uint8_t* const p_smem = ring + stages * tile_bytes;
   AttendShared& sh = *reinterpret_cast<AttendShared*>(p_smem + HT * kRowBytes);
   const int tid = static_cast<int>(threadIdx.x), warp = tid >> 5, lane = tid & 31;
   const int head_tile = static_cast<int>(blockIdx.x) % p.head_tiles, worker = static_cast<int>(blockIdx.x) / p.head_tiles;
@@ -503,11 +503,11 @@ attend_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__
   }
   pdl_wait();
   pdl_launch_dependents();
-  // Tiles before each thread's run of sequences, and where this worker's share begins.
+  // Places before each thread's run of sequences, and where this worker's share begins.
   const int run = (p.batch + kAttendThreads - 1) / kAttendThreads;
   const int b0 = min(p.batch, tid * run), b1 = min(p.batch, b0 + run);
   long long mine = 0;
-  for (int b = b0; b < b1; ++b) mine += cache_walk::tiles_of(rows_of(c, b, p.max_len));
+  for (int b = b0; b < b1; ++b) mine += cache_walk::places_of(rows_of(c, b, p.max_len), p.extra);
   long long upto = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -518,45 +518,46 @@ attend_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__
   tcgen05_fence_before();
   __syncthreads();
   tcgen05_fence_after();
-  constexpr uint32_t tmem = 0;  // all columns are this CTA's, so they begin at the first (checked below)
+  constexpr uint32_t tmem = 0;  // all columns are this CTA's, so they begin at the first (checked here)
   if (tid == 0 && sh.tmem_base != tmem) sh.expired = 1;
   {
-    long long before = upto - mine, tiles = 0;
+    long long before = upto - mine, places = 0;
     for (int w = 0; w < kAttendThreads / 32; ++w) {
       if (w < warp) before += sh.sums[w];
-      tiles += sh.sums[w];
+      places += sh.sums[w];
     }
-    const int workers = cache_walk::workers_of(tiles, p.workers, p.least);
-    const long long begin = worker < workers ? cache_walk::share_begin(tiles, workers, worker) : 0;
-    const long long end = worker < workers ? cache_walk::share_begin(tiles, workers, worker + 1) : 0;
+    const int workers = cache_walk::workers_of(places, p.workers, p.least);
+    const long long begin = worker < workers ? cache_walk::share_begin(places, workers, worker) : 0;
+    const long long end = worker < workers ? cache_walk::share_begin(places, workers, worker + 1) : 0;
     if (tid == 0) {
       sh.share = begin;
       sh.share_end = end;
+      if (begin == end) sh.first_begin = end;
     }
     if (begin < end && before <= begin && begin < before + mine) {
-      long long at = begin - before;
+      long long at = before;
       int b = b0;
       for (;; ++b) {
-        const int n = cache_walk::tiles_of(rows_of(c, b, p.max_len));
-        if (at < n) break;
-        at -= n;
+        const int n = cache_walk::places_of(rows_of(c, b, p.max_len), p.extra);
+        if (begin < at + n) break;
+        at += n;
       }
       sh.first_seq = b;
-      sh.first_tile = static_cast<int>(at);
+      sh.first_begin = at;
     }
     if (blockIdx.x == 0) {
       for (int b = b0; b < b1; ++b) {
-        p.first_tile[b] = before;
-        before += cache_walk::tiles_of(rows_of(c, b, p.max_len));
+        p.begins[b] = before;
+        before += cache_walk::places_of(rows_of(c, b, p.max_len), p.extra);
       }
-      if (tid == 0) p.first_tile[p.batch] = tiles;
+      if (tid == 0) p.begins[p.batch] = places;
     }
   }
   __syncthreads();
 
   if (warp == 4) {
     // Copies. Lane l knows where pieces l and l + 32 (copy_rows rows each) of a tile come from.
-    const int pieces = kTile / p.copy_rows;
+    const int pieces = kTile / copy_rows;
     int stage = 0, segment = 0;
     uint32_t lap = 0;  // parity of the ring's current use
     bool first_lap = true, ok = __all_sync(0xffffffffu, sh.expired == 0);
@@ -568,7 +569,7 @@ attend_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__
       auto place = [&](int tile) {
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-          const int piece = lane + 32 * k, row = tile * kTile + piece * p.copy_rows;
+          const int piece = lane + 32 * k, row = tile * kTile + piece * copy_rows;
           page[k] = c.pages;
           slot[k] = 0;
           if (piece < pieces && tile < walk.t + walk.count && row < walk.rows) {
@@ -586,24 +587,24 @@ attend_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__
         if (!first_lap && !(ok = waits.wait_all(smem_u32(&sh.pv_done[stage]), lap ^ 1, kAtFree))) break;
         if (lane == 0) mbar_expect_tx(full, tile_bytes);
         __syncwarp();
-        if (p.copy_rows >= 8) {
+        if (copy_rows >= 8) {
           for (int i = 0; i < pieces; ++i)
-            tma_load_5d(to + i * (p.copy_rows >> 3) * group_bytes, &row_map, 0, 0, __shfl_sync(0xffffffffu, slot[0], i) >> 3,
+            tma_load_5d(to + i * (copy_rows >> 3) * group_bytes, &row_map, 0, 0, __shfl_sync(0xffffffffu, slot[0], i) >> 3,
                         __shfl_sync(0xffffffffu, page[0], i), full);
         } else {
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
-            const int piece = lane + 32 * k, row = piece * p.copy_rows;
+            const int piece = lane + 32 * k, row = piece * copy_rows;
             if (piece < pieces)
-              for (int i = 0; i < p.chunks; ++i)
+              for (int i = 0; i < chunks; ++i)
                 tma_load_4d_own(to + (row >> 3) * group_bytes + i * kGroupBytes + (row & 7) * kRowBytes, &row_map, slot[k], i, page[k], full);
           }
         }
-        if (++stage == p.stages) stage = 0, lap ^= 1, first_lap = false;
+        if (++stage == stages) stage = 0, lap ^= 1, first_lap = false;
         if (tile == 0) {
           // The queries of this segment, once the first products of the segment before are over.
           if (segment > 0 && !(ok = waits.wait_all(smem_u32(&sh.q_empty), (segment - 1) & 1, kAtQEmpty))) break;
-          if (lane == 0) mbar_expect_tx(smem_u32(&sh.q_full), p.chunks * HT * kRowBytes);
+          if (lane == 0) mbar_expect_tx(smem_u32(&sh.q_full), chunks * HT * kRowBytes);
           __syncwarp();
           tma_load_4d(smem_u32(q_smem), &q_map, head0, 0, walk.b, smem_u32(&sh.q_full));
         }
@@ -619,7 +620,7 @@ attend_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__
           for (int n = 0; n < 1000 && !mbar_try_wait(smem_u32(bar), parity, 10000); ++n) {
           }
       };
-      for (int n = 0; n < p.stages; ++n) drain(&sh.full[n]);
+      for (int n = 0; n < stages; ++n) drain(&sh.full[n]);
       drain(&sh.q_full);
     }
     __syncwarp();
@@ -649,7 +650,7 @@ attend_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__
       tcgen05_fence_after();
       uint32_t values = uniform(kLoV | (ring_at + pv_stage * (tile_bytes >> 4))), o = tmem;
 #pragma unroll 1
-      for (int u = 0; u < p.v_units; ++u, values += 2 * kGroupBytes >> 4, o += HT)
+      for (int u = 0; u < v_units; ++u, values += 2 * kGroupBytes >> 4, o += HT)
         umma_f16_x4(o, values, hi_rows, 2 * group_bytes >> 4, p_lo, kHiDense, kIdescO, pending_first ? 0u : 1u);
       umma_commit(smem_u32(&sh.pv_done[pv_stage]));
       pending = false;
@@ -693,7 +694,7 @@ attend_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__
         const uint32_t s = uniform(tmem + kTmemLogits + (i & 1) * kTile);
         uint32_t rows = uniform(kLoK | (ring_at + stage * (tile_bytes >> 4))), q_at = q_lo;
 #pragma unroll 1
-        for (int n = 0; n < p.chunks; ++n, q_at += HT * kRowBytes >> 4, rows += kGroupBytes >> 4)
+        for (int n = 0; n < chunks; ++n, q_at += HT * kRowBytes >> 4, rows += kGroupBytes >> 4)
           umma_f16_x4(s, q_at, kHiDense, 2, rows, hi_rows, kIdescS, n > 0);
         umma_commit(smem_u32(&sh.s_full[i & 1]));
         if (tile == count - 1) umma_commit(smem_u32(&sh.q_empty));
@@ -706,7 +707,7 @@ attend_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__
         pending_first = tile == 0;
         pv_stage = stage;
         pv_segment = segment;
-        if (++stage == p.stages) stage = 0, lap ^= 1;
+        if (++stage == stages) stage = 0, lap ^= 1;
       }
       ++segment;
     }
@@ -752,25 +753,25 @@ attend_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__
         if (active) {
           if (left >= kTile) {
 #pragma unroll
-            for (int n = 0; n < 32; ++n) x[n] = __float_as_uint(__uint_as_float(x[n]) * p.scale_log2);
+            for (int n = 0; n < 32; ++n) x[n] = __float_as_uint(__uint_as_float(x[n]) * scale_log2);
           } else {
 #pragma unroll
             for (int n = 0; n < 32; ++n) {
               const int col = 8 * (n / 4) + 2 * (lane % 4) + (n & 1);
-              x[n] = __float_as_uint(col < left ? __uint_as_float(x[n]) * p.scale_log2 : -INFINITY);
+              x[n] = __float_as_uint(col < left ? __uint_as_float(x[n]) * scale_log2 : -INFINITY);
             }
           }
 #pragma unroll
           for (int n = 0; n < 32; ++n) {
             if (n & 2) t1 = fmaxf(t1, __uint_as_float(x[n])); else t0 = fmaxf(t0, __uint_as_float(x[n]));
           }
-          if (p.logits != nullptr) {
-            float* to = p.logits + ((static_cast<long long>(walk.b) * p.logit_tiles + walk.t + tile) * p.heads + head0) * kTile + 2 * (lane % 4);
+          if (logits != nullptr) {
+            float* to = logits + ((static_cast<long long>(walk.b) * p.logit_tiles + walk.t + tile) * heads_all + head0) * kTile + 2 * (lane % 4);
 #pragma unroll
             for (int n = 0; n < 8; ++n) {
-              if (row0 < HT && head0 + row0 < p.heads)
+              if (row0 < HT && head0 + row0 < heads_all)
                 *reinterpret_cast<uint2*>(to + row0 * kTile + 8 * n) = make_uint2(x[4 * n], x[4 * n + 1]);
-              if (row1 < HT && head0 + row1 < p.heads)
+              if (row1 < HT && head0 + row1 < heads_all)
                 *reinterpret_cast<uint2*>(to + row1 * kTile + 8 * n) = make_uint2(x[4 * n + 2], x[4 * n + 3]);
             }
           }
@@ -811,7 +812,7 @@ attend_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__
         if (i > 0) wait(&sh.pv_done[before.stage], before.lap, kAtPvDone);
         if (rescale) {
           tcgen05_fence_after();
-          for (int col = 0; col < p.v_units * HT; col += 16) {
+          for (int col = 0; col < v_units * HT; col += 16) {
             uint32_t o[16];
             tmem_ld_32x16(tmem + lanes + col, o);
 #pragma unroll
@@ -835,7 +836,7 @@ attend_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__
           // What lies behind the sequence in its last page may be anything: as values it has to be 0, because 0 weights times
           // infinity or NaN would be NaN.
           uint8_t* const tile_at = ring + here.stage * tile_bytes;
-          const int pieces = 2 * p.v_units * (kRowBytes / 16);  // of a row's value
+          const int pieces = 2 * v_units * (kRowBytes / 16);  // of a row's value
           for (int at = tid; at < (kTile - left) * pieces; at += kSoftmaxThreads) {
             const int row = left + at / pieces, piece = at % pieces;
             *reinterpret_cast<uint4*>(tile_at + (row >> 3) * group_bytes + (piece >> 3) * kGroupBytes + (row & 7) * kRowBytes + (piece & 7) * 16) =
@@ -843,7 +844,7 @@ attend_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__
           }
         }
         before = here;
-        if (++here.stage == p.stages) here.stage = 0, here.lap ^= 1;
+        if (++here.stage == stages) here.stage = 0, here.lap ^= 1;
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&sh.p_full));
@@ -865,26 +866,25 @@ attend_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__
       softmax_sync();
       wait(&sh.pv_done[before.stage], before.lap, kAtPvDone);
       tcgen05_fence_after();
-      const int heads = min(HT, p.heads - head0);
+      const int heads = min(HT, heads_all - head0);
       const bool whole = walk.whole();
       const long long part = (static_cast<long long>(worker) * p.head_tiles + head_tile) * 2 + (first_segment ? 0 : 1);
       // kCols heads of 128 value elements at a time: a warp writes 32 elements of a head at once
       constexpr int kCols = HT < 32 ? HT : 32;
-      for (int u = 0; u < p.v_units; ++u) {
+      for (int u = 0; u < v_units; ++u) {
 #pragma unroll
         for (int h0 = 0; h0 < HT; h0 += kCols) {
           uint32_t o[kCols];
           tmem_ld_32(tmem + lanes + u * HT + h0, o);
           if (whole) {
-            T* out = static_cast<T*>(p.out) + walk.b * p.out_sb + (head0 + h0) * p.out_sh + u * 128 + tid;
+            T* out = static_cast<T*>(p.out) + walk.b * out_sb + (head0 + h0) * out_sh + u * 128 + tid;
 #pragma unroll
-            for (int n = 0; n < kCols; ++n, out += p.out_sh)
+            for (int n = 0; n < kCols; ++n, out += out_sh)
               if (h0 + n < heads) from_float(__uint_as_float(o[n]) * sh.inverse[h0 + n], out);
           } else {
-            float* const out = p.part_out + (part * HT + h0) * c.dv + u * 128 + tid;
+            float* const out = part_out + ((part * v_units + u) * HT + h0) * 128 + tid;
 #pragma unroll
-            for (int n = 0; n < kCols; ++n)
-              if (h0 + n < heads) out[n * c.dv] = __uint_as_float(o[n]);
+            for (int n = 0; n < kCols; ++n) out[n * 128] = __uint_as_float(o[n]);
           }
         }
       }
@@ -895,7 +895,7 @@ attend_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__
         if (tid < heads) {
           const float2 st = sh.stat[tid];
           const float lse2 = (st.x == -INFINITY ? 0.f : st.x) + log2f(st.y);
-          const long long at = static_cast<long long>(walk.b) * p.heads + head0 + tid;
+          const long long at = static_cast<long long>(walk.b) * heads_all + head0 + tid;
           p.lse2[at] = lse2;
           if (p.lse != nullptr) p.lse[at] = lse2 * kLn2;
         }
@@ -923,7 +923,7 @@ __global__ void __launch_bounds__(128 * GROUPS) attend_join_kernel(const __grid_
   pdl_wait();
   pdl_launch_dependents();
   const int h = static_cast<int>(blockIdx.x), b = static_cast<int>(blockIdx.y), tid = static_cast<int>(threadIdx.x);
-  const long long tiles = p.first_tile[p.batch], begin = p.first_tile[b], end = p.first_tile[b + 1];
+  const long long places = p.begins[p.batch], begin = p.begins[b], end = p.begins[b + 1];
   const int dv = p.cache.dv, group = tid >> 7, e = tid & 127, lane = tid & 31;
   T* const out = static_cast<T*>(p.out) + b * p.out_sb + h * p.out_sh;
   const long long at = static_cast<long long>(b) * p.heads + h;
@@ -935,23 +935,22 @@ __global__ void __launch_bounds__(128 * GROUPS) attend_join_kernel(const __grid_
     }
     return;
   }
-  const int workers = cache_walk::workers_of(tiles, p.workers, p.least);
-  const int g0 = cache_walk::worker_of(tiles, workers, begin), parts = cache_walk::worker_of(tiles, workers, end - 1) - g0 + 1;
+  const int workers = cache_walk::workers_of(places, p.workers, p.least);
+  const int g0 = cache_walk::worker_of(places, workers, begin + p.extra), parts = cache_walk::worker_of(places, workers, end - 1) - g0 + 1;
   if (parts == 1) return;  // written by its worker
   const int head_tile = h / tile_heads, in_tile = h - head_tile * tile_heads;
   // Only the first part can lie behind another sequence's in its worker's share.
-  const int slot0 = cache_walk::part_slot(cache_walk::share_begin(tiles, workers, g0), begin);
-  auto part_of = [&](int i) {
-    return ((static_cast<long long>(g0 + i) * p.head_tiles + head_tile) * 2 + (i == 0 ? slot0 : 0)) * tile_heads + in_tile;
-  };
+  const int slot0 = cache_walk::part_slot(cache_walk::share_begin(places, workers, g0), begin);
+  auto part_of = [&](int i) { return (static_cast<long long>(g0 + i) * p.head_tiles + head_tile) * 2 + (i == 0 ? slot0 : 0); };
+  auto stat_of = [&](int i) { return p.part_stat[part_of(i) * tile_heads + in_tile]; };
   float top = -INFINITY;
-  for (int i = lane; i < parts; i += 32) top = fmaxf(top, p.part_stat[part_of(i)].x);
+  for (int i = lane; i < parts; i += 32) top = fmaxf(top, stat_of(i).x);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
   const float base = top == -INFINITY ? 0.f : top;
   float total = 0.f;
   for (int i = lane; i < parts; i += 32) {
-    const float2 s = p.part_stat[part_of(i)];
+    const float2 s = stat_of(i);
     total += s.y * exp2_fast(s.x - base);
   }
 #pragma unroll
@@ -960,9 +959,8 @@ __global__ void __launch_bounds__(128 * GROUPS) attend_join_kernel(const __grid_
   if (4 * e < dv) {
 #pragma unroll 4
     for (int i = group; i < parts; i += GROUPS) {
-      const long long at_part = part_of(i);
-      const float w = exp2_fast(p.part_stat[at_part].x - base);
-      const float4 v = *reinterpret_cast<const float4*>(p.part_out + at_part * dv + 4 * e);
+      const float w = exp2_fast(stat_of(i).x - base);
+      const float4 v = *reinterpret_cast<const float4*>(p.part_out + ((part_of(i) * (dv / 128) + e / 32) * tile_heads + in_tile) * 128 + 4 * (e % 32));
       sum.x += w * v.x;
       sum.y += w * v.y;
       sum.z += w * v.z;
@@ -1234,7 +1232,11 @@ int view_of(const b200_mla_cache* c, CacheView* v) {
 
 constexpr int kMaxHeads = 1 << 16;
 constexpr int kMaxDevices = 64;
-constexpr int kLeastTiles = 1;
+constexpr int kLeastPlaces = 1;
+
+// What beginning and ending a sequence costs a worker, in tiles: its accumulators are read out and written while the tensor core
+// has little to do. 64 heads: 128 KB at the 32 bytes that an SM stores per clock, 5000 clocks against 3400 of a tile.
+int extra_for(int ht) { return ht < 64 ? 1 : 2; }
 
 int current_device() {
   int dev = -1;
@@ -1430,12 +1432,13 @@ int b200_mla_cache_attend(const b200_mla_cache* cache, const void* q, long long 
   p.max_len = max_len;
   p.batch = cache->batch;
   p.workers = attend_workers(heads, sms);
-  p.least = kLeastTiles;
+  p.least = kLeastPlaces + extra_for(ht);
+  p.extra = extra_for(ht);
   p.copy_rows = cache_walk::copy_rows(cache->page_size);
   p.v_units = cache->dv / 128;
   p.chunks = p.cache.d / 64;
   p.scale_log2 = scale * kLog2E;
-  p.first_tile = reinterpret_cast<long long*>(ws);
+  p.begins = reinterpret_cast<long long*>(ws);
   p.lse2 = reinterpret_cast<float*>(ws + w.lse2);
   p.part_stat = reinterpret_cast<float2*>(ws + w.part_stat);
   p.part_out = reinterpret_cast<float*>(ws + w.part_out);

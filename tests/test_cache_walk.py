@@ -14,30 +14,36 @@ PROGRAM = """
 #include <vector>
 #include "cache_walk.h"
 using namespace cache_walk;
-// walk <most> <least> <rows of sequence 0> <rows of sequence 1> ...: per worker "worker begin end", then per part of a split sequence,
-// as the attention writes them "w sequence worker slot first count", as the join looks them up "j sequence worker slot"
+// walk <most> <least> <extra> <rows of sequence 0> <rows of sequence 1> ...: per worker "worker places", per segment "s sequence worker
+// first count", per part of a split sequence "w sequence worker slot first count" as the attention writes it, "j sequence worker slot" as
+// the join looks it up
 int main(int argc, char** argv) {
-  const int most = atoi(argv[1]), least = atoi(argv[2]);
-  std::vector<long long> first{0};
-  for (int i = 3; i < argc; ++i) first.push_back(first.back() + tiles_of(atoi(argv[i])));
-  const long long tiles = first.back();
-  const int workers = workers_of(tiles, most, least);
+  const int most = atoi(argv[1]), least = atoi(argv[2]), extra = atoi(argv[3]), batch = argc - 4;
+  std::vector<int> rows;
+  std::vector<long long> begins{0};
+  for (int b = 0; b < batch; ++b) {
+    rows.push_back(atoi(argv[4 + b]));
+    begins.push_back(begins.back() + places_of(rows[b], extra));
+  }
+  const long long places = begins.back();
+  const int workers = workers_of(places, most, least);
   for (int g = 0; g < workers; ++g) {
-    long long t = share_begin(tiles, workers, g);
-    const long long end = share_begin(tiles, workers, g + 1);
-    printf("%d %lld %lld\\n", g, t, end);
-    for (int segment = 0; t < end; ++segment) {
-      int b = 0;
-      while (first[b + 1] <= t) ++b;
-      const long long to = end < first[b + 1] ? end : first[b + 1];
-      if (t != first[b] || to != first[b + 1]) printf("w %d %d %d %lld %lld\\n", b, g, segment == 0 ? 0 : 1, t - first[b], to - t);
-      t = to;
+    const long long from = share_begin(places, workers, g), to = share_begin(places, workers, g + 1);
+    printf("%d %lld\\n", g, to - from);
+    bool first_segment = true;
+    for (int b = 0; b < batch; ++b) {
+      int first;
+      const int count = rows[b] > 0 ? tiles_in(begins[b], tiles_of(rows[b]), extra, from, to, &first) : 0;
+      if (count == 0) continue;
+      printf("s %d %d %d %d\\n", b, g, first, count);
+      if (count != tiles_of(rows[b])) printf("w %d %d %d %d %d\\n", b, g, first_segment ? 0 : 1, first, count);
+      first_segment = false;
     }
   }
-  for (int b = 0; b + 3 < argc; ++b) {
-    if (first[b] == first[b + 1]) continue;
-    const int g0 = worker_of(tiles, workers, first[b]), g1 = worker_of(tiles, workers, first[b + 1] - 1);
-    for (int g = g0; g1 > g0 && g <= g1; ++g) printf("j %d %d %d\\n", b, g, part_slot(share_begin(tiles, workers, g), first[b]));
+  for (int b = 0; b < batch; ++b) {
+    if (begins[b] == begins[b + 1]) continue;
+    const int g0 = worker_of(places, workers, begins[b] + extra), g1 = worker_of(places, workers, begins[b + 1] - 1);
+    for (int g = g0; g1 > g0 && g <= g1; ++g) printf("j %d %d %d\\n", b, g, g == g0 ? part_slot(share_begin(places, workers, g), begins[b]) : 0);
   }
   for (int p = 1; p <= 300; ++p) printf("r %d %d\\n", p, copy_rows(p));
   // far beyond 32 bits
@@ -60,33 +66,33 @@ def walk(tmp_path_factory):
     return lambda *args: [line.split() for line in subprocess.check_output([str(d / "walk"), *map(str, args)], text=True).splitlines()]
 
 
+@pytest.mark.parametrize("extra", [0, 1, 2, 5])
 @pytest.mark.parametrize("most,least", [(1, 1), (2, 1), (74, 1), (148, 1), (148, 3), (512, 2)])
-def test_shares_and_parts(walk, most, least):
-    rng = random.Random(most + least)
+def test_shares_and_parts(walk, most, least, extra):
+    rng = random.Random(most + least + extra)
     for rows in ([1], [64], [65], [0, 0], [0, 5, 0], [9000], [1] * 200, [rng.randint(0, 900) for _ in range(60)],
                  [rng.choice([0, 1, 64, 65, 20000]) for _ in range(30)]):
-        lines = walk(most, least, *rows)
-        shares = [tuple(map(int, f)) for f in lines if f[0].isdigit()]
-        tiles = sum(-(-n // 64) for n in rows)
-        assert 1 <= len(shares) <= most and shares[0][1] == 0 and shares[-1][2] == tiles
-        assert all(a[2] == b[1] for a, b in zip(shares, shares[1:]))
-        sizes = [e - b for _, b, e in shares]
+        lines = walk(most, least, extra, *rows)
+        sizes = [int(f[1]) for f in lines if f[0].isdigit()]
+        tiles = [-(-n // 64) for n in rows]
+        places = sum(n + extra for n in tiles if n)
+        assert 1 <= len(sizes) <= most and sum(sizes) == places
         assert max(sizes) - min(sizes) <= 1
-        assert len(shares) == 1 or tiles > (len(shares) - 1) * least
-        written = [tuple(map(int, f[1:])) for f in lines if f[0] == "w"]
-        assert [w[:3] for w in written] == sorted(w[:3] for w in written)
-        assert [w[:3] for w in written] == [tuple(map(int, f[1:])) for f in lines if f[0] == "j"]
-        assert len({w[1:3] for w in written}) == len(written)  # no two parts in one place
-        for b in {w[0] for w in written}:
+        assert len(sizes) == 1 or places > (len(sizes) - 1) * least
+        segments = [tuple(map(int, f[1:])) for f in lines if f[0] == "s"]
+        for b, n in enumerate(tiles):  # every tile once, in the order of the workers
             at = 0
-            for w in (w for w in written if w[0] == b):
-                assert w[3] == at and w[4] > 0
-                at += w[4]
-            assert at == -(-rows[b] // 64)
+            for s in (s for s in segments if s[0] == b):
+                assert s[2] == at and s[3] > 0
+                at += s[3]
+            assert at == n
+        written = [tuple(map(int, f[1:])) for f in lines if f[0] == "w"]
+        assert [w[:3] for w in sorted(written)] == [tuple(map(int, f[1:])) for f in lines if f[0] == "j"]
+        assert len({w[1:3] for w in written}) == len(written)  # no two parts in one place
 
 
 def test_copies_stay_inside_their_page_and_tile(walk):
-    lines = walk(1, 1, 1)
+    lines = walk(1, 1, 0, 1)
     assert ["far"] not in lines
     for _, page, rows in (f for f in lines if f[0] == "r"):
         page, rows = int(page), int(rows)
