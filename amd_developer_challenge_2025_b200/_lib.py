@@ -96,7 +96,7 @@ class _PythonChecks:
     def fp8_mm(*args):
         return False
 
-    fp8_mm_grouped = mla_decode = div_softmax = fp8_mm
+    fp8_mm_grouped = mla_decode = div_softmax = mla_cache_append = mla_cache_attend = mla_cache_evict = fp8_mm
 
 
 def host_calls():
@@ -121,6 +121,9 @@ def _load_host():
     spec.loader.exec_module(mod)
     mod.bind(*(ctypes.cast(f, ctypes.c_void_p).value for f in
                (lib.b200_fp8_mm_strided, lib.b200_fp8_mm_grouped, lib.b200_mla_rope, lib.b200_mla_div_softmax)))
+    mod.bind_cache(*(ctypes.cast(f, ctypes.c_void_p).value for f in
+                     (lib.b200_mla_cache_append, lib.b200_mla_cache_attend, lib.b200_mla_cache_attend_workspace_bytes,
+                      lib.b200_mla_cache_evict, lib.b200_mla_cache_evict_workspace_bytes)))
     _host = mod
     return mod
 

@@ -3,17 +3,21 @@
 // microseconds; the same checks and the argument conversion of a ctypes call took 12 to 15 us in Python and take about
 // one here. Every call is checked in full, nothing is remembered between calls.
 //
-// A function returns True when the kernel has been launched. It returns False, having done nothing, for anything but
+// A function returns True (or its results) when the kernel has been launched. It returns False, having done nothing, for anything but
 // the plain case (a check that fails, tensors that are not plain CUDA tensors on the current device, a workspace that
 // does not exist yet, a code other than 0 from the library): the caller then goes through the checks in Python, which
 // raise the error or handle the case.
 
 #include <ATen/core/Tensor.h>
+#include <ATen/ops/empty.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <cmath>
+
 #include "b200_fp8_mm.h"
+#include "b200_mla_cache.h"
 #include "b200_mla_consumers.h"
 
 namespace {
@@ -22,6 +26,11 @@ decltype(&b200_fp8_mm_strided) g_strided = nullptr;
 decltype(&b200_fp8_mm_grouped) g_grouped = nullptr;
 decltype(&b200_mla_rope) g_rope = nullptr;
 decltype(&b200_mla_div_softmax) g_softmax = nullptr;
+decltype(&b200_mla_cache_append) g_append = nullptr;
+decltype(&b200_mla_cache_attend) g_attend = nullptr;
+decltype(&b200_mla_cache_attend_workspace_bytes) g_attend_workspace = nullptr;
+decltype(&b200_mla_cache_evict) g_evict = nullptr;
+decltype(&b200_mla_cache_evict_workspace_bytes) g_evict_workspace = nullptr;
 
 constexpr int64_t kScaleBlock = 128;
 
@@ -189,6 +198,204 @@ bool run_softmax(PyObject* const* args) {
                    static_cast<int>(v[3]), static_cast<int>(v[4]), stream);
 }
 
+// ---- Operators around a paged latent cache: the checks of mla_cache.py
+
+// No two elements share an address.
+bool distinct(const at::Tensor& t) {
+  int64_t need = 1;
+  bool used[3] = {};
+  for (int64_t round = 0; round < t.dim(); ++round) {
+    int64_t best = -1;
+    for (int64_t i = 0; i < t.dim(); ++i)
+      if (!used[i] && (best < 0 || t.stride(i) < t.stride(best))) best = i;
+    used[best] = true;
+    if (t.size(best) <= 1) continue;
+    if (t.stride(best) < need) return false;
+    need += t.stride(best) * (t.size(best) - 1);
+  }
+  return true;
+}
+
+// The bytes from the first to behind the last element do not meet. (Where they do, Python looks closer.)
+bool apart(const at::Tensor& a, const at::Tensor& b) {
+  auto end = [](const at::Tensor& t) {
+    int64_t n = 1;
+    for (int64_t i = 0; i < t.dim(); ++i) n += t.stride(i) * (t.size(i) - 1);
+    return static_cast<const char*>(t.data_ptr()) + n * static_cast<int64_t>(t.element_size());
+  };
+  return end(a) <= static_cast<const char*>(b.data_ptr()) || end(b) <= static_cast<const char*>(a.data_ptr());
+}
+
+bool same(const at::Tensor& a, const at::Tensor& b) {
+  return a.data_ptr() == b.data_ptr() && a.sizes() == b.sizes() && a.strides() == b.strides();
+}
+
+struct CacheCall {
+  b200_mla_cache c;
+  const at::Tensor* cache;
+  int64_t batch, capacity, d;
+  c10::DeviceIndex dev;
+};
+
+bool cache_call(PyObject* cache_arg, PyObject* table_arg, PyObject* lens_arg, long long dv, CacheCall* out) {
+  const at::Tensor *cache = plain_tensor(cache_arg), *table = plain_tensor(table_arg), *lens = plain_tensor(lens_arg);
+  if (!cache || !table || !lens) return false;
+  const c10::DeviceIndex dev = c10::cuda::current_device();
+  const auto type = cache->scalar_type();
+  if ((type != at::kBFloat16 && type != at::kHalf) || !is_cuda(*cache, type, 3, dev) || !is_cuda(*table, at::kInt, 2, dev) ||
+      !is_cuda(*lens, at::kInt, 1, dev))
+    return false;
+  const int64_t pages = cache->size(0), ps = cache->size(1), d = cache->size(2), batch = table->size(0), per = table->size(1);
+  if (dv < 128 || dv > 512 || dv % 128 != 0 || d < dv || d > 576 || d % 64 != 0 || pages <= 0 || ps <= 0 || !fits_int(pages) || !fits_int(ps))
+    return false;
+  if (cache->stride(2) != 1 || cache->stride(0) % 8 != 0 || cache->stride(1) % 8 != 0 || cache->stride(0) < d || cache->stride(1) < d ||
+      !aligned16(*cache))
+    return false;
+  if (per <= 0 || table->stride(1) != 1 || batch <= 0 || batch >= 65536 || lens->size(0) != batch || (batch > 1 && lens->stride(0) != 1) ||
+      per > (1 << 30) / ps)
+    return false;
+  out->c = b200_mla_cache{cache->data_ptr(), static_cast<const int*>(table->data_ptr()), static_cast<const int*>(lens->data_ptr()),
+                          type == at::kBFloat16 ? B200_MLA_CACHE_BF16 : B200_MLA_CACHE_FP16, static_cast<int>(pages), static_cast<int>(ps),
+                          static_cast<int>(dv), static_cast<int>(d - dv), static_cast<int>(batch), static_cast<int>(per),
+                          cache->stride(0), cache->stride(1), table->stride(0)};
+  out->cache = cache;
+  out->batch = batch;
+  out->capacity = per * ps;
+  out->d = d;
+  out->dev = dev;
+  return true;
+}
+
+// A value per slot of every sequence.
+bool slots(const at::Tensor* t, c10::ScalarType type, const CacheCall& k) {
+  return t && is_cuda(*t, type, 2, k.dev) && t->size(0) == k.batch && t->size(1) >= k.capacity && t->stride(1) == 1;
+}
+
+bool head_rows(const at::Tensor* t, const CacheCall& k, int64_t width) {
+  return t && is_cuda(*t, k.cache->scalar_type(), 3, k.dev) && t->size(0) == k.batch && t->size(1) > 0 && t->size(2) == width && t->stride(2) == 1;
+}
+
+bool number(PyObject* o, double* out) {
+  if (!PyFloat_CheckExact(o) && !PyLong_CheckExact(o)) return false;
+  *out = PyFloat_AsDouble(o);
+  return std::isfinite(*out) && !PyErr_Occurred();
+}
+
+// mla_cache_append(row, position, cache, block_table, lens, dv, theta, q, q_out, score, slot_position), the last four maybe None
+bool run_append(PyObject* const* args) {
+  CacheCall k;
+  long long dv;
+  double theta;
+  if (!ints(args + 5, 1, 1 << 20, &dv) || !number(args[6], &theta) || theta <= 0 || !cache_call(args[2], args[3], args[4], dv, &k)) return false;
+  const at::Tensor *row = plain_tensor(args[0]), *position = plain_tensor(args[1]);
+  if (!row || !position || !is_cuda(*row, k.cache->scalar_type(), 2, k.dev) || row->size(0) != k.batch || row->size(1) != k.d || row->stride(1) != 1 ||
+      !is_cuda(*position, at::kInt, 1, k.dev) || position->size(0) != k.batch || (k.batch > 1 && position->stride(0) != 1))
+    return false;
+  if (!distinct(*k.cache) || !apart(*row, *k.cache)) return false;
+  const at::Tensor *q = nullptr, *q_out = nullptr, *score = nullptr, *at_slot = nullptr;
+  if (args[7] != Py_None) {
+    q = plain_tensor(args[7]);
+    q_out = args[8] != Py_None ? plain_tensor(args[8]) : q;
+    if (!head_rows(q, k, k.d) || !head_rows(q_out, k, k.d) || q->size(1) != q_out->size(1) || q->size(1) > (1 << 20) || !distinct(*q_out) ||
+        !(same(*q, *q_out) || apart(*q, *q_out)) || !apart(*q_out, *row) || !apart(*q_out, *k.cache) || !apart(*q, *k.cache))
+      return false;
+  } else if (args[8] != Py_None) {
+    return false;
+  }
+  if (args[9] != Py_None && (!slots(score = plain_tensor(args[9]), at::kFloat, k) || !distinct(*score))) return false;
+  if (args[10] != Py_None && (!slots(at_slot = plain_tensor(args[10]), at::kInt, k) || !distinct(*at_slot))) return false;
+  cudaStream_t stream = c10::cuda::getCurrentCUDAStream(k.dev).stream();
+  return launched(g_append, static_cast<const b200_mla_cache*>(&k.c), row->data_ptr(), static_cast<long long>(row->stride(0)),
+                  static_cast<const int*>(position->data_ptr()), theta, q ? q->data_ptr() : nullptr, q ? static_cast<long long>(q->stride(0)) : 0,
+                  q ? static_cast<long long>(q->stride(1)) : 0, q_out ? q_out->data_ptr() : nullptr,
+                  q_out ? static_cast<long long>(q_out->stride(0)) : 0, q_out ? static_cast<long long>(q_out->stride(1)) : 0,
+                  q ? static_cast<int>(q->size(1)) : 0, score ? static_cast<float*>(score->data_ptr()) : nullptr,
+                  score ? static_cast<long long>(score->stride(0)) : 0, at_slot ? static_cast<int*>(at_slot->data_ptr()) : nullptr,
+                  at_slot ? static_cast<long long>(at_slot->stride(0)) : 0, stream);
+}
+
+// mla_cache_attend(q, cache, block_table, lens, dv, scale, out, score, score_out, max_len, return_lse, status); out, score, score_out and
+// max_len maybe None. Returns out, or (out, lse).
+PyObject* run_attend(PyObject* const* args) {
+  CacheCall k;
+  long long dv, most;
+  double scale;
+  if (!ints(args + 4, 1, 1 << 20, &dv) || !number(args[5], &scale) || !cache_call(args[1], args[2], args[3], dv, &k)) return nullptr;
+  const at::Tensor* q = plain_tensor(args[0]);
+  if (!head_rows(q, k, k.d) || q->size(1) > (1 << 16) || !aligned16(*q)) return nullptr;
+  for (int i = 0; i < 2; ++i)
+    if (q->size(i) > 1 && (q->stride(i) % 8 != 0 || q->stride(i) < k.d)) return nullptr;
+  most = k.capacity;
+  if (args[9] != Py_None && (!ints(args + 9, 1, 1ll << 40, &most) || most <= 0)) return nullptr;
+  if (most > k.capacity) most = k.capacity;
+  if (args[10] != Py_True && args[10] != Py_False) return nullptr;
+  at::Tensor out, lse;
+  if (args[6] != Py_None) {
+    const at::Tensor* given = plain_tensor(args[6]);
+    if (!head_rows(given, k, dv) || given->size(1) != q->size(1) || !distinct(*given) || !apart(*given, *q) || !apart(*given, *k.cache)) return nullptr;
+    out = *given;
+  }
+  const at::Tensor *score = nullptr, *score_out = nullptr;
+  if (args[7] != Py_None) {
+    score = plain_tensor(args[7]);
+    score_out = args[8] != Py_None ? plain_tensor(args[8]) : score;
+    if (!slots(score, at::kFloat, k) || !slots(score_out, at::kFloat, k) || !distinct(*score_out) || !(same(*score, *score_out) || apart(*score, *score_out)))
+      return nullptr;
+  } else if (args[8] != Py_None) {
+    return nullptr;
+  }
+  const at::Tensor* st = lookup(args[11], PyLong_FromLong(k.dev));
+  if (st == nullptr) return nullptr;
+  const int heads = static_cast<int>(q->size(1));
+  // All of torch's allocator on the current stream, as in Python.
+  if (!out.defined()) out = at::empty({k.batch, heads, dv}, q->options());
+  if (args[10] == Py_True) lse = at::empty({k.batch, heads}, q->options().dtype(at::kFloat));
+  const size_t bytes = g_attend_workspace(static_cast<int>(k.batch), heads, static_cast<int>(dv), static_cast<int>(k.d - dv), static_cast<int>(most), score != nullptr);
+  const at::Tensor ws = at::empty({static_cast<int64_t>(bytes)}, q->options().dtype(at::kByte));
+  cudaStream_t stream = c10::cuda::getCurrentCUDAStream(k.dev).stream();
+  if (!launched(g_attend, static_cast<const b200_mla_cache*>(&k.c), q->data_ptr(), static_cast<long long>(q->stride(0)), static_cast<long long>(q->stride(1)),
+                heads, static_cast<float>(scale), out.data_ptr(), static_cast<long long>(out.stride(0)), static_cast<long long>(out.stride(1)),
+                lse.defined() ? static_cast<float*>(lse.data_ptr()) : nullptr, score ? static_cast<const float*>(score->data_ptr()) : nullptr,
+                score ? static_cast<long long>(score->stride(0)) : 0, score ? static_cast<float*>(score_out->data_ptr()) : nullptr,
+                score ? static_cast<long long>(score_out->stride(0)) : 0, static_cast<int>(most), ws.data_ptr(), bytes,
+                static_cast<int*>(st->data_ptr()), stream))
+    return nullptr;
+  PyObject* o = THPVariable_Wrap(out);
+  if (o == nullptr || !lse.defined()) return o;
+  PyObject* l = THPVariable_Wrap(lse);
+  if (l == nullptr) {
+    Py_DECREF(o);
+    return nullptr;
+  }
+  PyObject* both = PyTuple_Pack(2, o, l);
+  Py_DECREF(o);
+  Py_DECREF(l);
+  return both;
+}
+
+// mla_cache_evict(cache, block_table, lens, score, slot_position, budget, recent, lens_out, score_out, position_out)
+bool run_evict(PyObject* const* args) {
+  CacheCall k;
+  long long v[2];
+  if (!ints(args + 5, 2, 0x7fffffff, v) || v[0] <= 0 || v[1] < 0 || v[1] > v[0] || !cache_call(args[0], args[1], args[2], 128, &k)) return false;
+  const at::Tensor *lens = plain_tensor(args[2]), *score = plain_tensor(args[3]), *at_slot = plain_tensor(args[4]), *lens_out = plain_tensor(args[7]),
+                   *score_out = plain_tensor(args[8]), *at_out = plain_tensor(args[9]);
+  if (!lens_out || !is_cuda(*lens_out, at::kInt, 1, k.dev) || lens_out->size(0) != k.batch || (k.batch > 1 && lens_out->stride(0) != 1)) return false;
+  if (!slots(score, at::kFloat, k) || !slots(score_out, at::kFloat, k) || !slots(at_slot, at::kInt, k) || !slots(at_out, at::kInt, k)) return false;
+  if (!distinct(*k.cache) || !distinct(*score_out) || !distinct(*at_out)) return false;
+  if (!(same(*lens, *lens_out) || apart(*lens, *lens_out)) || !(same(*score, *score_out) || apart(*score, *score_out)) ||
+      !(same(*at_slot, *at_out) || apart(*at_slot, *at_out)))
+    return false;
+  const size_t bytes = g_evict_workspace(static_cast<int>(k.batch), static_cast<int>(k.capacity), static_cast<int>(v[0]));
+  const at::Tensor ws = at::empty({static_cast<int64_t>(bytes)}, score->options().dtype(at::kByte));
+  cudaStream_t stream = c10::cuda::getCurrentCUDAStream(k.dev).stream();
+  return launched(g_evict, static_cast<const b200_mla_cache*>(&k.c), static_cast<const float*>(score->data_ptr()), static_cast<long long>(score->stride(0)),
+                  static_cast<const int*>(at_slot->data_ptr()), static_cast<long long>(at_slot->stride(0)), static_cast<int>(v[0]),
+                  static_cast<int>(v[1]), static_cast<int*>(lens_out->data_ptr()), static_cast<float*>(score_out->data_ptr()),
+                  static_cast<long long>(score_out->stride(0)), static_cast<int*>(at_out->data_ptr()), static_cast<long long>(at_out->stride(0)),
+                  ws.data_ptr(), bytes, stream);
+}
+
 // A C++ exception (a tensor without storage, a device that is gone) is "not the plain case" too.
 // The last `Optional` of the N arguments may be left out (null).
 template <bool (*F)(PyObject* const*), Py_ssize_t N, Py_ssize_t Optional = 0>
@@ -208,6 +415,44 @@ PyObject* entry(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     }
   }
   return PyBool_FromLong(done);
+}
+
+// The same for a function that returns its results, or null.
+template <PyObject* (*F)(PyObject* const*), Py_ssize_t N>
+PyObject* results(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  PyObject* found = nullptr;
+  if (nargs == N) {
+    try {
+      found = F(args);
+    } catch (...) {
+      found = nullptr;
+    }
+    if (PyErr_Occurred()) {
+      PyErr_Clear();
+      Py_CLEAR(found);
+    }
+  }
+  if (found != nullptr) return found;
+  Py_RETURN_FALSE;
+}
+
+// bind_cache(append, attend, attend_workspace_bytes, evict, evict_workspace_bytes): addresses of the loaded library's functions.
+PyObject* bind_cache(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  void* f[5];
+  if (nargs != 5) {
+    PyErr_SetString(PyExc_TypeError, "bind_cache takes five addresses");
+    return nullptr;
+  }
+  for (int i = 0; i < 5; ++i) {
+    f[i] = PyLong_AsVoidPtr(args[i]);
+    if (PyErr_Occurred()) return nullptr;
+  }
+  g_append = reinterpret_cast<decltype(g_append)>(f[0]);
+  g_attend = reinterpret_cast<decltype(g_attend)>(f[1]);
+  g_attend_workspace = reinterpret_cast<decltype(g_attend_workspace)>(f[2]);
+  g_evict = reinterpret_cast<decltype(g_evict)>(f[3]);
+  g_evict_workspace = reinterpret_cast<decltype(g_evict_workspace)>(f[4]);
+  Py_RETURN_NONE;
 }
 
 // bind(strided, grouped, rope, softmax): addresses of the loaded library's functions.
@@ -239,6 +484,10 @@ PyMethodDef methods[] = {
     {"fp8_mm_grouped", fast<entry<run_grouped, 7>>(), METH_FASTCALL, nullptr},
     {"mla_decode", fast<entry<run_rope, 12>>(), METH_FASTCALL, nullptr},
     {"div_softmax", fast<entry<run_softmax, 6>>(), METH_FASTCALL, nullptr},
+    {"bind_cache", fast<bind_cache>(), METH_FASTCALL, nullptr},
+    {"mla_cache_append", fast<entry<run_append, 11>>(), METH_FASTCALL, nullptr},
+    {"mla_cache_attend", fast<results<run_attend, 12>>(), METH_FASTCALL, nullptr},
+    {"mla_cache_evict", fast<entry<run_evict, 10>>(), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -52,8 +52,8 @@ __device__ __forceinline__ int rows_of(const CacheView& c, int b, int most) { re
 // Append
 // ---------------------------------------------------------------------------------------------
 
-constexpr int kAppendThreads = 128;
-constexpr int kAppendHeads = 4;  // query heads per CTA
+constexpr int kAppendThreads = 256;
+constexpr int kAppendHeads = 8;  // query heads per CTA
 constexpr int kMaxPairs = 224;   // dr / 2
 
 struct AppendParams {
@@ -67,29 +67,70 @@ struct AppendParams {
   long long row_stride, q_sb, q_sh, qo_sb, qo_sh, score_stride, slot_position_stride;
   int heads, half;
   int copy;      // the elements before the rotated ones go to q_out too (0: q_out is q)
-  int vec;       // every row of q, q_out and `row` starts on a 16-byte boundary
   double turns[kMaxPairs];  // theta^(-2t/dr) / (2 pi): turns per position
 };
 
-// dst[0..dv + 2 half) = src with its last 2 half elements rotated; all threads of the CTA. src may be dst (copy = 0).
 template <typename T, bool VEC>
-__device__ __forceinline__ void rotate_rows(const T* src, long long src_step, T* dst, long long dst_step, int rows, int dv, int half,
-                                            bool copy, const float2* cs) {
-  constexpr int E = VEC ? 8 : 1;
-  struct alignas(sizeof(T) * E) Piece {
-    T v[E];
-  };
-  const int nope = copy ? dv / E : 0, pairs = half / E, each = nope + pairs;
-  for (int i = static_cast<int>(threadIdx.x); i < rows * each; i += kAppendThreads) {
+struct Piece;
+template <typename T>
+struct alignas(16) Piece<T, true> {
+  static constexpr int E = 8;
+  T v[8];
+};
+template <typename T>
+struct Piece<T, false> {
+  static constexpr int E = 1;
+  T v[1];
+};
+
+// `rows` rows of dv + 2 half elements from src to dst (which may be src, then copy = false), the last 2 half rotated for `position`.
+// The unrotated elements, most of the bytes, are on their way while the angles are worked out.
+template <typename T, bool VEC>
+__device__ __forceinline__ void rotate_rows(const AppendParams& p, const T* src, long long src_step, T* dst, long long dst_step, int rows, int dv,
+                                            bool copy, int position, float2* cs) {
+  using P = Piece<T, VEC>;
+  constexpr int E = P::E, kAhead = 2;
+  const int tid = static_cast<int>(threadIdx.x), half = p.half, each = dv / E, nope = copy ? rows * each : 0;
+  auto at = [&](int i, const T** s, T** o) {
     const int r = i / each, k = i - r * each;
-    const T* s = src + r * src_step;
-    T* o = dst + r * dst_step;
-    if (k < nope) {
-      *reinterpret_cast<Piece*>(o + k * E) = *reinterpret_cast<const Piece*>(s + k * E);
-      continue;
-    }
-    const int t = (k - nope) * E;
-    Piece a = *reinterpret_cast<const Piece*>(s + dv + t), b = *reinterpret_cast<const Piece*>(s + dv + half + t);
+    *s = src + r * src_step + k * E;
+    *o = dst + r * dst_step + k * E;
+  };
+  P ahead[kAhead];
+#pragma unroll
+  for (int n = 0; n < kAhead; ++n) {
+    const T* s;
+    T* o;
+    at(tid + n * kAppendThreads, &s, &o);
+    if (tid + n * kAppendThreads < nope) ahead[n] = *reinterpret_cast<const P*>(s);
+  }
+  for (int t = tid; t < half; t += kAppendThreads) {
+    // In 64 bits up to the whole turns, which no function of the angle sees: position 10^6 leaves 32 bits with two digits.
+    const double turns = position * p.turns[t];
+    float sn, co;
+    sincospif(2.0f * static_cast<float>(turns - rint(turns)), &sn, &co);
+    cs[t] = make_float2(co, sn);
+  }
+#pragma unroll
+  for (int n = 0; n < kAhead; ++n) {
+    const T* s;
+    T* o;
+    at(tid + n * kAppendThreads, &s, &o);
+    if (tid + n * kAppendThreads < nope) *reinterpret_cast<P*>(o) = ahead[n];
+  }
+  for (int i = tid + kAhead * kAppendThreads; i < nope; i += kAppendThreads) {
+    const T* s;
+    T* o;
+    at(i, &s, &o);
+    *reinterpret_cast<P*>(o) = *reinterpret_cast<const P*>(s);
+  }
+  __syncthreads();
+  const int pairs = half / E;
+  for (int i = tid; i < rows * pairs; i += kAppendThreads) {
+    const int r = i / pairs, t = (i - r * pairs) * E;
+    const T* s = src + r * src_step + dv + t;
+    T* o = dst + r * dst_step + dv + t;
+    P a = *reinterpret_cast<const P*>(s), b = *reinterpret_cast<const P*>(s + half);
 #pragma unroll
     for (int e = 0; e < E; ++e) {
       const float x1 = to_float(a.v[e]), x2 = to_float(b.v[e]);
@@ -97,51 +138,35 @@ __device__ __forceinline__ void rotate_rows(const T* src, long long src_step, T*
       from_float(x1 * w.x - x2 * w.y, &a.v[e]);
       from_float(x2 * w.x + x1 * w.y, &b.v[e]);
     }
-    *reinterpret_cast<Piece*>(o + dv + t) = a;
-    *reinterpret_cast<Piece*>(o + dv + half + t) = b;
+    *reinterpret_cast<P*>(o) = a;
+    *reinterpret_cast<P*>(o + half) = b;
   }
 }
 
-template <typename T>
+// Writes the new rows (the first CTA of a sequence) and rotates the queries (the others, kAppendHeads heads each).
+// Memory-bound where there are many heads: every element of q once in and once out. 128 sequences x 128 heads.
+template <typename T, bool VEC>
 __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_constant__ AppendParams p) {
   __shared__ float2 cs[kMaxPairs];
   pdl_wait();
   pdl_launch_dependents();
   const CacheView& c = p.cache;
-  const int b = static_cast<int>(blockIdx.y);
-  const int position = p.position[b];
-  for (int t = static_cast<int>(threadIdx.x); t < p.half; t += kAppendThreads) {
-    // In 64 bits up to the whole turns, which no function of the angle sees: position 10^6 leaves 32 bits with two digits.
-    const double turns = position * p.turns[t];
-    float s, co;
-    sincospif(2.0f * static_cast<float>(turns - rint(turns)), &s, &co);
-    cs[t] = make_float2(co, s);
-  }
-  __syncthreads();
+  const int b = static_cast<int>(blockIdx.y), position = p.position[b];
   if (blockIdx.x == 0) {
     const int j = c.lens[b];
     if (j < 0 || j >= c.capacity) return;
-    const long long at = slot_offset(c, b, j);
-    if (at < 0) return;
-    const T* src = static_cast<const T*>(p.row) + b * p.row_stride;
-    T* dst = static_cast<T*>(c.data) + at;
-    if (p.vec)
-      rotate_rows<T, true>(src, 0, dst, 0, 1, c.dv, p.half, true, cs);
-    else
-      rotate_rows<T, false>(src, 0, dst, 0, 1, c.dv, p.half, true, cs);
+    const long long to = slot_offset(c, b, j);
+    if (to < 0) return;
+    rotate_rows<T, VEC>(p, static_cast<const T*>(p.row) + b * p.row_stride, 0, static_cast<T*>(c.data) + to, 0, 1, c.dv, true, position, cs);
     if (threadIdx.x == 0) {
       if (p.score != nullptr) p.score[b * p.score_stride + j] = 0.f;
       if (p.slot_position != nullptr) p.slot_position[b * p.slot_position_stride + j] = position;
     }
     return;
   }
-  const int h0 = (static_cast<int>(blockIdx.x) - 1) * kAppendHeads, rows = min(kAppendHeads, p.heads - h0);
-  const T* src = static_cast<const T*>(p.q) + b * p.q_sb + h0 * p.q_sh;
-  T* dst = static_cast<T*>(p.q_out) + b * p.qo_sb + h0 * p.qo_sh;
-  if (p.vec)
-    rotate_rows<T, true>(src, p.q_sh, dst, p.qo_sh, rows, c.dv, p.half, p.copy != 0, cs);
-  else
-    rotate_rows<T, false>(src, p.q_sh, dst, p.qo_sh, rows, c.dv, p.half, p.copy != 0, cs);
+  const int h0 = (static_cast<int>(blockIdx.x) - 1) * kAppendHeads;
+  rotate_rows<T, VEC>(p, static_cast<const T*>(p.q) + b * p.q_sb + h0 * p.q_sh, p.q_sh, static_cast<T*>(p.q_out) + b * p.qo_sb + h0 * p.qo_sh,
+                      p.qo_sh, min(kAppendHeads, p.heads - h0), c.dv, p.copy != 0, position, cs);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -1027,6 +1052,11 @@ __global__ void __launch_bounds__(kScoreThreads) attend_score_kernel(const __gri
 
 constexpr int kSelectThreads = 1024;
 constexpr int kSelectWarps = kSelectThreads / 32;
+constexpr int kMaxCluster = 8;
+constexpr int kDigitBits = 11, kDigits = 3;     // of a rank: 11 + 11 + 10 bits
+constexpr int kBins = 1 << kDigitBits;
+constexpr int kMaxStaged = 32768;               // ranks of a CTA's slots that are kept in shared memory (128 KB)
+constexpr int kFewMoves = 64;                   // a sequence's rows that the selecting CTAs move themselves
 constexpr int kMoveThreads = 256;
 
 struct EvictParams {
@@ -1043,6 +1073,9 @@ struct EvictParams {
   int* late;     // [batch][most]: slots kept behind it, ascending
   int most;
   int vecs;      // 16-byte pieces of a row
+  int cluster;   // CTAs per sequence
+  int staged;    // ranks that fit the CTA's shared memory
+  int few;       // the selecting CTAs move the rows
 };
 
 // Order of the scores as unsigned integers: protected rows above all, NaN above every number, -0 as 0.
@@ -1053,111 +1086,208 @@ __device__ __forceinline__ uint32_t rank_of(float score, int position, long long
   return (u >> 31) ? ~u : (u | 0x80000000u);
 }
 
-// Exclusive sum over the warps' values v (one per warp, given by lane 0 through `scratch`), and the total.
-__device__ __forceinline__ int warps_before(int v, int* scratch, int* total) {
+// Exclusive sum of v over the CTA's threads, and the total.
+__device__ __forceinline__ int threads_before(int v, int* scratch, int* total) {
   const int warp = static_cast<int>(threadIdx.x) >> 5, lane = static_cast<int>(threadIdx.x) & 31;
-  __syncthreads();
-  if (lane == 0) scratch[warp] = v;
-  __syncthreads();
-  int before = 0, all = 0;
-  for (int w = 0; w < kSelectWarps; ++w) {
-    if (w < warp) before += scratch[w];
-    all += scratch[w];
+  int upto = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int u = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += u;
   }
-  *total = all;
-  return before;
+  __syncthreads();  // (scratch may still be read from the last time)
+  if (lane == 31) scratch[warp] = upto;
+  __syncthreads();
+  int w = scratch[lane];  // kSelectWarps = 32
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int u = __shfl_up_sync(0xffffffffu, w, o);
+    if (lane >= o) w += u;
+  }
+  *total = __shfl_sync(0xffffffffu, w, 31);
+  const int before = __shfl_sync(0xffffffffu, w, (warp + 31) & 31);
+  return (warp > 0 ? before : 0) + upto - v;
 }
+static_assert(kSelectWarps == 32, "threads_before sums one value per lane");
 
-// One CTA per sequence: the budget-th largest rank, eight bits at a time, then the slots to fill and the slots to move.
-__global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const __grid_constant__ EvictParams p) {
-  __shared__ int hist[256];
-  __shared__ int scratch[kSelectWarps];
-  __shared__ int found[2];
+__device__ __forceinline__ void move_row(const EvictParams& p, int b, int i, int lane) {
+  const CacheView& c = p.cache;
+  const int to = p.holes[static_cast<long long>(b) * p.most + i], of = p.late[static_cast<long long>(b) * p.most + i];
+  const long long dst = slot_offset(c, b, to), src = slot_offset(c, b, of);
+  if (dst >= 0) {
+    uint4* o = reinterpret_cast<uint4*>(static_cast<uint16_t*>(c.data) + dst);
+    const uint4* s = reinterpret_cast<const uint4*>(static_cast<uint16_t*>(c.data) + src);
+    uint4 v[3];  // 72 pieces at most
+#pragma unroll
+    for (int k = 0; k < 3; ++k) v[k] = src >= 0 && lane + 32 * k < p.vecs ? s[lane + 32 * k] : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+    for (int k = 0; k < 3; ++k)
+      if (lane + 32 * k < p.vecs) o[lane + 32 * k] = v[k];
+  }
+  if (lane == 0) {
+    p.score_out[b * p.score_out_stride + to] = p.score[b * p.score_stride + of];
+    p.position_out[b * p.position_out_stride + to] = p.position[b * p.position_stride + of];
+  }
+}
+static_assert(kMaxD / 8 <= 96, "move_row holds a row in three pieces a lane");
+
+// A cluster of CTAs per sequence, each with a run of its slots. Finds the budget-th largest rank, eleven bits at a time, then the slots
+// to fill and the slots to move, in order. Scores and positions are read once from memory and once from cache; from then on the ranks
+// lie in shared memory, and the CTAs of a cluster read each other's counts there. What it costs is a chain of some twenty barriers.
+__global__ void __launch_bounds__(kSelectThreads, 1) evict_select_kernel(const __grid_constant__ EvictParams p) {
+  extern __shared__ uint32_t ranks[];
+  __shared__ int bins[kDigits][kBins];
+  __shared__ int scratch[kSelectWarps], found[2], newest_here, totals[2];
+  const CacheView& c = p.cache;
+  const int tid = static_cast<int>(threadIdx.x), warp = tid >> 5, lane = tid & 31;
+  const int cluster = p.cluster, b = static_cast<int>(blockIdx.x) / cluster, me = static_cast<int>(blockIdx.x) % cluster, budget = p.budget;
+  auto sync = [&]() {
+    if (cluster == 1) {
+      __syncthreads();
+    } else {
+      asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+      asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    }
+  };
+  // The same variable of CTA `from` of the cluster.
+  auto of_cta = [&](const int* mine, int from) {
+    uint32_t at;
+    int v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(mine)), "r"(from));
+    asm volatile("ld.shared::cluster.b32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
+    return v;
+  };
+  for (int i = tid; i < kDigits * kBins; i += kSelectThreads) (&bins[0][0])[i] = 0;
   pdl_wait();
   pdl_launch_dependents();
-  const CacheView& c = p.cache;
-  const int b = static_cast<int>(blockIdx.x), tid = static_cast<int>(threadIdx.x), warp = tid >> 5, lane = tid & 31;
-  const int len = c.lens[b], n = rows_of(c, b, c.capacity), budget = p.budget;
+  const int len = c.lens[b], n = max(0, min(len, c.capacity));
   const float* score = p.score + b * p.score_stride;
   const int* position = p.position + b * p.position_stride;
   float* score_out = p.score_out + b * p.score_out_stride;
   int* position_out = p.position_out + b * p.position_out_stride;
-  __syncthreads();  // lens_out may be lens
-  if (tid == 0) p.lens_out[b] = min(len, budget);
+  sync();  // lens_out may be lens
+  if (me == 0 && tid == 0) p.lens_out[b] = min(len, budget);
   if (n <= budget) {
-    if (tid == 0) p.moves[b] = 0;
-    for (int i = tid; i < n; i += kSelectThreads) {
+    if (me == 0 && tid == 0) p.moves[b] = 0;
+    for (int i = me * kSelectThreads + tid; i < n; i += cluster * kSelectThreads) {
       score_out[i] = score[i];
       position_out[i] = position[i];
     }
     return;
   }
+  const int run = ((n + cluster - 1) / cluster + 31) / 32 * 32, begin = min(n, me * run), count = min(n, begin + run) - begin;
   int newest = INT_MIN;
-  for (int i = tid; i < n; i += kSelectThreads) newest = max(newest, position[i]);
+#pragma unroll 4
+  for (int i = tid; i < count; i += kSelectThreads) newest = max(newest, position[begin + i]);
   newest = __reduce_max_sync(0xffffffffu, newest);
   if (lane == 0) scratch[warp] = newest;
   __syncthreads();
-  for (int w = 0; w < kSelectWarps; ++w) newest = max(newest, scratch[w]);
+  newest = __reduce_max_sync(0xffffffffu, scratch[lane]);
+  if (tid == 0) newest_here = newest;
+  sync();
+  for (int k = 0; k < cluster; ++k) newest = max(newest, of_cta(&newest_here, k));
   const long long safe_above = static_cast<long long>(newest) - p.recent;
+  auto rank_at = [&](int i) { return i < p.staged ? ranks[i] : rank_of(score[begin + i], position[begin + i], safe_above); };
+#pragma unroll 4
+  for (int i = tid; i < count; i += kSelectThreads) {
+    const uint32_t r = rank_of(score[begin + i], position[begin + i], safe_above);
+    if (i < p.staged) ranks[i] = r;
+    atomicAdd(&bins[0][r >> (32 - kDigitBits)], 1);
+  }
   uint32_t bits = 0, mask = 0;
   int left = budget;  // of the rows that share `bits` under `mask`, how many are kept
-  for (int shift = 24; shift >= 0; shift -= 8) {
-    __syncthreads();
-    if (tid < 256) hist[tid] = 0;
-    __syncthreads();
-    for (int i = tid; i < n; i += kSelectThreads) {
-      const uint32_t r = rank_of(score[i], position[i], safe_above);
-      if ((r & mask) == bits) atomicAdd(&hist[(r >> shift) & 255], 1);
+  int bin = 0;
+  for (int digit = 0; digit < kDigits; ++digit) {
+    const int shift = digit < 2 ? 32 - kDigitBits * (digit + 1) : 0, width = digit < 2 ? kBins : 1 << (32 - 2 * kDigitBits);
+    if (digit > 0) {
+      for (int i = tid; i < count; i += kSelectThreads) {
+        const uint32_t r = rank_at(i);
+        if ((r & mask) == bits) atomicAdd(&bins[digit][(r >> shift) & (width - 1)], 1);
+      }
+    }
+    sync();
+    // Thread t has bins width - 1 - 2 t and the one below: counted from the top.
+    const int high = width - 1 - 2 * tid;
+    int n0 = 0, n1 = 0;
+    if (high > 0) {
+      for (int k = 0; k < cluster; ++k) {
+        n0 += of_cta(&bins[digit][high], k);
+        n1 += of_cta(&bins[digit][high - 1], k);
+      }
+    }
+    int total;
+    const int above = threads_before(n0 + n1, scratch, &total);
+    if (above < left && left <= above + n0 + n1) {
+      const bool second = left > above + n0;
+      found[0] = high - (second ? 1 : 0);
+      found[1] = above + (second ? n0 : 0);
     }
     __syncthreads();
-    if (tid == 0) {
-      int above = 0, v = 255;
-      while (above + hist[v] < left) above += hist[v--];
-      found[0] = v;
-      found[1] = above;
-    }
-    __syncthreads();
-    bits |= static_cast<uint32_t>(found[0]) << shift;
-    mask |= 255u << shift;
+    bin = found[0];
+    bits |= static_cast<uint32_t>(bin) << shift;
+    mask |= static_cast<uint32_t>(width - 1) << shift;
     left -= found[1];
+    __syncthreads();
   }
-  // A warp takes a run of slots, so that what it finds is in order. Of the rows at the threshold the first `left` stay.
-  const int run = (n + kSelectThreads - 1) / kSelectThreads * 32;
-  const int begin = min(n, warp * run), end = min(n, begin + run);
-  int total, ties = 0;
-  for (int i0 = begin; i0 < end; i0 += 32) {
-    const int i = i0 + lane;
-    ties += __popc(__ballot_sync(0xffffffffu, i < end && rank_of(score[i], position[i], safe_above) == bits));
+  // Of the rows at the threshold the first `left` stay. A thread takes a run of words of 32 slots; ties of the CTAs before this one are
+  // in their last counts.
+  int ties_before = 0;
+  for (int k = 0; k < me; ++k) ties_before += of_cta(&bins[kDigits - 1][bin], k);
+  const int words = (count + 31) / 32, per_warp = (words + kSelectWarps - 1) / kSelectWarps;
+  const int w0 = min(words, warp * per_warp), w1 = min(words, w0 + per_warp);
+  int total, mine = 0;
+  for (int w = w0; w < w1; ++w) {
+    const int i = 32 * w + lane;
+    mine += __popc(__ballot_sync(0xffffffffu, i < count && rank_at(i) == bits));
   }
-  const int ties_before = warps_before(ties, scratch, &total);
+  int seen0 = threads_before(lane == 0 ? mine : 0, scratch, &total);  // (lane 0's is the warp's)
+  seen0 = ties_before + __shfl_sync(0xffffffffu, seen0, 0);
   int holes_at = 0, late_at = 0;
   for (int pass = 0; pass < 2; ++pass) {
-    int seen = ties_before, holes = 0, late = 0;
-    for (int i0 = begin; i0 < end; i0 += 32) {
-      const int i = i0 + lane;
-      const uint32_t r = i < end ? rank_of(score[i], position[i], safe_above) : 0u;
-      const uint32_t tie = __ballot_sync(0xffffffffu, i < end && r == bits);
-      const uint32_t below = (1u << lane) - 1u;
-      const bool kept = i < end && (r > bits || (r == bits && seen + __popc(tie & below) < left));
+    int seen = seen0, holes = 0, late = 0;
+    for (int w = w0; w < w1; ++w) {
+      const int i = 32 * w + lane, slot = begin + i;
+      const uint32_t r = i < count ? rank_at(i) : 0u;
+      const uint32_t tie = __ballot_sync(0xffffffffu, i < count && r == bits), below = (1u << lane) - 1u;
+      const bool kept = i < count && (r > bits || (r == bits && seen + __popc(tie & below) < left));
       seen += __popc(tie);
-      const bool hole = i < end && !kept && i < budget, moved = kept && i >= budget;
+      const bool hole = i < count && !kept && slot < budget, moved = kept && slot >= budget;
       const uint32_t hm = __ballot_sync(0xffffffffu, hole), lm = __ballot_sync(0xffffffffu, moved);
       if (pass == 1) {
-        if (hole) p.holes[static_cast<long long>(b) * p.most + holes_at + holes + __popc(hm & below)] = i;
-        if (moved) p.late[static_cast<long long>(b) * p.most + late_at + late + __popc(lm & below)] = i;
-        if (kept && i < budget) {
-          score_out[i] = score[i];
-          position_out[i] = position[i];
+        if (hole) p.holes[static_cast<long long>(b) * p.most + holes_at + holes + __popc(hm & below)] = slot;
+        if (moved) p.late[static_cast<long long>(b) * p.most + late_at + late + __popc(lm & below)] = slot;
+        if (kept && slot < budget) {
+          score_out[slot] = score[slot];
+          position_out[slot] = position[slot];
         }
       }
       holes += __popc(hm);
       late += __popc(lm);
     }
     if (pass == 0) {
-      late_at = warps_before(late, scratch, &total);
-      holes_at = warps_before(holes, scratch, &total);
-      if (tid == 0) p.moves[b] = total;
+      int all_holes, all_late;
+      holes_at = threads_before(lane == 0 ? holes : 0, scratch, &all_holes);
+      late_at = threads_before(lane == 0 ? late : 0, scratch, &all_late);
+      if (tid == 0) {
+        totals[0] = all_holes;
+        totals[1] = all_late;
+      }
+      sync();
+      holes_at = __shfl_sync(0xffffffffu, holes_at, 0);
+      late_at = __shfl_sync(0xffffffffu, late_at, 0);
+      for (int k = 0; k < me; ++k) {
+        holes_at += of_cta(&totals[0], k);
+        late_at += of_cta(&totals[1], k);
+      }
+      if (me == cluster - 1 && tid == 0) p.moves[b] = holes_at + all_holes;
     }
+  }
+  sync();  // the lists are complete, and no CTA leaves while another reads its counts
+  if (p.few) {
+    int moves = 0;
+    for (int k = 0; k < cluster; ++k) moves += of_cta(&totals[0], k);
+    for (int i = me * kSelectWarps + warp; i < moves; i += cluster * kSelectWarps) move_row(p, b, i, lane);
+    sync();
   }
 }
 
@@ -1165,23 +1295,9 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const __gr
 __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const __grid_constant__ EvictParams p) {
   pdl_wait();
   pdl_launch_dependents();
-  const CacheView& c = p.cache;
-  const int b = static_cast<int>(blockIdx.y), lane = static_cast<int>(threadIdx.x) & 31;
-  const int warps = static_cast<int>(gridDim.x) * (kMoveThreads / 32);
-  const int moves = p.moves[b];
-  for (int i = static_cast<int>(blockIdx.x) * (kMoveThreads / 32) + (static_cast<int>(threadIdx.x) >> 5); i < moves; i += warps) {
-    const int to = p.holes[static_cast<long long>(b) * p.most + i], of = p.late[static_cast<long long>(b) * p.most + i];
-    const long long dst = slot_offset(c, b, to), src = slot_offset(c, b, of);
-    if (dst >= 0) {
-      uint4* o = reinterpret_cast<uint4*>(static_cast<uint16_t*>(c.data) + dst);
-      const uint4* s = reinterpret_cast<const uint4*>(static_cast<uint16_t*>(c.data) + src);
-      for (int v = lane; v < p.vecs; v += 32) o[v] = src >= 0 ? s[v] : make_uint4(0u, 0u, 0u, 0u);
-    }
-    if (lane == 0) {
-      p.score_out[b * p.score_out_stride + to] = p.score[b * p.score_stride + of];
-      p.position_out[b * p.position_out_stride + to] = p.position[b * p.position_stride + of];
-    }
-  }
+  const int b = static_cast<int>(blockIdx.y), warps = static_cast<int>(gridDim.x) * (kMoveThreads / 32), moves = p.moves[b];
+  for (int i = static_cast<int>(blockIdx.x) * (kMoveThreads / 32) + (static_cast<int>(threadIdx.x) >> 5); i < moves; i += warps)
+    move_row(p, b, i, static_cast<int>(threadIdx.x) & 31);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -1190,22 +1306,31 @@ __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const __grid_c
 
 // <<<grid, threads>>> on `stream`, allowed to begin under the kernel before it (see pdl_wait).
 template <typename... Params>
-int launch_pdl(void (*kernel)(Params...), dim3 grid, int threads, size_t smem, void* stream, const std::decay_t<Params>&... params) {
+int launch_clusters(void (*kernel)(Params...), int cluster, dim3 grid, int threads, size_t smem, void* stream, const std::decay_t<Params>&... params) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = dim3(static_cast<unsigned>(threads), 1, 1);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = static_cast<cudaStream_t>(stream);
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = static_cast<unsigned>(cluster);
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
   if (cudaLaunchKernelEx(&cfg, kernel, params...) != cudaSuccess) {
     (void)cudaGetLastError();
     return B200_FP8_MM_ERR_LAUNCH;
   }
   return B200_FP8_MM_OK;
+}
+
+template <typename... Params>
+int launch_pdl(void (*kernel)(Params...), dim3 grid, int threads, size_t smem, void* stream, const std::decay_t<Params>&... params) {
+  return launch_clusters(kernel, 1, grid, threads, smem, stream, params...);
 }
 
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
@@ -1338,16 +1463,15 @@ AttendFn attend_fn(bool bf16, int ht) {
   return ht == 16 ? attend_kernel<__half, 16> : ht == 32 ? attend_kernel<__half, 32> : attend_kernel<__half, 64>;
 }
 
-// Lets the kernel take all of an SM's shared memory, once per device.
-bool opt_in(AttendFn fn, bool bf16, int ht, int device) {
-  static std::atomic<bool> done[kMaxDevices][6];
-  std::atomic<bool>& d = done[device][(bf16 ? 0 : 3) + (ht == 16 ? 0 : ht == 32 ? 1 : 2)];
-  if (d.load(std::memory_order_relaxed)) return true;
-  if (cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem) != cudaSuccess) {
+// Lets a kernel take that much shared memory, once per device.
+template <typename Fn>
+bool opt_in(Fn fn, int bytes, std::atomic<bool>* done) {
+  if (done->load(std::memory_order_relaxed)) return true;
+  if (cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) {
     (void)cudaGetLastError();
     return false;
   }
-  d.store(true, std::memory_order_relaxed);
+  done->store(true, std::memory_order_relaxed);
   return true;
 }
 
@@ -1385,12 +1509,13 @@ int b200_mla_cache_append(const b200_mla_cache* cache, const void* row, long lon
   p.heads = q != nullptr ? heads : 0;
   p.half = cache->dr / 2;
   p.copy = q != q_out || q_sb != qo_sb || q_sh != qo_sh;
-  p.vec = aligned16(row) && row_stride % 8 == 0 &&
+  const bool vec = aligned16(row) && row_stride % 8 == 0 &&
           (q == nullptr || (aligned16(q) && aligned16(q_out) && q_sb % 8 == 0 && q_sh % 8 == 0 && qo_sb % 8 == 0 && qo_sh % 8 == 0));
   for (int t = 0; t < p.half; ++t) p.turns[t] = pow(theta, -static_cast<double>(t) / p.half) / 6.283185307179586476925;
   const dim3 grid(static_cast<unsigned>(1 + (p.heads + kAppendHeads - 1) / kAppendHeads), static_cast<unsigned>(cache->batch));
-  return cache->dtype == B200_MLA_CACHE_BF16 ? launch_pdl(append_kernel<__nv_bfloat16>, grid, kAppendThreads, 0, stream, p)
-                                             : launch_pdl(append_kernel<__half>, grid, kAppendThreads, 0, stream, p);
+  if (cache->dtype == B200_MLA_CACHE_BF16)
+    return launch_pdl(vec ? append_kernel<__nv_bfloat16, true> : append_kernel<__nv_bfloat16, false>, grid, kAppendThreads, 0, stream, p);
+  return launch_pdl(vec ? append_kernel<__half, true> : append_kernel<__half, false>, grid, kAppendThreads, 0, stream, p);
 }
 
 size_t b200_mla_cache_attend_workspace_bytes(int batch, int heads, int dv, int dr, int max_len, int with_score) {
@@ -1460,7 +1585,8 @@ int b200_mla_cache_attend(const b200_mla_cache* cache, const void* q, long long 
   row_dims.add(cache->pages, cache->page_stride, 1);
   if (!q_dims.encode(&q_map, q, bf16) || !row_dims.encode(&row_map, cache->data, bf16)) return B200_FP8_MM_ERR_DRIVER;
   const AttendFn fn = attend_fn(bf16, ht);
-  if (!opt_in(fn, bf16, ht, device)) return B200_FP8_MM_ERR_DRIVER;
+  static std::atomic<bool> opted[kMaxDevices][6];
+  if (!opt_in(fn, kMaxSmem, &opted[device][(bf16 ? 0 : 3) + (ht == 16 ? 0 : ht == 32 ? 1 : 2)])) return B200_FP8_MM_ERR_DRIVER;
   rc = launch_pdl(fn, dim3(static_cast<unsigned>(p.workers) * p.head_tiles), kAttendThreads, smem, stream, q_map, row_map, p);
   if (rc != B200_FP8_MM_OK) return rc;
   // Eight groups where a sequence has eight parts and more on average, one where most have one or two.
@@ -1507,8 +1633,18 @@ int b200_mla_cache_evict(const b200_mla_cache* cache, const float* score, long l
   p.holes = p.moves + cache->batch;
   p.late = p.holes + static_cast<size_t>(cache->batch) * p.most;
   p.vecs = p.cache.d / 8;
-  rc = launch_pdl(evict_select_kernel, dim3(static_cast<unsigned>(cache->batch)), kSelectThreads, 0, stream, p);
-  if (rc != B200_FP8_MM_OK || p.most == 0) return rc;
+  // CTAs per sequence: 2048 slots each where the batch leaves SMs for it.
+  p.cluster = 1;
+  while (p.cluster < kMaxCluster && 2 * p.cluster * cache->batch <= 148 && p.cache.capacity > 2048 * p.cluster) p.cluster *= 2;
+  const int slots = ((p.cache.capacity + p.cluster - 1) / p.cluster + 31) / 32 * 32;
+  p.staged = slots < kMaxStaged ? slots : kMaxStaged;
+  p.few = p.most <= kFewMoves;
+  const int device = current_device();
+  static std::atomic<bool> opted[kMaxDevices];
+  if (device < 0 || !opt_in(evict_select_kernel, kMaxStaged * 4, &opted[device])) return B200_FP8_MM_ERR_DRIVER;
+  rc = launch_clusters(evict_select_kernel, p.cluster, dim3(static_cast<unsigned>(cache->batch * p.cluster)), kSelectThreads,
+                       static_cast<size_t>(p.staged) * 4, stream, p);
+  if (rc != B200_FP8_MM_OK || p.most == 0 || p.few) return rc;
   const int want = (p.most + kMoveThreads / 32 - 1) / (kMoveThreads / 32);
   const int fill = (148 * 8 + cache->batch - 1) / cache->batch;
   const dim3 grid(static_cast<unsigned>(want < fill ? want : fill), static_cast<unsigned>(cache->batch));

@@ -16,7 +16,7 @@ import math
 import torch
 
 from . import _lib
-from .fp8_mm import Fp8MmError, _check, _status_words
+from .fp8_mm import Fp8MmError, _check, _status, _status_words
 
 _TYPES = {torch.bfloat16: 0, torch.float16: 1}
 
@@ -120,6 +120,9 @@ def mla_cache_append(row, position, cache, block_table, lens, dv: int, theta: fl
     the others are copied). score (float32) and slot_position (int32), [batch, slots], optional: the new slot's entries become 0
     and position[b]. The rotation pairs element t with t + dr/2, angle position * theta**(-2t/dr), and unlike `mla_decode`
     neither rounds the angle nor the products to bf16: one rounding, at the end. Returns q_out."""
+    if _lib.host_calls().mla_cache_append(row, position, cache, block_table, lens, dv, theta, q, q_out, score, slot_position):
+        return q if q_out is None else q_out
+    # Not the plain case, or a call that will be refused: the same checks here, with their errors.
     batch, capacity = _check_cache(cache, block_table, lens, dv)
     d = cache.shape[2]
     _check(_distinct(cache), "cache must not overlap itself")
@@ -173,7 +176,13 @@ def mla_cache_attend(q, cache, block_table, lens, dv: int, scale: float, out=Non
     is never looked at. lens above the block table's capacity count as the capacity; a page that is not one of the cache's reads
     as rows of zeros. score (float32 [batch, slots]), optional: score_out[b, j] = score[b, j] + the weights that slot j received
     from all heads (score_out default: score itself), j < lens[b]; other entries are left as they were. max_len, optional: no
-    sequence is longer (longer ones are cut to it); it sizes the scratch that the weights need, batch * heads * max_len floats."""
+    sequence is longer (longer ones are cut to it); it sizes the scratch that the weights need, batch * heads * max_len floats.
+
+    Sums, maxima and joins are in 32 bits; the weights are rounded to the cache's type before they meet the values. A call repeats to
+    the bit. Where a long sequence is split depends on the other sequences' lengths, and so does the order of its sums."""
+    done = _lib.host_calls().mla_cache_attend(q, cache, block_table, lens, dv, scale, out, score, score_out, max_len, return_lse, _status)
+    if done is not False:
+        return done
     batch, capacity = _check_cache(cache, block_table, lens, dv)
     d = cache.shape[2]
     _check_heads("q", q, cache, batch, d)
@@ -231,13 +240,15 @@ def mla_cache_evict(cache, block_table, lens, score, slot_position, budget: int,
     score_out and position_out default to the inputs themselves. Slots are in no particular order afterwards, which no
     attention over rotated rows can tell; what lies behind the budget is left as it was, and its pages are free. A page with
     slots below the budget must belong to one sequence alone."""
+    lens_out = lens if lens_out is None else lens_out
+    score_out = score if score_out is None else score_out
+    position_out = slot_position if position_out is None else position_out
+    if _lib.host_calls().mla_cache_evict(cache, block_table, lens, score, slot_position, budget, recent, lens_out, score_out, position_out):
+        return lens_out
     batch, capacity = _check_cache(cache, block_table, lens, dv=128)
     _check(_distinct(cache), "cache must not overlap itself")
     _check(isinstance(budget, int) and isinstance(recent, int) and 0 < budget < 1 << 31 and 0 <= recent <= budget,
            "budget must be positive and recent between 0 and budget")
-    lens_out = lens if lens_out is None else lens_out
-    score_out = score if score_out is None else score_out
-    position_out = slot_position if position_out is None else position_out
     _check(lens_out.dtype == torch.int32 and tuple(lens_out.shape) == (batch,) and (batch < 2 or lens_out.stride(0) == 1),
            "lens_out must be contiguous int32 [batch]")
     for name, t, dtype in (("score", score, torch.float32), ("slot_position", slot_position, torch.int32),

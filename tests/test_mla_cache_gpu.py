@@ -549,3 +549,29 @@ def test_decode_loop(captured):
             assert torch.equal(held, torch.stack(rows[i]))
             assert torch.equal(at[i, :len(took)], at0[i, torch.tensor(took, device="cuda")])
     check_device_status()
+
+
+def test_results_without_the_native_module(monkeypatch):
+    """The Python checks and ctypes calls do what the native module does."""
+    from amd_developer_challenge_2025_b200 import _lib
+
+    def all_calls():
+        bt = Batch([70, 0, 33], 5, 128, 64, 16, seed=41, spare=16)
+        score, at = bt.slots(1.0), bt.slots(0, torch.int32)
+        at[:] = torch.arange(bt.capacity, device="cuda")
+        row = torch.randn(3, bt.d, generator=bt.g, device="cuda").to(bt.dtype)
+        found = [pkg.mla_cache_append(row, bt.lens.clone(), bt.cache, bt.table, bt.lens, 128, 5000.0, bt.q, torch.empty_like(bt.q), score, at)]
+        bt.lens += 1
+        found += [*bt.attend(return_lse=True, score=score, max_len=80), bt.attend(out=torch.empty(3, 5, 128, dtype=bt.dtype, device="cuda"))]
+        found += [pkg.mla_cache_evict(bt.cache, bt.table, bt.lens, score, at, 20, 4), score, at, bt.cache.nan_to_num(7.0)]
+        return found
+
+    want = all_calls()
+    monkeypatch.setattr(_lib, "_host", _lib._PythonChecks)
+    for g, w in zip(all_calls(), want):
+        assert g.shape == w.shape and g.dtype == w.dtype and torch.equal(g, w)
+
+
+@pytest.mark.parametrize("batch,n,budget", [(1, 70001, 30000), (3, 9000, 4000), (20, 5000, 64), (150, 300, 290), (1, 300000, 17)])
+def test_evict_shapes_of_clusters(batch, n, budget):
+    run_evict([n - i for i in range(batch)], budget, budget // 3, page=64, seed=n, in_place=True)
