@@ -1050,11 +1050,7 @@ __global__ void __launch_bounds__(kScoreThreads) attend_score_kernel(const __gri
 // Evict
 // ---------------------------------------------------------------------------------------------
 
-constexpr int kSelectThreads = 1024;
-constexpr int kSelectWarps = kSelectThreads / 32;
 constexpr int kMaxCluster = 8;
-constexpr int kDigitBits = 11, kDigits = 3;     // of a rank: 11 + 11 + 10 bits
-constexpr int kBins = 1 << kDigitBits;
 constexpr int kMaxStaged = 32768;               // ranks of a CTA's slots that are kept in shared memory (128 KB)
 constexpr int kFewMoves = 64;                   // a sequence's rows that the selecting CTAs move themselves
 constexpr int kMoveThreads = 256;
@@ -1087,7 +1083,9 @@ __device__ __forceinline__ uint32_t rank_of(float score, int position, long long
 }
 
 // Exclusive sum of v over the CTA's threads, and the total.
+template <int THREADS>
 __device__ __forceinline__ int threads_before(int v, int* scratch, int* total) {
+  constexpr int kWarps = THREADS / 32;
   const int warp = static_cast<int>(threadIdx.x) >> 5, lane = static_cast<int>(threadIdx.x) & 31;
   int upto = v;
 #pragma unroll
@@ -1098,17 +1096,16 @@ __device__ __forceinline__ int threads_before(int v, int* scratch, int* total) {
   __syncthreads();  // (scratch may still be read from the last time)
   if (lane == 31) scratch[warp] = upto;
   __syncthreads();
-  int w = scratch[lane];  // kSelectWarps = 32
+  int w = lane < kWarps ? scratch[lane] : 0;
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
+  for (int o = 1; o < kWarps; o <<= 1) {
     const int u = __shfl_up_sync(0xffffffffu, w, o);
     if (lane >= o) w += u;
   }
-  *total = __shfl_sync(0xffffffffu, w, 31);
+  *total = __shfl_sync(0xffffffffu, w, kWarps - 1);
   const int before = __shfl_sync(0xffffffffu, w, (warp + 31) & 31);
   return (warp > 0 ? before : 0) + upto - v;
 }
-static_assert(kSelectWarps == 32, "threads_before sums one value per lane");
 
 __device__ __forceinline__ void move_row(const EvictParams& p, int b, int i, int lane) {
   const CacheView& c = p.cache;
@@ -1131,13 +1128,20 @@ __device__ __forceinline__ void move_row(const EvictParams& p, int b, int i, int
 }
 static_assert(kMaxD / 8 <= 96, "move_row holds a row in three pieces a lane");
 
-// A cluster of CTAs per sequence, each with a run of its slots. Finds the budget-th largest rank, eleven bits at a time, then the slots
+// A cluster of CTAs per sequence, each with a run of its slots. Finds the budget-th largest rank, as many bits at a time as two bins to
+// a thread allow (9 of 256 threads, 11 of 1024), then the slots
 // to fill and the slots to move, in order. Scores and positions are read once from memory and once from cache; from then on the ranks
-// lie in shared memory, and the CTAs of a cluster read each other's counts there. What it costs is a chain of some twenty barriers.
-__global__ void __launch_bounds__(kSelectThreads, 1) evict_select_kernel(const __grid_constant__ EvictParams p) {
+// lie in shared memory, and the CTAs of a cluster read each other's counts there. What it costs is a chain of some thirty barriers,
+// which are dearer the more threads wait: one slot after the other is cheaper up to 4096 slots of a CTA.
+template <int THREADS>
+__global__ void __launch_bounds__(THREADS, 1) evict_select_kernel(const __grid_constant__ EvictParams p) {
+  constexpr int kWarps = THREADS / 32, kBins = 2 * THREADS, kDigitBits = THREADS == 256 ? 9 : 11, kDigits = (32 + kDigitBits - 1) / kDigitBits;
+  static_assert(kBins == 1 << kDigitBits, "two bins to a thread");
   extern __shared__ uint32_t ranks[];
-  __shared__ int bins[kDigits][kBins];
-  __shared__ int scratch[kSelectWarps], found[2], newest_here, totals[2];
+  __shared__ alignas(8) int bins[kDigits][kBins];
+  __shared__ alignas(8) int newest_of[kMaxCluster], totals[2];
+  __shared__ int scratch[kWarps], found[2];
+  __shared__ uint32_t above_words[THREADS], tie_words[THREADS];  // which of 32 slots lie above the threshold, and on it
   const CacheView& c = p.cache;
   const int tid = static_cast<int>(threadIdx.x), warp = tid >> 5, lane = tid & 31;
   const int cluster = p.cluster, b = static_cast<int>(blockIdx.x) / cluster, me = static_cast<int>(blockIdx.x) % cluster, budget = p.budget;
@@ -1149,15 +1153,23 @@ __global__ void __launch_bounds__(kSelectThreads, 1) evict_select_kernel(const _
       asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
     }
   };
-  // The same variable of CTA `from` of the cluster.
-  auto of_cta = [&](const int* mine, int from) {
-    uint32_t at;
-    int v;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(mine)), "r"(from));
-    asm volatile("ld.shared::cluster.b32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
-    return v;
+  // Two neighbouring values of the cluster's CTAs `from` to `to`, in sum. (All loads of a thread are on their way together.)
+  auto sum_over = [&](const int* mine, int from, int to) {
+    if (cluster == 1) return from < to ? *reinterpret_cast<const int2*>(mine) : make_int2(0, 0);
+    int2 v[kMaxCluster], s = make_int2(0, 0);
+#pragma unroll
+    for (int k = 0; k < kMaxCluster; ++k) {
+      v[k] = make_int2(0, 0);
+      if (k < from || k >= to) continue;
+      uint32_t at;
+      asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(mine)), "r"(k));
+      asm volatile("ld.shared::cluster.v2.b32 {%0, %1}, [%2];" : "=r"(v[k].x), "=r"(v[k].y) : "r"(at) : "memory");
+    }
+#pragma unroll
+    for (int k = 0; k < kMaxCluster; ++k) s.x += v[k].x, s.y += v[k].y;
+    return s;
   };
-  for (int i = tid; i < kDigits * kBins; i += kSelectThreads) (&bins[0][0])[i] = 0;
+  for (int i = tid; i < kDigits * kBins; i += THREADS) (&bins[0][0])[i] = 0;
   pdl_wait();
   pdl_launch_dependents();
   const int len = c.lens[b], n = max(0, min(len, c.capacity));
@@ -1169,7 +1181,7 @@ __global__ void __launch_bounds__(kSelectThreads, 1) evict_select_kernel(const _
   if (me == 0 && tid == 0) p.lens_out[b] = min(len, budget);
   if (n <= budget) {
     if (me == 0 && tid == 0) p.moves[b] = 0;
-    for (int i = me * kSelectThreads + tid; i < n; i += cluster * kSelectThreads) {
+    for (int i = me * THREADS + tid; i < n; i += cluster * THREADS) {
       score_out[i] = score[i];
       position_out[i] = position[i];
     }
@@ -1177,30 +1189,48 @@ __global__ void __launch_bounds__(kSelectThreads, 1) evict_select_kernel(const _
   }
   const int run = ((n + cluster - 1) / cluster + 31) / 32 * 32, begin = min(n, me * run), count = min(n, begin + run) - begin;
   int newest = INT_MIN;
-#pragma unroll 4
-  for (int i = tid; i < count; i += kSelectThreads) newest = max(newest, position[begin + i]);
+#pragma unroll 8
+  for (int i = tid; i < count; i += THREADS) newest = max(newest, position[begin + i]);
   newest = __reduce_max_sync(0xffffffffu, newest);
   if (lane == 0) scratch[warp] = newest;
   __syncthreads();
-  newest = __reduce_max_sync(0xffffffffu, scratch[lane]);
-  if (tid == 0) newest_here = newest;
-  sync();
-  for (int k = 0; k < cluster; ++k) newest = max(newest, of_cta(&newest_here, k));
+  newest = __reduce_max_sync(0xffffffffu, lane < kWarps ? scratch[lane] : INT_MIN);
+  if (cluster > 1) {  // every CTA's goes to all
+    if (tid < cluster) {
+      uint32_t at;
+      asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(&newest_of[me])), "r"(tid));
+      asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(at), "r"(newest) : "memory");
+    }
+    sync();
+    for (int k = 0; k < cluster; ++k) newest = max(newest, newest_of[k]);
+  }
   const long long safe_above = static_cast<long long>(newest) - p.recent;
-  auto rank_at = [&](int i) { return i < p.staged ? ranks[i] : rank_of(score[begin + i], position[begin + i], safe_above); };
+  const int staged = p.staged;
+  int* const holes_list = p.holes + static_cast<long long>(b) * p.most;
+  int* const late_list = p.late + static_cast<long long>(b) * p.most;
+  auto rank_at = [&](int i) { return i < staged ? ranks[i] : rank_of(score[begin + i], position[begin + i], safe_above); };
+  // Slots below the budget keep what they have for now; those given up are written again by the rows that move there.
+  const bool copy_scores = score_out != score, copy_positions = position_out != position;
 #pragma unroll 4
-  for (int i = tid; i < count; i += kSelectThreads) {
-    const uint32_t r = rank_of(score[begin + i], position[begin + i], safe_above);
-    if (i < p.staged) ranks[i] = r;
+  for (int i = tid; i < count; i += THREADS) {
+    const float s = score[begin + i];
+    const int at = position[begin + i];
+    const uint32_t r = rank_of(s, at, safe_above);
+    if (i < staged) ranks[i] = r;
     atomicAdd(&bins[0][r >> (32 - kDigitBits)], 1);
+    if (begin + i < budget) {
+      if (copy_scores) score_out[begin + i] = s;
+      if (copy_positions) position_out[begin + i] = at;
+    }
   }
   uint32_t bits = 0, mask = 0;
   int left = budget;  // of the rows that share `bits` under `mask`, how many are kept
   int bin = 0;
   for (int digit = 0; digit < kDigits; ++digit) {
-    const int shift = digit < 2 ? 32 - kDigitBits * (digit + 1) : 0, width = digit < 2 ? kBins : 1 << (32 - 2 * kDigitBits);
+    const bool last = digit == kDigits - 1;
+    const int shift = last ? 0 : 32 - kDigitBits * (digit + 1), width = last ? 1 << (32 - (kDigits - 1) * kDigitBits) : kBins;
     if (digit > 0) {
-      for (int i = tid; i < count; i += kSelectThreads) {
+      for (int i = tid; i < count; i += THREADS) {
         const uint32_t r = rank_at(i);
         if ((r & mask) == bits) atomicAdd(&bins[digit][(r >> shift) & (width - 1)], 1);
       }
@@ -1208,15 +1238,10 @@ __global__ void __launch_bounds__(kSelectThreads, 1) evict_select_kernel(const _
     sync();
     // Thread t has bins width - 1 - 2 t and the one below: counted from the top.
     const int high = width - 1 - 2 * tid;
-    int n0 = 0, n1 = 0;
-    if (high > 0) {
-      for (int k = 0; k < cluster; ++k) {
-        n0 += of_cta(&bins[digit][high], k);
-        n1 += of_cta(&bins[digit][high - 1], k);
-      }
-    }
+    const int2 pair = high > 0 ? sum_over(&bins[digit][high - 1], 0, cluster) : make_int2(0, 0);
+    const int n0 = pair.y, n1 = pair.x;
     int total;
-    const int above = threads_before(n0 + n1, scratch, &total);
+    const int above = threads_before<THREADS>(n0 + n1, scratch, &total);
     if (above < left && left <= above + n0 + n1) {
       const bool second = left > above + n0;
       found[0] = high - (second ? 1 : 0);
@@ -1229,66 +1254,64 @@ __global__ void __launch_bounds__(kSelectThreads, 1) evict_select_kernel(const _
     left -= found[1];
     __syncthreads();
   }
-  // Of the rows at the threshold the first `left` stay. A thread takes a run of words of 32 slots; ties of the CTAs before this one are
-  // in their last counts.
-  int ties_before = 0;
-  for (int k = 0; k < me; ++k) ties_before += of_cta(&bins[kDigits - 1][bin], k);
-  const int words = (count + 31) / 32, per_warp = (words + kSelectWarps - 1) / kSelectWarps;
-  const int w0 = min(words, warp * per_warp), w1 = min(words, w0 + per_warp);
-  int total, mine = 0;
-  for (int w = w0; w < w1; ++w) {
-    const int i = 32 * w + lane;
-    mine += __popc(__ballot_sync(0xffffffffu, i < count && rank_at(i) == bits));
-  }
-  int seen0 = threads_before(lane == 0 ? mine : 0, scratch, &total);  // (lane 0's is the warp's)
-  seen0 = ties_before + __shfl_sync(0xffffffffu, seen0, 0);
-  int holes_at = 0, late_at = 0;
+  // Of the rows at the threshold the first `left` stay; ties of the CTAs before this one are in their last counts. A thread takes a
+  // word of 32 slots; slots of more words than threads are gone through in blocks, and then twice.
+  const int2 ties = sum_over(&bins[kDigits - 1][bin & ~1], 0, me);
+  const int words = (count + 31) / 32, blocks = (words + THREADS - 1) / THREADS;
+  int holes_at = 0, late_at = 0, moves = 0;
   for (int pass = 0; pass < 2; ++pass) {
-    int seen = seen0, holes = 0, late = 0;
-    for (int w = w0; w < w1; ++w) {
-      const int i = 32 * w + lane, slot = begin + i;
-      const uint32_t r = i < count ? rank_at(i) : 0u;
-      const uint32_t tie = __ballot_sync(0xffffffffu, i < count && r == bits), below = (1u << lane) - 1u;
-      const bool kept = i < count && (r > bits || (r == bits && seen + __popc(tie & below) < left));
-      seen += __popc(tie);
-      const bool hole = i < count && !kept && slot < budget, moved = kept && slot >= budget;
-      const uint32_t hm = __ballot_sync(0xffffffffu, hole), lm = __ballot_sync(0xffffffffu, moved);
-      if (pass == 1) {
-        if (hole) p.holes[static_cast<long long>(b) * p.most + holes_at + holes + __popc(hm & below)] = slot;
-        if (moved) p.late[static_cast<long long>(b) * p.most + late_at + late + __popc(lm & below)] = slot;
-        if (kept && slot < budget) {
-          score_out[slot] = score[slot];
-          position_out[slot] = position[slot];
+    int seen = bin & 1 ? ties.y : ties.x, holes = 0, late = 0;
+    for (int block = 0; block < blocks; ++block) {
+      const int w0 = block * THREADS, here = min(THREADS, words - w0);
+      if (pass == 0 || blocks > 1) {
+        __syncthreads();
+        for (int w = warp; w < here; w += kWarps) {
+          const int i = 32 * (w0 + w) + lane;
+          const uint32_t r = i < count ? rank_at(i) : 0u;
+          const uint32_t above = __ballot_sync(0xffffffffu, i < count && r > bits), tie = __ballot_sync(0xffffffffu, i < count && r == bits);
+          if (lane == 0) {
+            above_words[w] = above;
+            tie_words[w] = tie;
+          }
         }
+        __syncthreads();
       }
-      holes += __popc(hm);
-      late += __popc(lm);
+      const uint32_t tie = tid < here ? tie_words[tid] : 0u;
+      int all_ties, all_holes, all_late;
+      const int tie_rank = seen + threads_before<THREADS>(__popc(tie), scratch, &all_ties);
+      // the first ties of the word that stay: those below its (left - tie_rank)-th
+      uint32_t kept = tid < here ? above_words[tid] : 0u;
+      const int stay = max(0, min(__popc(tie), left - tie_rank));
+      kept |= stay == __popc(tie) ? tie : stay == 0 ? 0u : tie & ((2u << __fns(tie, 0, stay)) - 1u);
+      const int slot = begin + 32 * (w0 + tid), in_run = count - 32 * (w0 + tid);
+      const uint32_t valid = in_run >= 32 ? 0xffffffffu : in_run > 0 ? (1u << in_run) - 1u : 0u;
+      const uint32_t low = budget - slot >= 32 ? 0xffffffffu : budget > slot ? (1u << (budget - slot)) - 1u : 0u;  // below the budget
+      uint32_t hole = ~kept & valid & low, moved = kept & ~low;
+      int h = holes_at + holes + threads_before<THREADS>(__popc(hole), scratch, &all_holes);
+      int l = late_at + late + threads_before<THREADS>(__popc(moved), scratch, &all_late);
+      if (pass == 1) {
+        for (; hole != 0; hole &= hole - 1) holes_list[h++] = slot + __ffs(hole) - 1;
+        for (; moved != 0; moved &= moved - 1) late_list[l++] = slot + __ffs(moved) - 1;
+      }
+      seen += all_ties;
+      holes += all_holes;
+      late += all_late;
     }
     if (pass == 0) {
-      int all_holes, all_late;
-      holes_at = threads_before(lane == 0 ? holes : 0, scratch, &all_holes);
-      late_at = threads_before(lane == 0 ? late : 0, scratch, &all_late);
       if (tid == 0) {
-        totals[0] = all_holes;
-        totals[1] = all_late;
+        totals[0] = holes;
+        totals[1] = late;
       }
       sync();
-      holes_at = __shfl_sync(0xffffffffu, holes_at, 0);
-      late_at = __shfl_sync(0xffffffffu, late_at, 0);
-      for (int k = 0; k < me; ++k) {
-        holes_at += of_cta(&totals[0], k);
-        late_at += of_cta(&totals[1], k);
-      }
-      if (me == cluster - 1 && tid == 0) p.moves[b] = holes_at + all_holes;
+      const int2 before = sum_over(totals, 0, me);
+      holes_at = before.x;
+      late_at = before.y;
+      if (me == cluster - 1 && tid == 0) p.moves[b] = holes_at + holes;
+      if (p.few) moves = sum_over(totals, 0, cluster).x;
     }
   }
   sync();  // the lists are complete, and no CTA leaves while another reads its counts
-  if (p.few) {
-    int moves = 0;
-    for (int k = 0; k < cluster; ++k) moves += of_cta(&totals[0], k);
-    for (int i = me * kSelectWarps + warp; i < moves; i += cluster * kSelectWarps) move_row(p, b, i, lane);
-    sync();
-  }
+  for (int i = me * kWarps + warp; i < moves; i += cluster * kWarps) move_row(p, b, i, lane);
 }
 
 // A warp per moved row: the row, its score and its position.
@@ -1640,9 +1663,11 @@ int b200_mla_cache_evict(const b200_mla_cache* cache, const float* score, long l
   p.staged = slots < kMaxStaged ? slots : kMaxStaged;
   p.few = p.most <= kFewMoves;
   const int device = current_device();
-  static std::atomic<bool> opted[kMaxDevices];
-  if (device < 0 || !opt_in(evict_select_kernel, kMaxStaged * 4, &opted[device])) return B200_FP8_MM_ERR_DRIVER;
-  rc = launch_clusters(evict_select_kernel, p.cluster, dim3(static_cast<unsigned>(cache->batch * p.cluster)), kSelectThreads,
+  static std::atomic<bool> opted[kMaxDevices][2];
+  const bool small = slots <= 4096;
+  const auto select = small ? evict_select_kernel<256> : evict_select_kernel<1024>;
+  if (device < 0 || !opt_in(select, kMaxStaged * 4, &opted[device][small ? 0 : 1])) return B200_FP8_MM_ERR_DRIVER;
+  rc = launch_clusters(select, p.cluster, dim3(static_cast<unsigned>(cache->batch * p.cluster)), small ? 256 : 1024,
                        static_cast<size_t>(p.staged) * 4, stream, p);
   if (rc != B200_FP8_MM_OK || p.most == 0 || p.few) return rc;
   const int want = (p.most + kMoveThreads / 32 - 1) / (kMoveThreads / 32);
