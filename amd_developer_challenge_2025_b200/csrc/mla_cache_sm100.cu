@@ -494,6 +494,7 @@ attend_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__
   const float scale_log2 = p.scale_log2;
   const long long out_sb = p.out_sb, out_sh = p.out_sh;
   float *const logits = p.logits, *const part_out = p.part_out;
+  T* const out_at = static_cast<T*>(p.out);
   const int group_bytes = chunks * kGroupBytes, tile_bytes = kTile / 8 * group_bytes;
   uint8_t* const q_smem = smem;  // [chunk][HT rows x 128 bytes]; the first product reads 64 rows, those behind HT are never looked at
   uint8_t* const ring = q_smem + chunks * HT * kRowBytes;
@@ -671,9 +672,10 @@ attend_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__
     // The second product that is still to be issued, of the tile before.
     bool pending = false, pending_first = false;
     int pv_stage = 0, pv_segment = 0;
+    uint32_t pv_values = 0;
     auto second = [&]() {
       tcgen05_fence_after();
-      uint32_t values = uniform(kLoV | (ring_at + pv_stage * (tile_bytes >> 4))), o = tmem;
+      uint32_t values = pv_values, o = tmem;
 #pragma unroll 1
       for (int u = 0; u < v_units; ++u, values += 2 * kGroupBytes >> 4, o += HT)
         umma_f16_x4(o, values, hi_rows, 2 * group_bytes >> 4, p_lo, kHiDense, kIdescO, pending_first ? 0u : 1u);
@@ -731,6 +733,7 @@ attend_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__
         pending = true;
         pending_first = tile == 0;
         pv_stage = stage;
+        pv_values = uniform(kLoV | (ring_at + stage * (tile_bytes >> 4)));
         pv_segment = segment;
         if (++stage == stages) stage = 0, lap ^= 1;
       }
@@ -770,8 +773,6 @@ attend_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__
         uint32_t x[32];
         if (active) tmem_ld_16x64(tmem + lanes + kTmemLogits + (i & 1) * kTile, x);
         tcgen05_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&sh.s_free[i & 1]));
         const int left = walk.rows - (walk.t + tile) * kTile;  // rows that exist from this tile on
         float t0 = -INFINITY, t1 = -INFINITY;
         bool up = false;
@@ -859,20 +860,22 @@ attend_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__
         }
         if (left < kTile) {
           // What lies behind the sequence in its last page may be anything: as values it has to be 0, because 0 weights times
-          // infinity or NaN would be NaN.
-          uint8_t* const tile_at = ring + here.stage * tile_bytes;
-          const int pieces = 2 * v_units * (kRowBytes / 16);  // of a row's value
-          for (int at = tid; at < (kTile - left) * pieces; at += kSoftmaxThreads) {
-            const int row = left + at / pieces, piece = at % pieces;
-            *reinterpret_cast<uint4*>(tile_at + (row >> 3) * group_bytes + (piece >> 3) * kGroupBytes + (row & 7) * kRowBytes + (piece & 7) * 16) =
-                make_uint4(0u, 0u, 0u, 0u);
+          // infinity or NaN would be NaN. (Pieces that begin behind the sequence have come as zeros.)
+          const int end = (left + copy_rows - 1) / copy_rows * copy_rows;
+          for (int row = left + warp; row < end; row += kSoftmaxThreads / 32) {
+            uint8_t* const at = ring + here.stage * tile_bytes + (row >> 3) * group_bytes + (row & 7) * kRowBytes;
+            for (int piece = lane; piece < 16 * v_units; piece += 32)  // 16 bytes each
+              *reinterpret_cast<uint4*>(at + (piece >> 3) * kGroupBytes + (piece & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
           }
         }
         before = here;
         if (++here.stage == stages) here.stage = 0, here.lap ^= 1;
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&sh.p_full));
+        if (lane == 0) {
+          mbar_arrive(smem_u32(&sh.p_full));
+          mbar_arrive(smem_u32(&sh.s_free[i & 1]));
+        }
       }
       // End of the segment: sums over the four threads of a head, then the accumulators, a value element per thread.
       if (active) {
@@ -902,10 +905,12 @@ attend_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__
           uint32_t o[kCols];
           tmem_ld_32(tmem + lanes + u * HT + h0, o);
           if (whole) {
-            T* out = static_cast<T*>(p.out) + walk.b * out_sb + (head0 + h0) * out_sh + u * 128 + tid;
+            T* out = out_at + walk.b * out_sb + (head0 + h0) * out_sh + u * 128 + tid;
+#pragma unroll
+            for (int n = 0; n < kCols; ++n) o[n] = __float_as_uint(__uint_as_float(o[n]) * sh.inverse[h0 + n]);
 #pragma unroll
             for (int n = 0; n < kCols; ++n, out += out_sh)
-              if (h0 + n < heads) from_float(__uint_as_float(o[n]) * sh.inverse[h0 + n], out);
+              if (h0 + n < heads) from_float(__uint_as_float(o[n]), out);
           } else {
             float* const out = part_out + ((part * v_units + u) * HT + h0) * 128 + tid;
 #pragma unroll
