@@ -1,6 +1,6 @@
 // How the tiles of a batch of cached sequences are shared out, for the kernels of mla_cache_sm100.cu and a host test.
 //
-// A sequence of n rows has ceil(n / 64) tiles, and costs `extra` tiles more to begin and end. On a line, every sequence that has
+// A sequence of n rows has ceil(n / tile) tiles, and costs `extra` tiles more to begin and end. On a line, every sequence that has
 // rows takes its extra places and then one for each tile, and worker g of `workers` takes the places [share_begin(g), share_begin(g +
 // 1)), whatever sequences these belong to: shares differ by one place at most, however ragged the batch is. A sequence whose tiles lie
 // in the shares of several workers leaves a part with each of them; a border among the extra places splits nothing.
@@ -15,12 +15,10 @@
 
 namespace cache_walk {
 
-constexpr int kTileRows = 64;
-
-CACHE_WALK_FN int tiles_of(int rows) { return (rows + kTileRows - 1) / kTileRows; }
+CACHE_WALK_FN int tiles_of(int rows, int tile) { return (rows + tile - 1) / tile; }
 
 // Places on the line of a sequence.
-CACHE_WALK_FN int places_of(int rows, int extra) { return rows > 0 ? tiles_of(rows) + extra : 0; }
+CACHE_WALK_FN int places_of(int rows, int tile, int extra) { return rows > 0 ? tiles_of(rows, tile) + extra : 0; }
 
 // Workers that get a share: as many as there are, but each with `least` places where the batch has that many.
 CACHE_WALK_FN int workers_of(long long places, int most, int least) {
@@ -50,11 +48,11 @@ CACHE_WALK_FN int tiles_in(long long begin, int tiles, int extra, long long from
 // A worker's parts of split sequences: 0 for the one its share begins with, 1 for one that begins inside its share.
 CACHE_WALK_FN int part_slot(long long share, long long begin_of_sequence) { return share >= begin_of_sequence ? 0 : 1; }
 
-// Rows that one copy can bring: the largest power of two, at most a tile's, that divides the page, so that no copy crosses a
-// page's end and every copy of a tile begins at a multiple of it.
-CACHE_WALK_FN int copy_rows(int page_size) {
+// Rows that one copy can bring: the largest power of two that divides the tile and the page, so that no copy crosses a page's end
+// and every copy of a tile begins at a multiple of it.
+CACHE_WALK_FN int copy_rows(int page_size, int tile) {
   int r = 1;
-  while (r < kTileRows && page_size % (2 * r) == 0) r *= 2;
+  while (tile % (2 * r) == 0 && page_size % (2 * r) == 0) r *= 2;
   return r;
 }
 

@@ -175,7 +175,10 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_con
 
 constexpr float kLn2 = 0.69314718055994531f, kLog2E = 1.4426950408889634f;
 constexpr int kMaxD = 576;
-constexpr int kTile = cache_walk::kTileRows;   // rows of the cache per tile
+// Rows of the cache per tile. A tile is fetched, multiplied, weighed and multiplied again, and several are under way at a time: what is
+// in flight decides the rate. 64 heads leave room for two tiles of 64 rows, fewer heads for three of 48: 128 sequences of 4096 rows with
+// 16 heads 132 -> 1xx us.
+__host__ __device__ constexpr int tile_rows_for(int tile_heads) { return tile_heads < 64 ? 48 : 64; }
 constexpr int kRowBytes = 128;                 // of a row that lie together under the 128-byte swizzle: a chunk of 64 elements
 constexpr int kGroupBytes = 8 * kRowBytes;     // 8 rows of a chunk, the swizzle's period
 constexpr int kMaxStages = 12;
@@ -197,7 +200,7 @@ struct AttendParams {
   long long out_sb, out_sh, score_stride, score_out_stride;
   int heads, head_tiles, max_len, batch;
   int workers, least;      // workers per head tile, and the least places worth one
-  int extra;               // see cache_walk.h
+  int tile, extra;         // rows per tile; see cache_walk.h
   int copy_rows;           // cache_walk::copy_rows(page_size)
   int stages;              // tiles of the ring
   int v_units, chunks;     // 128-element units of the value; 64-element chunks of a row
@@ -278,18 +281,13 @@ struct Waits {
   __device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, int where) const {
     return mbar_try_wait(bar, parity, 200000) || slow(bar, parity, where);
   }
-  // For a whole warp, which leaves together: every lane has a barrier of its own (0: none).
-  __device__ __forceinline__ bool wait_lanes(uint32_t bar, uint32_t parity, int where) const {
-    if (__all_sync(0xffffffffu, bar == 0 || mbar_try_wait(bar, parity, 200000))) return true;
-    return __all_sync(0xffffffffu, bar == 0 || slow(bar, parity, where)) != 0;
-  }
-  // The same barrier for all.
+  // For a whole warp, which leaves together.
   __device__ __forceinline__ bool wait_all(uint32_t bar, uint32_t parity, int where) const {
     return __all_sync(0xffffffffu, wait(bar, parity, where)) != 0;
   }
 };
 
-enum Where { kAtFree = 0x201, kAtQEmpty, kAtOperands, kAtWeights, kAtSFull, kAtPvDone };
+enum Where { kAtFree = 0x201, kAtQEmpty, kAtOperands, kAtSFull, kAtPvDone };
 
 // Copies for a whole warp, which comes here together: one lane issues.
 __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, int c1, int c2, int c3, uint32_t bar) {
@@ -319,17 +317,20 @@ __device__ __forceinline__ void tma_load_4d_own(uint32_t dst, const CUtensorMap*
 __device__ __forceinline__ void tcgen05_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tcgen05_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
-// Four products along K into one accumulator, a_step (of 16 bytes) of A and 32 bytes of B from one to the next. Matrix descriptors as
-// 32-bit halves, as in the GEMM: low word address and leading offset, high word stride offset, version and the 128-byte swizzle.
-// The whole warp comes here and one lane of it, always the same, issues. One statement for four, and rolled loops around it: a warp
-// that issues from unrolled code is held up by its instruction fetch (56 clocks a product against 30).
-__device__ __forceinline__ void umma_f16_x4(uint32_t d, uint32_t a_lo, uint32_t a_hi, uint32_t a_step, uint32_t b_lo, uint32_t b_hi,
-                                            uint32_t idesc, uint32_t accumulate) {
+// Three or four products along K into one accumulator, a_step (of 16 bytes) of A and 32 bytes of B from one to the next. Matrix
+// descriptors as 32-bit halves, as in the GEMM: low word address and leading offset, high word stride offset, version and the 128-byte
+// swizzle. The whole warp comes here and one lane of it, always the same, issues. One statement for all, and rolled loops around it: a
+// warp that issues from unrolled code is held up by its instruction fetch (56 clocks a product against 30).
+template <int N>
+__device__ __forceinline__ void umma_f16(uint32_t d, uint32_t a_lo, uint32_t a_hi, uint32_t a_step, uint32_t b_lo, uint32_t b_hi,
+                                         uint32_t idesc, uint32_t accumulate) {
+  static_assert(N == 3 || N == 4, "products of a statement");
   asm volatile(
-      "{\n\t.reg .pred p, leader, yes;\n\t.reg .b64 da, db;\n\t.reg .b32 la, lb;\n\t"
+      "{\n\t.reg .pred p, leader, yes, last;\n\t.reg .b64 da, db;\n\t.reg .b32 la, lb;\n\t"
       "elect.sync _|leader, 0xffffffff;\n\t"
       "setp.ne.b32 p, %6, 0;\n\t"
       "setp.eq.b32 yes, 0, 0;\n\t"
+      "setp.eq.and.b32 last, %8, 4, leader;\n\t"
       "mov.b64 da, {%1, %2};\n\t"
       "mov.b64 db, {%3, %4};\n\t"
       "@leader tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %5, p;\n\t"
@@ -338,11 +339,10 @@ __device__ __forceinline__ void umma_f16_x4(uint32_t d, uint32_t a_lo, uint32_t 
       "add.u32 la, la, %7;\n\tadd.u32 lb, %3, 4;\n\tmov.b64 da, {la, %2};\n\tmov.b64 db, {lb, %4};\n\t"
       "@leader tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %5, yes;\n\t"
       "add.u32 la, la, %7;\n\tadd.u32 lb, %3, 6;\n\tmov.b64 da, {la, %2};\n\tmov.b64 db, {lb, %4};\n\t"
-      "@leader tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %5, yes;\n\t}" ::"r"(d),
-      "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate), "r"(a_step)
+      "@last tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %5, yes;\n\t}" ::"r"(d),
+      "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate), "r"(a_step), "n"(N)
       : "memory");
 }
-static_assert(kTile == 64, "four products along a tile's rows");
 
 __device__ __forceinline__ void umma_commit(uint32_t bar) {
   asm volatile(
@@ -456,24 +456,24 @@ struct Walk {
     while (begin < to) {
       ++b;
       rows = rows_of(p.cache, b, p.max_len);
-      count = cache_walk::tiles_in(begin, cache_walk::tiles_of(rows), p.extra, from, to, &t);
-      begin += cache_walk::places_of(rows, p.extra);
+      count = cache_walk::tiles_in(begin, cache_walk::tiles_of(rows, p.tile), p.extra, from, to, &t);
+      begin += cache_walk::places_of(rows, p.tile, p.extra);
       if (rows > 0 && count > 0) return true;
     }
     return false;
   }
-  __device__ __forceinline__ bool whole() const { return count == cache_walk::tiles_of(rows); }
+  __device__ __forceinline__ bool whole(int tile) const { return count == cache_walk::tiles_of(rows, tile); }
 };
 
 // Flash attention of one token per sequence over a latent cache: heads x rows x (d + dv) products per row of d elements read.
 //
-//   S = Q K^T        [64 heads x 64 rows]   M = heads (64), K = d:     Q and the rows as they lie (K-major)
+//   S = Q K^T        [64 heads x rows]      M = heads (64), K = d:     Q and the rows as they lie (K-major)
 //   O^T += V^T P^T   [128 x heads] x dv/128 M = value elements, K = rows: the same rows read as an MN-major operand, so that
 //                                            a tile is fetched once for both products and never transposed
 // With the value's elements in the lanes, the accumulators of 64 heads take 256 of the 512 TMEM columns; with the heads in the
 // lanes, 128 heads would take them all and leave none for S. Fewer heads shrink N (16 or 32) and what Q takes of shared memory.
 //
-// A tile lies in shared memory as [8 groups of rows][chunk of 64 elements][8 rows x 128 bytes]: one stride from group to group and one
+// A tile lies in shared memory as [groups of 8 rows][chunk of 64 elements][8 rows x 128 bytes]: one stride from group to group and one
 // from chunk to chunk for both operands, and one copy brings all chunks of as many rows as lie together in a page, up to half a tile.
 // What bounds the loop is how long a tile stays, from its copy's way through memory over both products and the softmax between them,
 // and what fits next to Q; so the second product goes by halves of the rows and frees each for its next copy. (Tiles of 32 rows, more
@@ -487,6 +487,7 @@ struct Walk {
 template <typename T, int HT>
 __global__ void __launch_bounds__(kAttendThreads, 1)
 attend_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap row_map, const __grid_constant__ AttendParams p) {
+  constexpr int kTile = tile_rows_for(HT);
   extern __shared__ __align__(1024) uint8_t smem[];
   // The loops below are full of statements that touch memory, behind each of which a parameter would be read anew.
   const CacheView c = p.cache;
@@ -533,7 +534,7 @@ attend_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__
   const int run = (p.batch + kAttendThreads - 1) / kAttendThreads;
   const int b0 = min(p.batch, tid * run), b1 = min(p.batch, b0 + run);
   long long mine = 0;
-  for (int b = b0; b < b1; ++b) mine += cache_walk::places_of(rows_of(c, b, p.max_len), p.extra);
+  for (int b = b0; b < b1; ++b) mine += cache_walk::places_of(rows_of(c, b, p.max_len), kTile, p.extra);
   long long upto = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -563,8 +564,8 @@ attend_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__
     if (begin < end && before <= begin && begin < before + mine) {
       long long at = before;
       int b = b0;
-      for (;; ++b) {
-        const int n = cache_walk::places_of(rows_of(c, b, p.max_len), p.extra);
+      for (; b + 1 < b1; ++b) {  // (the last of the thread's sequences if none before it)
+        const int n = cache_walk::places_of(rows_of(c, b, p.max_len), kTile, p.extra);
         if (begin < at + n) break;
         at += n;
       }
@@ -574,7 +575,7 @@ attend_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__
     if (blockIdx.x == 0) {
       for (int b = b0; b < b1; ++b) {
         p.begins[b] = before;
-        before += cache_walk::places_of(rows_of(c, b, p.max_len), p.extra);
+        if (b + 1 < b1) before += cache_walk::places_of(rows_of(c, b, p.max_len), kTile, p.extra);
       }
       if (tid == 0) p.begins[p.batch] = places;
     }
@@ -671,75 +672,96 @@ attend_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__
     uint32_t lap = 0;
     // The second product that is still to be issued, of the tile before.
     bool pending = false, pending_first = false;
-    int pv_stage = 0, pv_segment = 0;
+    int pv_stage = 0, pv_segment = 0, pv_tile = 0;
     uint32_t pv_values = 0;
     auto second = [&]() {
       tcgen05_fence_after();
-      uint32_t values = pv_values, o = tmem;
+      uint32_t values = uniform(pv_values), o = tmem;
 #pragma unroll 1
       for (int u = 0; u < v_units; ++u, values += 2 * kGroupBytes >> 4, o += HT)
-        umma_f16_x4(o, values, hi_rows, 2 * group_bytes >> 4, p_lo, kHiDense, kIdescO, pending_first ? 0u : 1u);
+        umma_f16<kTile / 16>(o, values, hi_rows, 2 * group_bytes >> 4, p_lo, kHiDense, kIdescO, pending_first ? 0u : 1u);
       umma_commit(smem_u32(&sh.pv_done[pv_stage]));
       pending = false;
     };
-    // Waits for what the next products need, a barrier per lane: the first product of this tile for its rows (lane 0), a buffer of S (1)
-    // and the queries (2), the second product of the tile before for the weights (3) and, where it begins a segment, for the
-    // accumulators of the one before to have been read (4). Issues the second one if it can go and the first cannot; returns when
-    // the first can.
-    auto ready = [&](int tile) {
-      const bool fresh = pending_first && pv_segment > 0;
-      uint32_t bar = lane == 0 ? smem_u32(&sh.full[stage])
-                     : lane == 1 ? smem_u32(&sh.s_free[i & 1])
-                     : lane == 2 && tile == 0 ? smem_u32(&sh.q_full) : 0u;
-      uint32_t parity = lane == 0 ? lap : lane == 1 ? ((i >> 1) & 1) ^ 1 : segment & 1;
-      if (pending && lane >= 3) {
-        bar = lane == 3 ? smem_u32(&sh.p_full) : lane == 4 && fresh ? smem_u32(&sh.o_free) : 0u;
-        parity = static_cast<uint32_t>(lane == 3 ? i - 1 : pv_segment - 1) & 1u;
-      }
+    // What the products wait for is looked at all at once, a barrier per lane: the first product of tile i for its rows (lane 0), a buffer
+    // of S (1) and, where a segment begins, the queries (2); the pending second one for the weights (3) and, where its segment begins,
+    // for the accumulators of the one before to have been read (4). Without branches, which took as long as twenty products.
+    constexpr uint32_t kFirst = 7u, kSecond = 0x18u;
+    const uint32_t bar_base = smem_u32(lane == 1 ? &sh.s_free[0] : lane == 2 ? &sh.q_full : lane == 3 ? &sh.p_full : lane == 4 ? &sh.o_free : &sh.full[0]);
+    const uint32_t stage_step = lane == 0 ? 8u : 0u, buffer_step = lane == 1 ? 8u : 0u;
+    uint32_t bar = bar_base, parity = 0, idle = 0;
+    auto look_at = [&](uint32_t wanted, bool begins) {
+      const uint32_t parities = lap | ((static_cast<uint32_t>(i) >> 1 & 1u) ^ 1u) << 1 | (static_cast<uint32_t>(segment) & 1u) << 2 |
+                                (static_cast<uint32_t>(pv_tile) & 1u) << 3 | (static_cast<uint32_t>(pv_segment - 1) & 1u) << 4;
+      const uint32_t needed = wanted & (begins ? 0x1bu | 4u : 0x1bu) & (pending_first && pv_segment > 0 ? 0x1fu : 0xfu) & (pending ? 0x1fu : 7u);
+      bar = bar_base + static_cast<uint32_t>(stage) * stage_step + (static_cast<uint32_t>(i) & 1u) * buffer_step;
+      parity = parities >> lane & 1u;
+      idle = ~needed >> lane & 1u;
+    };
+    // Looks until all of `wanted` is there, and returns all that is; 0 when a wait has expired. While the first product cannot go, the
+    // second one does as soon as it can: it frees the ring.
+    auto until = [&](uint32_t wanted) {
       unsigned long long t0 = 0;  // (read late: reading the timer takes several hundred clocks)
       for (uint32_t spins = 1;; ++spins) {
-        const uint32_t there = __ballot_sync(kAll, bar == 0 || mbar_test(bar, parity));
-        if ((there & 7u) == 7u) return true;
-        if (pending && (there & 0x18u) == 0x18u) second();
+        const uint32_t there = __ballot_sync(kAll, (mbar_test(bar, parity) | idle) != 0);
+        if ((there & wanted) == wanted) return there;
+        if (wanted == kFirst && pending && (there & kSecond) == kSecond) second();
         if ((spins & 255u) == 0) {
           if (t0 == 0) t0 = global_ns();
-          if (__any_sync(kAll, waits.give_up(t0, parity, kAtOperands))) return false;
+          if (__any_sync(kAll, waits.give_up(t0, parity, kAtOperands))) return 0u;
         }
       }
-    };
-    auto weights = [&]() {
-      const uint32_t bar = lane == 0 ? smem_u32(&sh.p_full) : lane == 1 && pending_first && pv_segment > 0 ? smem_u32(&sh.o_free) : 0u;
-      return waits.wait_lanes(bar, static_cast<uint32_t>(lane == 0 ? i - 1 : pv_segment - 1) & 1u, kAtWeights);
     };
     bool ok = __all_sync(kAll, sh.expired == 0);
     Walk walk(sh);
     while (ok && __all_sync(kAll, walk.next(p))) {
       const int count = __shfl_sync(kAll, walk.count, 0);
+      bool known = false;  // all that the tile's first product needs has been seen
       for (int tile = 0; tile < count; ++tile) {
-        if (!(ok = ready(tile))) break;
+        if (!known) {
+          look_at(kFirst | kSecond, tile == 0);
+          if (until(kFirst) == 0) {
+            ok = false;
+            break;
+          }
+        }
         tcgen05_fence_after();
-        const uint32_t s = uniform(tmem + kTmemLogits + (i & 1) * kTile);
+        const uint32_t values = kLoV | (ring_at + stage * (tile_bytes >> 4));
+        const int here = stage;
         uint32_t rows = uniform(kLoK | (ring_at + stage * (tile_bytes >> 4))), q_at = q_lo;
+        const uint32_t s = tmem + kTmemLogits + (i & 1) * 64;
 #pragma unroll 1
         for (int n = 0; n < chunks; ++n, q_at += HT * kRowBytes >> 4, rows += kGroupBytes >> 4)
-          umma_f16_x4(s, q_at, kHiDense, 2, rows, hi_rows, kIdescS, n > 0);
+          umma_f16<4>(s, q_at, kHiDense, 2, rows, hi_rows, kIdescS, n > 0);
         umma_commit(smem_u32(&sh.s_full[i & 1]));
         if (tile == count - 1) umma_commit(smem_u32(&sh.q_empty));
+        if (++stage == stages) stage = 0, lap ^= 1;
+        known = false;
+        ++i;
         if (pending) {
-          if (!(ok = weights())) break;
+          // (of the tile before; what the next tile's first product needs is looked at along with it)
+          look_at(kFirst | kSecond, false);
+          const uint32_t there = until(kSecond);
+          if (there == 0) {
+            ok = false;
+            break;
+          }
+          known = tile + 1 < count && (there & kFirst) == kFirst;
           second();
         }
-        ++i;
         pending = true;
         pending_first = tile == 0;
-        pv_stage = stage;
-        pv_values = uniform(kLoV | (ring_at + stage * (tile_bytes >> 4)));
+        pv_tile = i - 1;
+        pv_stage = here;
+        pv_values = values;
         pv_segment = segment;
-        if (++stage == stages) stage = 0, lap ^= 1;
       }
       ++segment;
     }
-    if (ok && pending && weights()) second();
+    if (ok && pending) {
+      look_at(kSecond, false);
+      if (until(kSecond) != 0) second();
+    }
     if (__any_sync(kAll, sh.expired != 0)) {  // none in flight past here
       umma_commit(smem_u32(&sh.drained));
       for (int n = 0; n < 1000 && !mbar_try_wait(smem_u32(&sh.drained), 0, 10000); ++n) {
@@ -761,7 +783,7 @@ attend_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__
     // A wait that has expired does not end this role, because the other warps meet it at the barriers below: the rest of the walk
     // goes by without waiting, over whatever is there.
     auto wait = [&](uint64_t* bar, uint32_t parity, int where) {
-      if (ok) ok = waits.wait(smem_u32(bar), parity, where);
+      if (ok && !mbar_test(smem_u32(bar), parity)) ok = waits.wait(smem_u32(bar), parity, where);
     };
     Walk walk(sh);
     bool first_segment = true;
@@ -771,7 +793,7 @@ attend_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__
         wait(&sh.s_full[i & 1], (i >> 1) & 1, kAtSFull);
         tcgen05_fence_after();
         uint32_t x[32];
-        if (active) tmem_ld_16x64(tmem + lanes + kTmemLogits + (i & 1) * kTile, x);
+        if (active) tmem_ld_16x64(tmem + lanes + kTmemLogits + (i & 1) * 64, x);
         tcgen05_fence_before();
         const int left = walk.rows - (walk.t + tile) * kTile;  // rows that exist from this tile on
         float t0 = -INFINITY, t1 = -INFINITY;
@@ -779,22 +801,22 @@ attend_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__
         if (active) {
           if (left >= kTile) {
 #pragma unroll
-            for (int n = 0; n < 32; ++n) x[n] = __float_as_uint(__uint_as_float(x[n]) * scale_log2);
+            for (int n = 0; n < kTile / 2; ++n) x[n] = __float_as_uint(__uint_as_float(x[n]) * scale_log2);
           } else {
 #pragma unroll
-            for (int n = 0; n < 32; ++n) {
+            for (int n = 0; n < kTile / 2; ++n) {
               const int col = 8 * (n / 4) + 2 * (lane % 4) + (n & 1);
               x[n] = __float_as_uint(col < left ? __uint_as_float(x[n]) * scale_log2 : -INFINITY);
             }
           }
 #pragma unroll
-          for (int n = 0; n < 32; ++n) {
+          for (int n = 0; n < kTile / 2; ++n) {
             if (n & 2) t1 = fmaxf(t1, __uint_as_float(x[n])); else t0 = fmaxf(t0, __uint_as_float(x[n]));
           }
           if (logits != nullptr) {
             float* to = logits + ((static_cast<long long>(walk.b) * p.logit_tiles + walk.t + tile) * heads_all + head0) * kTile + 2 * (lane % 4);
 #pragma unroll
-            for (int n = 0; n < 8; ++n) {
+            for (int n = 0; n < kTile / 8; ++n) {
               if (row0 < HT && head0 + row0 < heads_all)
                 *reinterpret_cast<uint2*>(to + row0 * kTile + 8 * n) = make_uint2(x[4 * n], x[4 * n + 1]);
               if (row1 < HT && head0 + row1 < heads_all)
@@ -824,7 +846,7 @@ attend_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__
           }
           const float z0 = m0 == -INFINITY ? 0.f : m0, z1 = m1 == -INFINITY ? 0.f : m1;
 #pragma unroll
-          for (int n = 0; n < 8; ++n) {
+          for (int n = 0; n < kTile / 8; ++n) {
             const float a = exp2_fast(__uint_as_float(x[4 * n]) - z0), b = exp2_fast(__uint_as_float(x[4 * n + 1]) - z0);
             const float e = exp2_fast(__uint_as_float(x[4 * n + 2]) - z1), f = exp2_fast(__uint_as_float(x[4 * n + 3]) - z1);
             l0 += a + b;
@@ -852,7 +874,7 @@ attend_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__
           // 16-byte piece n of row r lies at piece n ^ (r % 8) of its 128 bytes (the swizzle of K-major operands)
           uint8_t* to = p_smem + 4 * (lane % 4);
 #pragma unroll
-          for (int n = 0; n < 8; ++n) {
+          for (int n = 0; n < kTile / 8; ++n) {
             const int piece = 16 * (n ^ (lane / 4));
             *reinterpret_cast<uint32_t*>(to + row0 * kRowBytes + piece) = x[2 * n];
             *reinterpret_cast<uint32_t*>(to + row1 * kRowBytes + piece) = x[2 * n + 1];
@@ -895,7 +917,7 @@ attend_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__
       wait(&sh.pv_done[before.stage], before.lap, kAtPvDone);
       tcgen05_fence_after();
       const int heads = min(HT, heads_all - head0);
-      const bool whole = walk.whole();
+      const bool whole = walk.whole(kTile);
       const long long part = (static_cast<long long>(worker) * p.head_tiles + head_tile) * 2 + (first_segment ? 0 : 1);
       // kCols heads of 128 value elements at a time: a warp writes 32 elements of a head at once
       constexpr int kCols = HT < 32 ? HT : 32;
@@ -973,6 +995,14 @@ __global__ void __launch_bounds__(128 * GROUPS) attend_join_kernel(const __grid_
   const int slot0 = cache_walk::part_slot(cache_walk::share_begin(places, workers, g0), begin);
   auto part_of = [&](int i) { return (static_cast<long long>(g0 + i) * p.head_tiles + head_tile) * 2 + (i == 0 ? slot0 : 0); };
   auto stat_of = [&](int i) { return p.part_stat[part_of(i) * tile_heads + in_tile]; };
+  auto value_of = [&](int i) {
+    return *reinterpret_cast<const float4*>(p.part_out + ((part_of(i) * (dv / 128) + e / 32) * tile_heads + in_tile) * 128 + 4 * (e % 32));
+  };
+  constexpr int kAhead = 4;  // parts whose values are on their way along with the statistics
+  float4 ahead[kAhead];
+#pragma unroll
+  for (int k = 0; k < kAhead; ++k)
+    if (group + k * GROUPS < parts && 4 * e < dv) ahead[k] = value_of(group + k * GROUPS);
   float top = -INFINITY;
   for (int i = lane; i < parts; i += 32) top = fmaxf(top, stat_of(i).x);
 #pragma unroll
@@ -986,16 +1016,19 @@ __global__ void __launch_bounds__(128 * GROUPS) attend_join_kernel(const __grid_
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
   float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+  auto add = [&](int i, const float4& v) {
+    const float w = exp2_fast(stat_of(i).x - base);
+    sum.x += w * v.x;
+    sum.y += w * v.y;
+    sum.z += w * v.z;
+    sum.w += w * v.w;
+  };
   if (4 * e < dv) {
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k)
+      if (group + k * GROUPS < parts) add(group + k * GROUPS, ahead[k]);
 #pragma unroll 4
-    for (int i = group; i < parts; i += GROUPS) {
-      const float w = exp2_fast(stat_of(i).x - base);
-      const float4 v = *reinterpret_cast<const float4*>(p.part_out + ((part_of(i) * (dv / 128) + e / 32) * tile_heads + in_tile) * 128 + 4 * (e % 32));
-      sum.x += w * v.x;
-      sum.y += w * v.y;
-      sum.z += w * v.z;
-      sum.w += w * v.w;
-    }
+    for (int i = group + kAhead * GROUPS; i < parts; i += GROUPS) add(i, value_of(i));
   }
   if constexpr (GROUPS > 1) {
     sums[group][e] = sum;
@@ -1026,9 +1059,9 @@ __global__ void __launch_bounds__(128 * GROUPS) attend_join_kernel(const __grid_
 
 // score_out = score + the weights of all heads, from the logits that the attention left: a CTA per tile, a group of threads for every fourth head.
 constexpr int kScoreGroups = 4;
-constexpr int kScoreThreads = kScoreGroups * kTile;
 
-__global__ void __launch_bounds__(kScoreThreads) attend_score_kernel(const __grid_constant__ AttendParams p) {
+template <int kTile>
+__global__ void __launch_bounds__(kScoreGroups * kTile) attend_score_kernel(const __grid_constant__ AttendParams p) {
   __shared__ float sums[kScoreGroups][kTile];
   pdl_wait();
   pdl_launch_dependents();
@@ -1431,7 +1464,8 @@ struct AttendWorkspace {
 };
 
 AttendWorkspace attend_workspace(int batch, int heads, int dv, int max_len, bool with_score, int sms) {
-  const size_t ht = tile_heads_for(heads), head_tiles = (heads + ht - 1) / ht;
+  const int ht = tile_heads_for(heads);
+  const size_t head_tiles = (heads + ht - 1) / ht;
   const size_t parts = 2 * head_tiles * attend_workers(heads, sms) * ht;
   auto up = [](size_t n) { return (n + 255) / 256 * 256; };
   AttendWorkspace w;
@@ -1439,13 +1473,13 @@ AttendWorkspace attend_workspace(int batch, int heads, int dv, int max_len, bool
   w.part_stat = w.lse2 + up(static_cast<size_t>(batch) * heads * sizeof(float));
   w.part_out = w.part_stat + up(parts * sizeof(float2));
   w.logits = w.part_out + up(parts * dv * sizeof(float));
-  w.bytes = w.logits + (with_score ? up(static_cast<size_t>(batch) * cache_walk::tiles_of(max_len) * heads * kTile * sizeof(float)) : 0);
+  w.bytes = w.logits + (with_score ? up(static_cast<size_t>(batch) * cache_walk::tiles_of(max_len, tile_rows_for(ht)) * heads * tile_rows_for(ht) * sizeof(float)) : 0);
   return w;
 }
 
 // Tiles in the ring: as many as fit, two of the largest next to 64 heads. Returns the shared memory of the CTA.
 size_t plan_ring(int ht, AttendParams* p) {
-  const int fixed = kHeaderBytes + (p->chunks + 1) * ht * kRowBytes, tile = p->chunks * kTile * kRowBytes;
+  const int fixed = kHeaderBytes + (p->chunks + 1) * ht * kRowBytes, tile = p->chunks * tile_rows_for(ht) * kRowBytes;
   const int fit = (kMaxSmem - fixed) / tile;
   p->stages = fit < kMaxStages ? fit : kMaxStages;
   return static_cast<size_t>(fixed) + p->stages * tile;
@@ -1586,8 +1620,9 @@ int b200_mla_cache_attend(const b200_mla_cache* cache, const void* q, long long 
   p.batch = cache->batch;
   p.workers = attend_workers(heads, sms);
   p.least = kLeastPlaces + extra_for(ht);
+  p.tile = tile_rows_for(ht);
   p.extra = extra_for(ht);
-  p.copy_rows = cache_walk::copy_rows(cache->page_size);
+  p.copy_rows = cache_walk::copy_rows(cache->page_size, p.tile);
   p.v_units = cache->dv / 128;
   p.chunks = p.cache.d / 64;
   p.scale_log2 = scale * kLog2E;
@@ -1596,7 +1631,7 @@ int b200_mla_cache_attend(const b200_mla_cache* cache, const void* q, long long 
   p.part_stat = reinterpret_cast<float2*>(ws + w.part_stat);
   p.part_out = reinterpret_cast<float*>(ws + w.part_out);
   p.logits = score_out != nullptr ? reinterpret_cast<float*>(ws + w.logits) : nullptr;
-  p.logit_tiles = cache_walk::tiles_of(max_len);
+  p.logit_tiles = cache_walk::tiles_of(max_len, p.tile);
   p.status = device_status;
   const size_t smem = plan_ring(ht, &p);
   const bool bf16 = cache->dtype == B200_MLA_CACHE_BF16;
@@ -1624,7 +1659,8 @@ int b200_mla_cache_attend(const b200_mla_cache* cache, const void* q, long long 
   else
     rc = launch_pdl(bf16 ? attend_join_kernel<__nv_bfloat16, 1> : attend_join_kernel<__half, 1>, joins, 128, 0, stream, p, ht);
   if (rc != B200_FP8_MM_OK || score_out == nullptr) return rc;
-  return launch_pdl(attend_score_kernel, dim3(static_cast<unsigned>(p.logit_tiles), static_cast<unsigned>(cache->batch)), kScoreThreads, 0, stream, p);
+  const dim3 tiles(static_cast<unsigned>(p.logit_tiles), static_cast<unsigned>(cache->batch));
+  return launch_pdl(p.tile == 64 ? attend_score_kernel<64> : attend_score_kernel<48>, tiles, kScoreGroups * p.tile, 0, stream, p);
 }
 
 size_t b200_mla_cache_evict_workspace_bytes(int batch, int capacity, int budget) {

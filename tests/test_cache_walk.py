@@ -14,16 +14,16 @@ PROGRAM = """
 #include <vector>
 #include "cache_walk.h"
 using namespace cache_walk;
-// walk <most> <least> <extra> <rows of sequence 0> <rows of sequence 1> ...: per worker "worker places", per segment "s sequence worker
+// walk <most> <least> <tile> <extra> <rows of sequence 0> <rows of sequence 1> ...: per worker "worker places", per segment "s sequence worker
 // first count", per part of a split sequence "w sequence worker slot first count" as the attention writes it, "j sequence worker slot" as
 // the join looks it up
 int main(int argc, char** argv) {
-  const int most = atoi(argv[1]), least = atoi(argv[2]), extra = atoi(argv[3]), batch = argc - 4;
+  const int most = atoi(argv[1]), least = atoi(argv[2]), tile = atoi(argv[3]), extra = atoi(argv[4]), batch = argc - 5;
   std::vector<int> rows;
   std::vector<long long> begins{0};
   for (int b = 0; b < batch; ++b) {
-    rows.push_back(atoi(argv[4 + b]));
-    begins.push_back(begins.back() + places_of(rows[b], extra));
+    rows.push_back(atoi(argv[5 + b]));
+    begins.push_back(begins.back() + places_of(rows[b], tile, extra));
   }
   const long long places = begins.back();
   const int workers = workers_of(places, most, least);
@@ -33,10 +33,10 @@ int main(int argc, char** argv) {
     bool first_segment = true;
     for (int b = 0; b < batch; ++b) {
       int first;
-      const int count = rows[b] > 0 ? tiles_in(begins[b], tiles_of(rows[b]), extra, from, to, &first) : 0;
+      const int count = rows[b] > 0 ? tiles_in(begins[b], tiles_of(rows[b], tile), extra, from, to, &first) : 0;
       if (count == 0) continue;
       printf("s %d %d %d %d\\n", b, g, first, count);
-      if (count != tiles_of(rows[b])) printf("w %d %d %d %d %d\\n", b, g, first_segment ? 0 : 1, first, count);
+      if (count != tiles_of(rows[b], tile)) printf("w %d %d %d %d %d\\n", b, g, first_segment ? 0 : 1, first, count);
       first_segment = false;
     }
   }
@@ -45,7 +45,7 @@ int main(int argc, char** argv) {
     const int g0 = worker_of(places, workers, begins[b] + extra), g1 = worker_of(places, workers, begins[b + 1] - 1);
     for (int g = g0; g1 > g0 && g <= g1; ++g) printf("j %d %d %d\\n", b, g, g == g0 ? part_slot(share_begin(places, workers, g), begins[b]) : 0);
   }
-  for (int p = 1; p <= 300; ++p) printf("r %d %d\\n", p, copy_rows(p));
+  for (int p = 1; p <= 300; ++p) printf("r %d %d\\n", p, copy_rows(p, tile));
   // far beyond 32 bits
   for (int g = 0; g < 148; ++g) {
     const long long many = (1ll << 24) * 65535;
@@ -66,15 +66,15 @@ def walk(tmp_path_factory):
     return lambda *args: [line.split() for line in subprocess.check_output([str(d / "walk"), *map(str, args)], text=True).splitlines()]
 
 
-@pytest.mark.parametrize("extra", [0, 1, 2, 5])
+@pytest.mark.parametrize("tile,extra", [(64, 0), (64, 2), (48, 1), (48, 0), (64, 5)])
 @pytest.mark.parametrize("most,least", [(1, 1), (2, 1), (74, 1), (148, 1), (148, 3), (512, 2)])
-def test_shares_and_parts(walk, most, least, extra):
+def test_shares_and_parts(walk, most, least, tile, extra):
     rng = random.Random(most + least + extra)
     for rows in ([1], [64], [65], [0, 0], [0, 5, 0], [9000], [1] * 200, [rng.randint(0, 900) for _ in range(60)],
                  [rng.choice([0, 1, 64, 65, 20000]) for _ in range(30)]):
-        lines = walk(most, least, extra, *rows)
+        lines = walk(most, least, tile, extra, *rows)
         sizes = [int(f[1]) for f in lines if f[0].isdigit()]
-        tiles = [-(-n // 64) for n in rows]
+        tiles = [-(-n // tile) for n in rows]
         places = sum(n + extra for n in tiles if n)
         assert 1 <= len(sizes) <= most and sum(sizes) == places
         assert max(sizes) - min(sizes) <= 1
@@ -91,9 +91,10 @@ def test_shares_and_parts(walk, most, least, extra):
         assert len({w[1:3] for w in written}) == len(written)  # no two parts in one place
 
 
-def test_copies_stay_inside_their_page_and_tile(walk):
-    lines = walk(1, 1, 0, 1)
+@pytest.mark.parametrize("tile", [48, 64])
+def test_copies_stay_inside_their_page_and_tile(walk, tile):
+    lines = walk(1, 1, tile, 0, 1)
     assert ["far"] not in lines
     for _, page, rows in (f for f in lines if f[0] == "r"):
         page, rows = int(page), int(rows)
-        assert page % rows == 0 and 64 % rows == 0 and (rows == 64 or page % (2 * rows) != 0)
+        assert page % rows == 0 and tile % rows == 0 and (tile % (2 * rows) != 0 or page % (2 * rows) != 0)
