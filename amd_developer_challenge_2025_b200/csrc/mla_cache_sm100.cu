@@ -183,7 +183,8 @@ constexpr int kRowBytes = 128;                 // of a row that lie together und
 constexpr int kGroupBytes = 8 * kRowBytes;     // 8 rows of a chunk, the swizzle's period
 constexpr int kMaxStages = 12;
 constexpr int kSoftmaxThreads = 128;
-constexpr int kAttendThreads = kSoftmaxThreads + 64;
+constexpr int kAttendThreads = kSoftmaxThreads + 128;
+constexpr int kRowWarps = 3;                   // that copy where pages are not whole groups of 8 rows
 constexpr int kHeaderBytes = 2048;             // barriers and small arrays, behind the rings
 constexpr int kMaxSmem = 232448;               // 227 KiB opt-in limit per CTA on sm_100
 constexpr int kTmemCols = 512;
@@ -201,7 +202,7 @@ struct AttendParams {
   int heads, head_tiles, max_len, batch;
   int workers, least;      // workers per head tile, and the least places worth one
   int tile, extra;         // rows per tile; see cache_walk.h
-  int copy_rows;           // cache_walk::copy_rows(page_size)
+  int copy_rows;           // rows of a TMA copy, 0: copies row by row
   int stages;              // tiles of the ring
   int v_units, chunks;     // 128-element units of the value; 64-element chunks of a row
   float scale_log2;        // scale * log2(e)
@@ -306,14 +307,6 @@ __device__ __forceinline__ void tma_load_5d(uint32_t dst, const CUtensorMap* map
       "l"(map), "r"(0), "r"(c1), "r"(c2), "r"(c3), "r"(c4), "r"(bar)
       : "memory");
 }
-// For one thread.
-__device__ __forceinline__ void tma_load_4d_own(uint32_t dst, const CUtensorMap* map, int c1, int c2, int c3, uint32_t bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
-      "l"(map), "r"(0), "r"(c1), "r"(c2), "r"(c3), "r"(bar)
-      : "memory");
-}
-
 __device__ __forceinline__ void tcgen05_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tcgen05_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
@@ -479,7 +472,8 @@ struct Walk {
 // and what fits next to Q; so the second product goes by halves of the rows and frees each for its next copy. (Tiles of 32 rows, more
 // of them in flight, are slower: an MMA takes 27 clocks to issue however small it is.)
 //
-// One CTA per SM and worker: warp 4 copies, warp 5 issues the products, warps 0 to 3 do the softmax (S comes as 16 x 256-bit
+// One CTA per SM and worker: warp 4 copies (with warps 6 and 7 where pages are not whole groups of 8 rows, which TMA would have to
+// bring in copies of 128 to 512 bytes: 16 bytes a thread then), warp 5 issues the products, warps 0 to 3 do the softmax (S comes as 16 x 256-bit
 // fragments, 4 threads to a head) and the epilogue. S is double buffered; the next tile's first product runs under this tile's
 // softmax. The running maximum is replaced only when a logit exceeds it by 2^8: the weights stay below 2^8, which no type here
 // minds, and rescaling the accumulators is rare. Sums are kept in fp32, weights are rounded to the cache's type for the second
@@ -507,7 +501,7 @@ attend_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__
   const Waits waits{&sh.expired, p.status};
   if (tid == 0) {
     for (int i = 0; i < kMaxStages; ++i) {
-      mbar_init(smem_u32(&sh.full[i]), 1);
+      mbar_init(smem_u32(&sh.full[i]), p.copy_rows > 0 ? 1 : kRowWarps);
       mbar_init(smem_u32(&sh.pv_done[i]), 1);
     }
     mbar_init(smem_u32(&sh.q_full), 1);
@@ -582,8 +576,32 @@ attend_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__
   }
   __syncthreads();
 
-  if (warp == 4) {
-    // Copies. Lane l knows where pieces l and l + 32 (copy_rows rows each) of a tile come from.
+  // The queries of a segment, once the first products of the segment before are over.
+  auto copy_queries = [&](int segment, int b) {
+    if (segment > 0 && !waits.wait_all(smem_u32(&sh.q_empty), (segment - 1) & 1, kAtQEmpty)) return false;
+    if (lane == 0) mbar_expect_tx(smem_u32(&sh.q_full), chunks * HT * kRowBytes);
+    __syncwarp();
+    tma_load_4d(smem_u32(q_smem), &q_map, head0, 0, b, smem_u32(&sh.q_full));
+    return true;
+  };
+  // At the end of a copying role: where a wait has expired, no copy may still be in flight when the CTA ends. A phase that will not
+  // complete (a use that was not begun) runs out of its 10 ms.
+  auto drain_copies = [&]() {
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    if (__any_sync(0xffffffffu, sh.expired != 0) && lane == 0 && warp == 4) {
+      auto drain = [&](uint64_t* bar) {
+        for (uint32_t parity = 0; parity < 2; ++parity)
+          for (int n = 0; n < 1000 && !mbar_try_wait(smem_u32(bar), parity, 10000); ++n) {
+          }
+      };
+      for (int n = 0; copy_rows > 0 && n < stages; ++n) drain(&sh.full[n]);
+      drain(&sh.q_full);
+    }
+    __syncwarp();
+  };
+
+  if (warp == 4 && copy_rows > 0) {
+    // Copies by TMA. Lane l knows where piece l (copy_rows rows) of a tile comes from.
     const int pieces = kTile / copy_rows;
     int stage = 0, segment = 0;
     uint32_t lap = 0;  // parity of the ring's current use
@@ -591,66 +609,103 @@ attend_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__
     Walk walk(sh);
     while (ok && __all_sync(0xffffffffu, walk.next(p))) {
       const int* table = c.block_table + walk.b * c.table_stride;
-      int page[2], slot[2];
+      int page, slot;
       // rows behind the sequence come from a page behind the last, as zeros
+      auto place = [&](int tile) {
+        const int row = tile * kTile + lane * copy_rows;
+        page = c.pages;
+        slot = 0;
+        if (lane < pieces && tile < walk.t + walk.count && row < walk.rows) {
+          const int at = row / c.page_size;
+          slot = row - at * c.page_size;
+          const int id = table[at];
+          page = id < 0 || id > c.pages ? c.pages : id;
+        }
+      };
+      place(walk.t);
+      const int count = __shfl_sync(0xffffffffu, walk.count, 0);
+      for (int tile = 0; tile < count; ++tile) {
+        const uint32_t full = smem_u32(&sh.full[stage]), to = smem_u32(ring) + stage * tile_bytes;
+        if (!first_lap && !(ok = waits.wait_all(smem_u32(&sh.pv_done[stage]), lap ^ 1, kAtFree))) break;
+        if (lane == 0) mbar_expect_tx(full, tile_bytes);
+        __syncwarp();
+        for (int k = 0; k < pieces; ++k)
+          tma_load_5d(to + k * (copy_rows >> 3) * group_bytes, &row_map, 0, 0, __shfl_sync(0xffffffffu, slot, k) >> 3,
+                      __shfl_sync(0xffffffffu, page, k), full);
+        if (++stage == stages) stage = 0, lap ^= 1, first_lap = false;
+        if (tile == 0 && !(ok = copy_queries(segment, walk.b))) break;
+        place(walk.t + tile + 1);  // on its way during the waits
+      }
+      ++segment;
+    }
+    drain_copies();
+  } else if ((warp == 4 || warp > 5) && copy_rows == 0) {
+    // Copies row by row, every third row of a tile, 16 bytes a lane. Lane l knows where rows l and l + 32 of a tile come from. A tile
+    // is announced once its copies have landed: when the next one's are on their way, or when nothing else can be done.
+    const int first_row = warp == 4 ? 0 : warp - 5;
+    const uint16_t* const data = static_cast<const uint16_t*>(c.data);
+    int stage = 0, segment = 0, landing = -1;
+    uint32_t lap = 0;
+    bool first_lap = true, ok = __all_sync(0xffffffffu, sh.expired == 0);
+    auto announce = [&](bool all) {
+      if (landing < 0) return;
+      if (all)
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+      else
+        asm volatile("cp.async.wait_group 1;" ::: "memory");
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&sh.full[landing]));
+      landing = -1;
+    };
+    Walk walk(sh);
+    while (ok && __all_sync(0xffffffffu, walk.next(p))) {
+      const int* table = c.block_table + walk.b * c.table_stride;
+      long long from[2];  // element offset, -1 where there is no row: zeros
       auto place = [&](int tile) {
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-          const int piece = lane + 32 * k, row = tile * kTile + piece * copy_rows;
-          page[k] = c.pages;
-          slot[k] = 0;
-          if (piece < pieces && tile < walk.t + walk.count && row < walk.rows) {
-            const int at = row / c.page_size;
-            slot[k] = row - at * c.page_size;
-            const int id = table[at];
-            page[k] = id < 0 || id > c.pages ? c.pages : id;
+          const int in_tile = lane + 32 * k, row = tile * kTile + in_tile;
+          from[k] = -1;
+          if (in_tile < kTile && tile < walk.t + walk.count && row < walk.rows) {
+            const int at = row / c.page_size, id = table[at];
+            if (id >= 0 && id < c.pages) from[k] = id * c.page_stride + static_cast<long long>(row - at * c.page_size) * c.slot_stride;
           }
         }
       };
       place(walk.t);
       const int count = __shfl_sync(0xffffffffu, walk.count, 0);
-      for (int tile = 0; ok && tile < count; ++tile) {
-        const uint32_t full = smem_u32(&sh.full[stage]), to = smem_u32(ring) + stage * tile_bytes;
-        if (!first_lap && !(ok = waits.wait_all(smem_u32(&sh.pv_done[stage]), lap ^ 1, kAtFree))) break;
-        if (lane == 0) mbar_expect_tx(full, tile_bytes);
-        __syncwarp();
-        if (copy_rows >= 8) {
-          for (int i = 0; i < pieces; ++i)
-            tma_load_5d(to + i * (copy_rows >> 3) * group_bytes, &row_map, 0, 0, __shfl_sync(0xffffffffu, slot[0], i) >> 3,
-                        __shfl_sync(0xffffffffu, page[0], i), full);
-        } else {
-#pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            const int piece = lane + 32 * k, row = piece * copy_rows;
-            if (piece < pieces)
-              for (int i = 0; i < chunks; ++i)
-                tma_load_4d_own(to + (row >> 3) * group_bytes + i * kGroupBytes + (row & 7) * kRowBytes, &row_map, slot[k], i, page[k], full);
-          }
+      for (int tile = 0; tile < count; ++tile) {
+        if (!first_lap && !__all_sync(0xffffffffu, mbar_test(smem_u32(&sh.pv_done[stage]), lap ^ 1))) {
+          announce(true);
+          if (!(ok = waits.wait_all(smem_u32(&sh.pv_done[stage]), lap ^ 1, kAtFree))) break;
         }
+        const uint32_t to = smem_u32(ring) + stage * tile_bytes;
+        for (int row = first_row; row < kTile; row += kRowWarps) {
+          const long long at = __shfl_sync(0xffffffffu, row < 32 ? from[0] : from[1], row & 31);
+          const uint16_t* const src = data + (at < 0 ? 0 : at) + 8 * lane;
+          const uint32_t bytes = at < 0 ? 0u : 16u;
+          // 16-byte piece n of a chunk's 128 bytes lies at piece n ^ (row % 8)
+          const uint32_t dst = to + (row >> 3) * group_bytes + (row & 7) * kRowBytes + (((lane & 7) ^ (row & 7)) << 4) + (lane >> 3) * kGroupBytes;
+#pragma unroll
+          for (int k = 0; k < 3; ++k)
+            if (lane + 32 * k < 8 * chunks)
+              asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + 4 * k * kGroupBytes), "l"(src + 256 * k), "r"(bytes) : "memory");
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        announce(false);
+        landing = stage;
         if (++stage == stages) stage = 0, lap ^= 1, first_lap = false;
-        if (tile == 0) {
-          // The queries of this segment, once the first products of the segment before are over.
-          if (segment > 0 && !(ok = waits.wait_all(smem_u32(&sh.q_empty), (segment - 1) & 1, kAtQEmpty))) break;
-          if (lane == 0) mbar_expect_tx(smem_u32(&sh.q_full), chunks * HT * kRowBytes);
-          __syncwarp();
-          tma_load_4d(smem_u32(q_smem), &q_map, head0, 0, walk.b, smem_u32(&sh.q_full));
+        if (tile == 0 && warp == 4) {
+          announce(true);
+          if (!(ok = copy_queries(segment, walk.b))) break;
         }
         place(walk.t + tile + 1);  // on its way during the waits
       }
       ++segment;
     }
-    if (__any_sync(0xffffffffu, sh.expired != 0) && lane == 0) {
-      // A wait has expired somewhere: no copy may still be in flight when the CTA ends. A phase that will not complete (a use that
-      // was not begun) runs out of its 10 ms.
-      auto drain = [&](uint64_t* bar) {
-        for (uint32_t parity = 0; parity < 2; ++parity)
-          for (int n = 0; n < 1000 && !mbar_try_wait(smem_u32(bar), parity, 10000); ++n) {
-          }
-      };
-      for (int n = 0; n < stages; ++n) drain(&sh.full[n]);
-      drain(&sh.q_full);
-    }
-    __syncwarp();
+    announce(true);
+    drain_copies();
   } else if (warp == 5) {
     // Products. All lanes walk along, and votes make the branches uniform: the operands of the instructions are then formed in
     // uniform registers. With one lane walking alone, each instruction took 97 clocks to issue. (Two issuing warps, one for each
@@ -768,7 +823,7 @@ attend_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__
       }
     }
     __syncwarp();
-  } else {
+  } else if (warp < 4) {
     // Softmax: warp w has heads 16 w .. 16 w + 15 of the tile, thread t rows (heads) t / 4 and t / 4 + 8 of these.
     const bool active = 16 * warp < HT;
     const int row0 = 16 * warp + lane / 4, row1 = row0 + 8;
@@ -883,7 +938,7 @@ attend_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__
         if (left < kTile) {
           // What lies behind the sequence in its last page may be anything: as values it has to be 0, because 0 weights times
           // infinity or NaN would be NaN. (Pieces that begin behind the sequence have come as zeros.)
-          const int end = (left + copy_rows - 1) / copy_rows * copy_rows;
+          const int end = copy_rows > 0 ? (left + copy_rows - 1) / copy_rows * copy_rows : left;
           for (int row = left + warp; row < end; row += kSoftmaxThreads / 32) {
             uint8_t* const at = ring + here.stage * tile_bytes + (row >> 3) * group_bytes + (row & 7) * kRowBytes;
             for (int piece = lane; piece < 16 * v_units; piece += 32)  // 16 bytes each
@@ -1623,6 +1678,7 @@ int b200_mla_cache_attend(const b200_mla_cache* cache, const void* q, long long 
   p.tile = tile_rows_for(ht);
   p.extra = extra_for(ht);
   p.copy_rows = cache_walk::copy_rows(cache->page_size, p.tile);
+  if (p.copy_rows < 8) p.copy_rows = 0;
   p.v_units = cache->dv / 128;
   p.chunks = p.cache.d / 64;
   p.scale_log2 = scale * kLog2E;
@@ -1640,13 +1696,17 @@ int b200_mla_cache_attend(const b200_mla_cache* cache, const void* q, long long 
   q_dims.add(heads, q_sh, ht);
   q_dims.add(p.chunks, 64, p.chunks);
   q_dims.add(cache->batch, q_sb, 1);
-  // Copies of whole groups of 8 rows bring all chunks; shorter ones (pages that no 8 divides) a chunk each.
-  const bool groups = p.copy_rows >= 8;
-  row_dims.add(groups ? 8 : cache->page_size, cache->slot_stride, groups ? 8 : p.copy_rows);
-  row_dims.add(p.chunks, 64, groups ? p.chunks : 1);
-  if (groups) row_dims.add(cache->page_size / 8, 8 * cache->slot_stride, p.copy_rows / 8);
-  row_dims.add(cache->pages, cache->page_stride, 1);
-  if (!q_dims.encode(&q_map, q, bf16) || !row_dims.encode(&row_map, cache->data, bf16)) return B200_FP8_MM_ERR_DRIVER;
+  if (p.copy_rows > 0) {
+    row_dims.add(8, cache->slot_stride, 8);
+    row_dims.add(p.chunks, 64, p.chunks);
+    row_dims.add(cache->page_size / 8, 8 * cache->slot_stride, p.copy_rows / 8);
+    row_dims.add(cache->pages, cache->page_stride, 1);
+  }
+  if (!q_dims.encode(&q_map, q, bf16)) return B200_FP8_MM_ERR_DRIVER;
+  if (p.copy_rows == 0)
+    row_map = q_map;  // (not used)
+  else if (!row_dims.encode(&row_map, cache->data, bf16))
+    return B200_FP8_MM_ERR_DRIVER;
   const AttendFn fn = attend_fn(bf16, ht);
   static std::atomic<bool> opted[kMaxDevices][6];
   if (!opt_in(fn, kMaxSmem, &opted[device][(bf16 ? 0 : 3) + (ht == 16 ? 0 : ht == 32 ? 1 : 2)])) return B200_FP8_MM_ERR_DRIVER;
