@@ -202,6 +202,7 @@ struct AttendParams {
   int heads, head_tiles, max_len, batch;
   int workers, least;      // workers per head tile, and the least places worth one
   int tile, extra;         // rows per tile; see cache_walk.h
+  int joined;              // a join follows; else no sequence can be split
   int copy_rows;           // rows of a TMA copy, 0: copies row by row
   int stages;              // tiles of the ring
   int v_units, chunks;     // 128-element units of the value; 64-element chunks of a row
@@ -442,14 +443,16 @@ static_assert(sizeof(AttendShared) <= kHeaderBytes, "the header is too small");
 // A worker's walk over its share: segment after segment, each a run of tiles of one sequence.
 struct Walk {
   int b, t, rows, count;   // sequence and first tile of the segment, rows of the sequence, tiles of the segment
+  int slot;                // where a part of it is left
   long long begin, from, to;
 
-  __device__ __forceinline__ Walk(const AttendShared& sh) : b(sh.first_seq - 1), t(0), rows(0), count(0), begin(sh.first_begin), from(sh.share), to(sh.share_end) {}
+  __device__ __forceinline__ Walk(const AttendShared& sh) : b(sh.first_seq - 1), t(0), rows(0), count(0), slot(0), begin(sh.first_begin), from(sh.share), to(sh.share_end) {}
   __device__ __forceinline__ bool next(const AttendParams& p) {
     while (begin < to) {
       ++b;
       rows = rows_of(p.cache, b, p.max_len);
       count = cache_walk::tiles_in(begin, cache_walk::tiles_of(rows, p.tile), p.extra, from, to, &t);
+      slot = cache_walk::part_slot(from, begin);
       begin += cache_walk::places_of(rows, p.tile, p.extra);
       if (rows > 0 && count > 0) return true;
     }
@@ -600,6 +603,22 @@ attend_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__
     __syncwarp();
   };
 
+  // Warps 6 and 7: where no join follows, what sequences without rows get.
+  auto write_empty = [&]() {
+    if (p.joined) return;
+    const int heads = min(HT, heads_all - head0);
+    for (int b = worker; b < p.batch; b += p.workers) {
+      if (rows_of(c, b, p.max_len) > 0) continue;
+      for (int h = warp - 6; h < heads; h += 2) {
+        T* const out = out_at + b * out_sb + (head0 + h) * out_sh;
+        for (int e = lane; e < c.dv; e += 32) from_float(0.f, out + e);
+        const long long at = static_cast<long long>(b) * heads_all + head0 + h;
+        if (lane == 0) p.lse2[at] = -INFINITY;
+        if (lane == 0 && p.lse != nullptr) p.lse[at] = -INFINITY;
+      }
+    }
+  };
+
   if (warp == 4 && copy_rows > 0) {
     // Copies by TMA. Lane l knows where piece l (copy_rows rows) of a tile comes from.
     const int pieces = kTile / copy_rows;
@@ -706,6 +725,9 @@ attend_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__
     }
     announce(true);
     drain_copies();
+    if (warp > 5) write_empty();
+  } else if (warp > 5) {
+    write_empty();
   } else if (warp == 5) {
     // Products. All lanes walk along, and votes make the branches uniform: the operands of the instructions are then formed in
     // uniform registers. With one lane walking alone, each instruction took 97 clocks to issue. (Two issuing warps, one for each
@@ -841,7 +863,6 @@ attend_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__
       if (ok && !mbar_test(smem_u32(bar), parity)) ok = waits.wait(smem_u32(bar), parity, where);
     };
     Walk walk(sh);
-    bool first_segment = true;
     while (walk.next(p)) {
       float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
       for (int tile = 0; tile < walk.count; ++tile, ++i) {
@@ -973,7 +994,7 @@ attend_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__
       tcgen05_fence_after();
       const int heads = min(HT, heads_all - head0);
       const bool whole = walk.whole(kTile);
-      const long long part = (static_cast<long long>(worker) * p.head_tiles + head_tile) * 2 + (first_segment ? 0 : 1);
+      const long long part = (static_cast<long long>(worker) * p.head_tiles + head_tile) * 2 + walk.slot;
       // kCols heads of 128 value elements at a time: a warp writes 32 elements of a head at once
       constexpr int kCols = HT < 32 ? HT : 32;
       for (int u = 0; u < v_units; ++u) {
@@ -1009,7 +1030,6 @@ attend_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__
       } else if (tid < heads) {
         p.part_stat[part * HT + tid] = sh.stat[tid];
       }
-      first_segment = false;
     }
   }
   tcgen05_fence_before();
@@ -1043,7 +1063,9 @@ __global__ void __launch_bounds__(128 * GROUPS) attend_join_kernel(const __grid_
     return;
   }
   const int workers = cache_walk::workers_of(places, p.workers, p.least);
-  const int g0 = cache_walk::worker_of(places, workers, begin + p.extra), parts = cache_walk::worker_of(places, workers, end - 1) - g0 + 1;
+  const int tiles = static_cast<int>(end - begin) - p.extra;
+  const int g0 = cache_walk::worker_of(places, workers, cache_walk::first_place(begin, tiles, p.extra));
+  const int parts = cache_walk::worker_of(places, workers, cache_walk::last_place(begin, tiles, p.extra)) - g0 + 1;
   if (parts == 1) return;  // written by its worker
   const int head_tile = h / tile_heads, in_tile = h - head_tile * tile_heads;
   // Only the first part can lie behind another sequence's in its worker's share.
@@ -1682,6 +1704,7 @@ int b200_mla_cache_attend(const b200_mla_cache* cache, const void* q, long long 
   p.v_units = cache->dv / 128;
   p.chunks = p.cache.d / 64;
   p.scale_log2 = scale * kLog2E;
+  p.joined = cache_walk::tiles_of(max_len, p.tile) > cache_walk::kWholeTiles;
   p.begins = reinterpret_cast<long long*>(ws);
   p.lse2 = reinterpret_cast<float*>(ws + w.lse2);
   p.part_stat = reinterpret_cast<float2*>(ws + w.part_stat);
@@ -1714,7 +1737,9 @@ int b200_mla_cache_attend(const b200_mla_cache* cache, const void* q, long long 
   if (rc != B200_FP8_MM_OK) return rc;
   // Eight groups where a sequence has eight parts and more on average, one where most have one or two.
   const dim3 joins(static_cast<unsigned>(heads), static_cast<unsigned>(cache->batch));
-  if (p.workers / cache->batch >= 8)
+  if (!p.joined)
+    rc = B200_FP8_MM_OK;
+  else if (p.workers / cache->batch >= 8)
     rc = launch_pdl(bf16 ? attend_join_kernel<__nv_bfloat16, 8> : attend_join_kernel<__half, 8>, joins, 1024, 0, stream, p, ht);
   else
     rc = launch_pdl(bf16 ? attend_join_kernel<__nv_bfloat16, 1> : attend_join_kernel<__half, 1>, joins, 128, 0, stream, p, ht);

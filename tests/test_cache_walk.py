@@ -30,19 +30,18 @@ int main(int argc, char** argv) {
   for (int g = 0; g < workers; ++g) {
     const long long from = share_begin(places, workers, g), to = share_begin(places, workers, g + 1);
     printf("%d %lld\\n", g, to - from);
-    bool first_segment = true;
     for (int b = 0; b < batch; ++b) {
       int first;
       const int count = rows[b] > 0 ? tiles_in(begins[b], tiles_of(rows[b], tile), extra, from, to, &first) : 0;
       if (count == 0) continue;
       printf("s %d %d %d %d\\n", b, g, first, count);
-      if (count != tiles_of(rows[b], tile)) printf("w %d %d %d %d %d\\n", b, g, first_segment ? 0 : 1, first, count);
-      first_segment = false;
+      if (count != tiles_of(rows[b], tile)) printf("w %d %d %d %d %d\\n", b, g, part_slot(from, begins[b]), first, count);
     }
   }
   for (int b = 0; b < batch; ++b) {
     if (begins[b] == begins[b + 1]) continue;
-    const int g0 = worker_of(places, workers, begins[b] + extra), g1 = worker_of(places, workers, begins[b + 1] - 1);
+    const int tiles = tiles_of(rows[b], tile);
+    const int g0 = worker_of(places, workers, first_place(begins[b], tiles, extra)), g1 = worker_of(places, workers, last_place(begins[b], tiles, extra));
     for (int g = g0; g1 > g0 && g <= g1; ++g) printf("j %d %d %d\\n", b, g, g == g0 ? part_slot(share_begin(places, workers, g), begins[b]) : 0);
   }
   for (int p = 1; p <= 300; ++p) printf("r %d %d\\n", p, copy_rows(p, tile));
@@ -71,7 +70,7 @@ def walk(tmp_path_factory):
 def test_shares_and_parts(walk, most, least, tile, extra):
     rng = random.Random(most + least + extra)
     for rows in ([1], [64], [65], [0, 0], [0, 5, 0], [9000], [1] * 200, [rng.randint(0, 900) for _ in range(60)],
-                 [rng.choice([0, 1, 64, 65, 20000]) for _ in range(30)]):
+                 [rng.choice([0, 1, 64, 65, 20000]) for _ in range(30)], [60] * 128, [256, 257, 192, 193, 300] * 20):
         lines = walk(most, least, tile, extra, *rows)
         sizes = [int(f[1]) for f in lines if f[0].isdigit()]
         tiles = [-(-n // tile) for n in rows]
@@ -86,6 +85,7 @@ def test_shares_and_parts(walk, most, least, tile, extra):
                 assert s[2] == at and s[3] > 0
                 at += s[3]
             assert at == n
+            assert n > 4 or sum(s[0] == b for s in segments) <= 1
         written = [tuple(map(int, f[1:])) for f in lines if f[0] == "w"]
         assert [w[:3] for w in sorted(written)] == [tuple(map(int, f[1:])) for f in lines if f[0] == "j"]
         assert len({w[1:3] for w in written}) == len(written)  # no two parts in one place

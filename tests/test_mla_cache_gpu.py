@@ -121,11 +121,17 @@ def test_attend_one_sequence(n):
 
 
 @pytest.mark.parametrize("lens", [[0], [0, 0, 0], [1] * 300, [0] * 150 + [2000] + [0] * 150, [5000, 1, 0, 4000, 70],
-                                  [(37 * i) % 400 for i in range(250)], [128] * 148, [64 * 149]],
-                         ids=["none", "all_empty", "many_single", "one_among_empty", "uneven", "250", "148", "149_tiles"])
-def test_attend_batches(lens):
-    bt = Batch(lens, 16, dv=256, page=16, seed=len(lens))
+                                  [(37 * i) % 400 for i in range(250)], [128] * 148, [64 * 149], [(11 * i) % 193 for i in range(300)]],
+                         ids=["none", "all_empty", "many_single", "one_among_empty", "uneven", "250", "148", "149_tiles", "short"])
+@pytest.mark.parametrize("heads,page", [(16, 16), (70, 5)])
+def test_attend_batches(lens, heads, page):
+    bt = Batch(lens, heads, dv=256, page=page, seed=len(lens))
     check_attend(bt, *bt.attend(return_lse=True))
+    if max(lens) <= 192:  # no sequence can be split then, and a single kernel does all
+        score = torch.rand(len(lens), bt.capacity, generator=bt.g, device="cuda")
+        before = score.clone()
+        out, lse = bt.attend(return_lse=True, score=score, max_len=max(max(lens), 1))
+        check_attend(bt, out, lse, score, before)
 
 
 @pytest.mark.parametrize("heads,lens", [(16, [300, 0, 1, 64, 1000]), (128, [2049, 65, 3]), (70, [4000]), (3, [1] * 200)])
