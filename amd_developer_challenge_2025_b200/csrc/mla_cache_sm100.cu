@@ -760,32 +760,32 @@ attend_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__
       umma_commit(smem_u32(&sh.pv_done[pv_stage]));
       pending = false;
     };
-    // What the products wait for is looked at all at once, a barrier per lane: the first product of tile i for its rows (lane 0), a buffer
-    // of S (1) and, where a segment begins, the queries (2); the pending second one for the weights (3) and, where its segment begins,
-    // for the accumulators of the one before to have been read (4). Without branches, which took as long as twenty products.
-    constexpr uint32_t kFirst = 7u, kSecond = 0x18u;
-    const uint32_t bar_base = smem_u32(lane == 1 ? &sh.s_free[0] : lane == 2 ? &sh.q_full : lane == 3 ? &sh.p_full : lane == 4 ? &sh.o_free : &sh.full[0]);
-    const uint32_t stage_step = lane == 0 ? 8u : 0u, buffer_step = lane == 1 ? 8u : 0u;
-    uint32_t bar = bar_base, parity = 0, idle = 0;
-    auto look_at = [&](uint32_t wanted, bool begins) {
-      const uint32_t parities = lap | ((static_cast<uint32_t>(i) >> 1 & 1u) ^ 1u) << 1 | (static_cast<uint32_t>(segment) & 1u) << 2 |
-                                (static_cast<uint32_t>(pv_tile) & 1u) << 3 | (static_cast<uint32_t>(pv_segment - 1) & 1u) << 4;
-      const uint32_t needed = wanted & (begins ? 0x1bu | 4u : 0x1bu) & (pending_first && pv_segment > 0 ? 0x1fu : 0xfu) & (pending ? 0x1fu : 7u);
-      bar = bar_base + static_cast<uint32_t>(stage) * stage_step + (static_cast<uint32_t>(i) & 1u) * buffer_step;
-      parity = parities >> lane & 1u;
-      idle = ~needed >> lane & 1u;
+    // Whether the first product of tile i can go: its rows, a buffer of S and, where a segment begins, the queries. The second one of the
+    // tile before: the weights and, where its segment begins, the accumulators of the one before read out. All lanes look at the same
+    // barriers: 17 clocks each; a barrier per lane, all at once, took 200.
+    auto first_ready = [&](bool begins) {
+      uint32_t there = mbar_test(smem_u32(&sh.full[stage]), lap) & mbar_test(smem_u32(&sh.s_free[i & 1]), (static_cast<uint32_t>(i) >> 1 & 1u) ^ 1u);
+      if (begins) there &= mbar_test(smem_u32(&sh.q_full), static_cast<uint32_t>(segment) & 1u);
+      return __all_sync(kAll, there != 0) != 0;
     };
-    // Looks until all of `wanted` is there, and returns all that is; 0 when a wait has expired. While the first product cannot go, the
-    // second one does as soon as it can: it frees the ring.
-    auto until = [&](uint32_t wanted) {
+    auto second_ready = [&]() {
+      uint32_t there = mbar_test(smem_u32(&sh.p_full), static_cast<uint32_t>(pv_tile) & 1u);
+      if (pending_first && pv_segment > 0) there &= mbar_test(smem_u32(&sh.o_free), static_cast<uint32_t>(pv_segment - 1) & 1u);
+      return __all_sync(kAll, there != 0) != 0;
+    };
+    // Waits for the first product to become possible, or for the pending second one (`first` false); the second one goes meanwhile as
+    // soon as it can, because it frees the ring.
+    auto until = [&](bool first, bool begins) {
       unsigned long long t0 = 0;  // (read late: reading the timer takes several hundred clocks)
       for (uint32_t spins = 1;; ++spins) {
-        const uint32_t there = __ballot_sync(kAll, (mbar_test(bar, parity) | idle) != 0);
-        if ((there & wanted) == wanted) return there;
-        if (wanted == kFirst && pending && (there & kSecond) == kSecond) second();
-        if ((spins & 255u) == 0) {
+        if (first && first_ready(begins)) return true;
+        if (pending && second_ready()) {
+          if (!first) return true;
+          second();
+        }
+        if ((spins & 1023u) == 0) {
           if (t0 == 0) t0 = global_ns();
-          if (__any_sync(kAll, waits.give_up(t0, parity, kAtOperands))) return 0u;
+          if (__any_sync(kAll, waits.give_up(t0, static_cast<uint32_t>(i), kAtOperands))) return false;
         }
       }
     };
@@ -793,14 +793,10 @@ attend_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__
     Walk walk(sh);
     while (ok && __all_sync(kAll, walk.next(p))) {
       const int count = __shfl_sync(kAll, walk.count, 0);
-      bool known = false;  // all that the tile's first product needs has been seen
       for (int tile = 0; tile < count; ++tile) {
-        if (!known) {
-          look_at(kFirst | kSecond, tile == 0);
-          if (until(kFirst) == 0) {
-            ok = false;
-            break;
-          }
+        if (!until(true, tile == 0)) {
+          ok = false;
+          break;
         }
         tcgen05_fence_after();
         const uint32_t values = kLoV | (ring_at + stage * (tile_bytes >> 4));
@@ -813,17 +809,12 @@ attend_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__
         umma_commit(smem_u32(&sh.s_full[i & 1]));
         if (tile == count - 1) umma_commit(smem_u32(&sh.q_empty));
         if (++stage == stages) stage = 0, lap ^= 1;
-        known = false;
         ++i;
         if (pending) {
-          // (of the tile before; what the next tile's first product needs is looked at along with it)
-          look_at(kFirst | kSecond, false);
-          const uint32_t there = until(kSecond);
-          if (there == 0) {
+          if (!until(false, false)) {
             ok = false;
             break;
           }
-          known = tile + 1 < count && (there & kFirst) == kFirst;
           second();
         }
         pending = true;
@@ -835,10 +826,7 @@ attend_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__
       }
       ++segment;
     }
-    if (ok && pending) {
-      look_at(kSecond, false);
-      if (until(kSecond) != 0) second();
-    }
+    if (ok && pending && until(false, false)) second();
     if (__any_sync(kAll, sh.expired != 0)) {  // none in flight past here
       umma_commit(smem_u32(&sh.drained));
       for (int n = 0; n < 1000 && !mbar_try_wait(smem_u32(&sh.drained), 0, 10000); ++n) {
