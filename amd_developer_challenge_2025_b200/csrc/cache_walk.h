@@ -38,7 +38,7 @@ CACHE_WALK_FN int worker_of(long long places, int workers, long long t) {
   return static_cast<int>(((t + 1) * workers - 1) / places);
 }
 
-constexpr int kWholeTiles = 4;  // 128 sequences of 60 rows, 32 heads: 20.6 us split evenly, 1x whole
+constexpr int kWholeTiles = 4;  // 128 sequences of 60 rows, 32 heads: 20.6 us split evenly, 16.2 whole
 
 // Places of a sequence whose holders have its first and its last part.
 CACHE_WALK_FN long long first_place(long long begin, int tiles, int extra) { return begin + extra + (tiles <= kWholeTiles ? tiles / 2 : 0); }

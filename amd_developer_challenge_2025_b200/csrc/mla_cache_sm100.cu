@@ -175,9 +175,8 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_con
 
 constexpr float kLn2 = 0.69314718055994531f, kLog2E = 1.4426950408889634f;
 constexpr int kMaxD = 576;
-// Rows of the cache per tile. A tile is fetched, multiplied, weighed and multiplied again, and several are under way at a time: what is
-// in flight decides the rate. 64 heads leave room for two tiles of 64 rows, fewer heads for three of 48: 128 sequences of 4096 rows with
-// 16 heads 132 -> 1xx us.
+// Rows of the cache per tile. 64 heads leave room for two tiles of 64 rows, fewer heads for three of 48 (more in flight: 128 sequences of
+// 4096 rows with 16 heads 132 -> 125 us).
 __host__ __device__ constexpr int tile_rows_for(int tile_heads) { return tile_heads < 64 ? 48 : 64; }
 constexpr int kRowBytes = 128;                 // of a row that lie together under the 128-byte swizzle: a chunk of 64 elements
 constexpr int kGroupBytes = 8 * kRowBytes;     // 8 rows of a chunk, the swizzle's period
@@ -470,17 +469,20 @@ struct Walk {
 // lanes, 128 heads would take them all and leave none for S. Fewer heads shrink N (16 or 32) and what Q takes of shared memory.
 //
 // A tile lies in shared memory as [groups of 8 rows][chunk of 64 elements][8 rows x 128 bytes]: one stride from group to group and one
-// from chunk to chunk for both operands, and one copy brings all chunks of as many rows as lie together in a page, up to half a tile.
-// What bounds the loop is how long a tile stays, from its copy's way through memory over both products and the softmax between them,
-// and what fits next to Q; so the second product goes by halves of the rows and frees each for its next copy. (Tiles of 32 rows, more
-// of them in flight, are slower: an MMA takes 27 clocks to issue however small it is.)
+// from chunk to chunk for both operands, and one copy brings all chunks of as many rows as lie together in a page, up to the tile.
 //
-// One CTA per SM and worker: warp 4 copies (with warps 6 and 7 where pages are not whole groups of 8 rows, which TMA would have to
-// bring in copies of 128 to 512 bytes: 16 bytes a thread then), warp 5 issues the products, warps 0 to 3 do the softmax (S comes as 16 x 256-bit
-// fragments, 4 threads to a head) and the epilogue. S is double buffered; the next tile's first product runs under this tile's
-// softmax. The running maximum is replaced only when a logit exceeds it by 2^8: the weights stay below 2^8, which no type here
-// minds, and rescaling the accumulators is rare. Sums are kept in fp32, weights are rounded to the cache's type for the second
-// product, as matrix operands have to be.
+// What bounds it: up to 32 heads, memory (6.2 TB/s while it runs); 64 heads, how long a tile stays. From its copy's way through memory
+// (2200 to 3000 clocks) over the first product (1170), the softmax (1300) and the second product (740) to the next copy it takes 6800, and
+// two tiles of 64 rows are all that fits next to Q: 3400 clocks a tile, where the tensor core needs 1900 and, for 128 heads, memory 1600.
+// Tiles of 32 rows, four of them in flight, were slower (162 against 142 us, 64 sequences of 4096 rows with 128 heads): an MMA takes 27
+// clocks to issue however small it is. So were units of 128 elements as the ring's grain, and halves of a tile freed one by one.
+//
+// One CTA per SM and worker: warp 4 copies (with warps 6 and 7, 16 bytes a lane, where pages are not whole groups of 8 rows: TMA would
+// have to bring them in copies of 128 to 512 bytes, 579 against 99 us for pages of one row), warp 5 issues the products, warps 0 to 3 do
+// the softmax (S comes as 16 x 256-bit fragments, 4 threads to a head) and the epilogue. S is double buffered; the next tile's first
+// product runs under this tile's softmax. The running maximum is replaced only when a logit exceeds it by 2^8: the weights stay below
+// 2^8, which no type here minds, and rescaling the accumulators is rare. Sums are kept in fp32, weights are rounded to the cache's type
+// for the second product, as matrix operands have to be.
 template <typename T, int HT>
 __global__ void __launch_bounds__(kAttendThreads, 1)
 attend_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap row_map, const __grid_constant__ AttendParams p) {
@@ -970,15 +972,16 @@ attend_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__
           l0 += __shfl_xor_sync(0xffffffffu, l0, o);
           l1 += __shfl_xor_sync(0xffffffffu, l1, o);
         }
-        if (lane % 4 == 0) {
-          sh.stat[row0] = make_float2(m0, l0);
-          sh.stat[row1] = make_float2(m1, l1);
-          sh.inverse[row0] = 1.f / l0;
-          sh.inverse[row1] = 1.f / l1;
-        }
+      }
+      // (The last second product has needed all four warps' weights: none of them still reads what the segment before left here.)
+      wait(&sh.pv_done[before.stage], before.lap, kAtPvDone);
+      if (active && lane % 4 == 0) {
+        sh.stat[row0] = make_float2(m0, l0);
+        sh.stat[row1] = make_float2(m1, l1);
+        sh.inverse[row0] = 1.f / l0;
+        sh.inverse[row1] = 1.f / l1;
       }
       softmax_sync();
-      wait(&sh.pv_done[before.stage], before.lap, kAtPvDone);
       tcgen05_fence_after();
       const int heads = min(HT, heads_all - head0);
       const bool whole = walk.whole(kTile);
