@@ -190,6 +190,10 @@ constexpr int kTmemCols = 512;
 constexpr int kTmemLogits = 256;               // two buffers of a tile's columns behind the accumulators
 constexpr unsigned long long kWaitLimitNs = 2000000000ull;
 constexpr float kRescaleAbove = 8.f;  // log2: a running maximum is replaced when it is exceeded by this much
+// log2 of the weight that a running maximum has. fp16 ends at 2^16 and loses bits below 2^-14: at 2^7 (with 2^8 above it to go), rows
+// keep all bits down to 2^-21 of the largest weight, and a long tail's error is 2^-32 of the largest weight a row. bf16 needs none.
+template <typename T>
+constexpr float kTopWeight = std::is_same<T, __half>::value ? 7.f : 0.f;
 
 struct AttendParams {
   CacheView cache;
@@ -480,8 +484,8 @@ struct Walk {
 // One CTA per SM and worker: warp 4 copies (with warps 6 and 7, 16 bytes a lane, where pages are not whole groups of 8 rows: TMA would
 // have to bring them in copies of 128 to 512 bytes, 579 against 99 us for pages of one row), warp 5 issues the products, warps 0 to 3 do
 // the softmax (S comes as 16 x 256-bit fragments, 4 threads to a head) and the epilogue. S is double buffered; the next tile's first
-// product runs under this tile's softmax. The running maximum is replaced only when a logit exceeds it by 2^8: the weights stay below
-// 2^8, which no type here minds, and rescaling the accumulators is rare. Sums are kept in fp32, weights are rounded to the cache's type
+// product runs under this tile's softmax. The running maximum is replaced only when a logit exceeds it by 8 (in base 2): the
+// weights stay below 2^8 in bf16 and 2^15 in fp16, and rescaling the accumulators is rare. Sums are kept in fp32, weights are rounded to the cache's type
 // for the second product, as matrix operands have to be.
 template <typename T, int HT>
 __global__ void __launch_bounds__(kAttendThreads, 1)
@@ -896,9 +900,11 @@ attend_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__
           }
           float f0 = 1.f, f1 = 1.f;
           if (tile == 0) {
-            m0 = t0;
-            m1 = t1;
+            m0 = t0 - kTopWeight<T>;
+            m1 = t1 - kTopWeight<T>;
           } else {
+            t0 -= kTopWeight<T>;
+            t1 -= kTopWeight<T>;
             const bool up0 = t0 > m0 + kRescaleAbove, up1 = t1 > m1 + kRescaleAbove;
             up = up0 || up1;
             if (up0) f0 = exp2_fast(m0 - t0), m0 = t0;
@@ -1662,7 +1668,7 @@ int b200_mla_cache_attend(const b200_mla_cache* cache, const void* q, long long 
   int rc = view_of(cache, &p.cache);
   if (rc != B200_FP8_MM_OK) return rc;
   if (q == nullptr || out == nullptr || (score_out != nullptr && score == nullptr)) return B200_FP8_MM_ERR_NULL;
-  if (heads <= 0 || heads > kMaxHeads || max_len < 0 || !isfinite(scale)) return B200_FP8_MM_ERR_SHAPE;
+  if (heads <= 0 || heads > kMaxHeads || max_len < 0 || !(fabsf(scale) < 0x1p127f)) return B200_FP8_MM_ERR_SHAPE;
   if (cache->batch == 1) q_sb = p.cache.d;  // (no second one)
   if (heads == 1) q_sh = p.cache.d;
   if (q_sb % 8 != 0 || q_sh % 8 != 0 || q_sb < p.cache.d || q_sh < p.cache.d) return B200_FP8_MM_ERR_STRIDE;

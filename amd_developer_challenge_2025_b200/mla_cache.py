@@ -192,7 +192,7 @@ def mla_cache_attend(q, cache, block_table, lens, dv: int, scale: float, out=Non
            and q.data_ptr() % 16 == 0,
            "q: strides must be multiples of 8 elements, at least a row's, and the base address a multiple of 16 bytes")
     scale = float(scale)
-    _check(math.isfinite(scale), "scale must be finite")
+    _check(abs(scale) < 2.0 ** 127, "scale must be finite and below 2**127 in magnitude")
     _check(max_len is None or (isinstance(max_len, int) and max_len > 0), "max_len must be a positive integer")
     max_len = capacity if max_len is None else min(max_len, capacity)
     tensors = [q, cache, block_table, lens]

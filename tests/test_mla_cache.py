@@ -1,5 +1,8 @@
 """Refusals of the paged-cache operators. They are checked before anything touches a GPU, so CPU tensors show them; a call that
 passes every other check is refused for being on the CPU."""
+import os
+import re
+
 import pytest
 import torch
 
@@ -124,7 +127,7 @@ def test_bad_attend(name, bad, match):
 
 def test_attend_arguments_that_disagree():
     t = base()
-    for scale in (float("inf"), float("nan")):
+    for scale in (float("inf"), float("nan"), 1e300, -3e38):
         with pytest.raises(ValueError, match="scale"):
             attend(t, scale=scale)
     for max_len in (0, -1, 2.5):
@@ -194,7 +197,7 @@ def test_error_codes_without_launch(built_library):
     for change in (dict(dtype=2), dict(batch=0), dict(batch=65536), dict(pages=0), dict(page_size=0), dict(pages_per_seq=0),
                    dict(dv=64), dict(dv=640), dict(dr=32), dict(dr=-64), dict(dr=512), dict(page_size=1 << 30)):
         assert call(cache(**change)) == 2, change
-    assert call(cache(), heads=0) == 2 and call(cache(), scale=float("nan")) == 2
+    assert call(cache(), heads=0) == 2 and call(cache(), scale=float("nan")) == 2 and call(cache(), scale=3e38) == 2
     assert call(cache(slot_stride=D - 8)) == 3 and call(cache(page_stride=PS * D + 4)) == 3 and call(cache(), q_sb=H * D + 1) == 3
     assert call(cache(data=4100)) == 4 and call(cache(), q=4104) == 4
     assert call(cache(), ws=None) == 6 and call(cache(), ws_bytes=0) == 6 and call(cache(), ws=4100) == 6
@@ -213,3 +216,12 @@ def test_error_codes_without_launch(built_library):
     assert drop(cache(), budget=0) == 2 and drop(cache(), recent=9) == 2 and drop(cache(), recent=-1) == 2
     assert drop(cache(), ws=None) == 6 and drop(cache(), ws_bytes=0) == 6
     assert lib.b200_mla_cache_evict_workspace_bytes(B, 0, 8) == 0
+
+
+def test_no_read_only_loads():
+    """The kernels begin under the kernel before them, which may still write what they read: nothing may go through the read-only path."""
+    with open(os.path.join(os.path.dirname(pkg.__file__), "csrc", "mla_cache_sm100.cu")) as f:
+        code = re.sub(r"//[^\n]*", "", f.read())
+    assert "griddepcontrol.wait" in code
+    for form in (r"__ldg\s*\(", r"\bld\.global\.nc", r"\bconst\s+[\w:]+\s*\*\s*__restrict__"):
+        assert not re.search(form, code), form

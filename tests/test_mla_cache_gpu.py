@@ -134,6 +134,13 @@ def test_attend_batches(lens, heads, page):
         check_attend(bt, out, lse, score, before)
 
 
+def test_attend_thousands_of_sequences():
+    lens = [37 * i % 130 for i in range(3000)]
+    lens[1234] = 9000
+    bt = Batch(lens, 4, 128, 0, 16, seed=1)
+    check_attend(bt, *bt.attend(return_lse=True))
+
+
 @pytest.mark.parametrize("heads,lens", [(16, [300, 0, 1, 64, 1000]), (128, [2049, 65, 3]), (70, [4000]), (3, [1] * 200)])
 @pytest.mark.parametrize("dtype", TYPES)
 def test_attend_score(heads, lens, dtype):
@@ -220,6 +227,31 @@ def test_attend_infinities_and_nan():
     got = bt.attend()
     bt.rows[0] = bt.rows[0][70:]
     check_attend(bt, got)
+
+
+@pytest.mark.parametrize("heads", [16, 64])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("first", [True, False])
+def test_attend_a_long_tail(heads, dtype, first):
+    """One row far above 20000 others whose weights, 2^-26 of it, are small numbers of fp16, and whose values outweigh its own. fp16
+    weights are kept as multiples of 2^-24, with the largest at 2^7 or more: an error of 2^-32 of the largest weight for each row."""
+    n = 20001
+    bt = Batch([n], heads, page=64, dtype=dtype)
+    bt.q.zero_()
+    bt.q[:, :, bt.dv] = 1
+    x = torch.zeros(n, bt.d, dtype=bt.dtype, device="cuda")
+    hot = 0 if first else n - 1
+    x[:, :bt.dv] = 1000
+    x[:, bt.dv] = -250
+    x[hot] = 2.0 ** -10
+    slot = torch.arange(n, device="cuda")
+    bt.cache[bt.table[0, slot // bt.page].long(), slot % bt.page] = x
+    p = torch.softmax(bt.scale * x[:, bt.dv].double(), 0)
+    want, u = p @ x[:, :bt.dv].double(), half_step(bt.dtype)
+    ds = bt.scale * (bt.d + 2) * 2.0 ** -23 * 250
+    tol = want * (2 * u + u * u + 2 * ds + 2.0 ** -20) + 2.0 ** -32 * n * 1000 * (bt.dtype == torch.float16)
+    assert float(tol.max() / want.min()) < 0.02
+    assert ((bt.attend()[0].double() - want).abs() <= tol).all()
 
 
 @pytest.mark.parametrize("scale", [0.0, -0.05, 3.0])
