@@ -1163,7 +1163,7 @@ __global__ void __launch_bounds__(kScoreGroups * kTile) attend_score_kernel(cons
 // ---------------------------------------------------------------------------------------------
 
 constexpr int kMaxCluster = 8;
-constexpr int kMaxStaged = 32768;               // ranks of a CTA's slots that are kept in shared memory (128 KB)
+constexpr int kMaxStaged = 20480;               // slots of a CTA whose ranks and positions are kept in shared memory (160 KB)
 constexpr int kFewMoves = 64;                   // a sequence's rows that the selecting CTAs move themselves
 constexpr int kMoveThreads = 256;
 
@@ -1186,10 +1186,10 @@ struct EvictParams {
   int few;       // the selecting CTAs move the rows
 };
 
-// Order of the scores as unsigned integers: protected rows above all, NaN above every number, -0 as 0.
-__device__ __forceinline__ uint32_t rank_of(float score, int position, long long safe_above) {
-  if (position > safe_above) return 0xffffffffu;
-  if (score != score) return 0xfffffffeu;
+// Order of the scores as unsigned integers: NaN above every number, -0 as 0. Protected rows are above all.
+constexpr uint32_t kProtected = 0xffffffffu;
+__device__ __forceinline__ uint32_t rank_of(float score) {
+  if (score != score) return kProtected - 1;
   const uint32_t u = __float_as_uint(score + 0.f);
   return (u >> 31) ? ~u : (u | 0x80000000u);
 }
@@ -1199,29 +1199,28 @@ template <int THREADS>
 __device__ __forceinline__ int threads_before(int v, int* scratch, int* total) {
   constexpr int kWarps = THREADS / 32;
   const int warp = static_cast<int>(threadIdx.x) >> 5, lane = static_cast<int>(threadIdx.x) & 31;
-  int upto = v;
+  uint32_t upto = static_cast<uint32_t>(v);  // (two counts of 16 bits may come as one)
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int u = __shfl_up_sync(0xffffffffu, upto, o);
+    const uint32_t u = __shfl_up_sync(0xffffffffu, upto, o);
     if (lane >= o) upto += u;
   }
   __syncthreads();  // (scratch may still be read from the last time)
-  if (lane == 31) scratch[warp] = upto;
+  if (lane == 31) scratch[warp] = static_cast<int>(upto);
   __syncthreads();
-  int w = lane < kWarps ? scratch[lane] : 0;
+  uint32_t w = lane < kWarps ? static_cast<uint32_t>(scratch[lane]) : 0u;
 #pragma unroll
   for (int o = 1; o < kWarps; o <<= 1) {
-    const int u = __shfl_up_sync(0xffffffffu, w, o);
+    const uint32_t u = __shfl_up_sync(0xffffffffu, w, o);
     if (lane >= o) w += u;
   }
-  *total = __shfl_sync(0xffffffffu, w, kWarps - 1);
-  const int before = __shfl_sync(0xffffffffu, w, (warp + 31) & 31);
-  return (warp > 0 ? before : 0) + upto - v;
+  *total = static_cast<int>(__shfl_sync(0xffffffffu, w, kWarps - 1));
+  const uint32_t before = __shfl_sync(0xffffffffu, w, (warp + 31) & 31);
+  return static_cast<int>((warp > 0 ? before : 0u) + upto - static_cast<uint32_t>(v));
 }
 
-__device__ __forceinline__ void move_row(const EvictParams& p, int b, int i, int lane) {
+__device__ __forceinline__ void move_row(const EvictParams& p, int b, int to, int of, int lane) {
   const CacheView& c = p.cache;
-  const int to = p.holes[static_cast<long long>(b) * p.most + i], of = p.late[static_cast<long long>(b) * p.most + i];
   const long long dst = slot_offset(c, b, to), src = slot_offset(c, b, of);
   if (dst >= 0) {
     uint4* o = reinterpret_cast<uint4*>(static_cast<uint16_t*>(c.data) + dst);
@@ -1240,48 +1239,69 @@ __device__ __forceinline__ void move_row(const EvictParams& p, int b, int i, int
 }
 static_assert(kMaxD / 8 <= 96, "move_row holds a row in three pieces a lane");
 
-// A cluster of CTAs per sequence, each with a run of its slots. Finds the budget-th largest rank, as many bits at a time as two bins to
-// a thread allow (9 of 256 threads, 11 of 1024), then the slots
-// to fill and the slots to move, in order. Scores and positions are read once from memory and once from cache; from then on the ranks
-// lie in shared memory, and the CTAs of a cluster read each other's counts there. What it costs is a chain of some thirty barriers,
-// which are dearer the more threads wait: one slot after the other is cheaper up to 4096 slots of a CTA.
+// A cluster of CTAs per sequence, each with a run of its slots. Finds the budget-th largest rank: the range of the ranks is cut into
+// as many bins as two to a thread (512 or 2048), the bin that holds it again, until the bin is one rank or holds no more of them than
+// there are threads, which then count for each how many are larger. Then the slots to fill and the slots to move, in order. Scores and
+// positions are read from memory once; from then on ranks and positions lie in shared memory, and the CTAs of a cluster read each
+// other's counts there. What it costs is a chain of barriers, which are dearer the more threads wait: one slot after the other is
+// cheaper up to 4096 slots of a CTA.
 template <int THREADS>
 __global__ void __launch_bounds__(THREADS, 1) evict_select_kernel(const __grid_constant__ EvictParams p) {
-  constexpr int kWarps = THREADS / 32, kBins = 2 * THREADS, kDigitBits = THREADS == 256 ? 9 : 11, kDigits = (32 + kDigitBits - 1) / kDigitBits;
-  static_assert(kBins == 1 << kDigitBits, "two bins to a thread");
+  constexpr int kWarps = THREADS / 32, kBins = 2 * THREADS, kDigitBits = THREADS == 256 ? 9 : 11;
+  // The first cut leaves one bin for the protected rows: 32 bits to 24 (22), then 15 and 6 (11), then none.
+  constexpr int kDigits = THREADS == 256 ? 4 : 3, kAtOnce = THREADS == 256 ? 16 : 8, kFew = THREADS / 4;
+  static_assert(kBins == 1 << kDigitBits && (kDigits - 1) * kDigitBits + kDigitBits - 1 >= 32, "two bins to a thread, cuts down to one rank");
   extern __shared__ uint32_t ranks[];
   __shared__ alignas(8) int bins[kDigits][kBins];
-  __shared__ alignas(8) int newest_of[kMaxCluster], totals[2];
-  __shared__ int scratch[kWarps], found[2];
-  __shared__ uint32_t above_words[THREADS], tie_words[THREADS];  // which of 32 slots lie above the threshold, and on it
+  __shared__ alignas(8) int totals[2];
+  __shared__ uint32_t newest_of[kMaxCluster], lowest_of[kMaxCluster], highest_of[kMaxCluster], few[kFew];
+  __shared__ int scratch[kWarps], found[4], equal[3], few_count, few_to[kFewMoves], few_of[kFewMoves];
+  // Which of 32 slots lie above the threshold, and on it; then which are to fill, which to move, and how many of both lie before.
+  __shared__ uint32_t above_words[THREADS], tie_words[THREADS], before_words[THREADS];
   const CacheView& c = p.cache;
   const int tid = static_cast<int>(threadIdx.x), warp = tid >> 5, lane = tid & 31;
   const int cluster = p.cluster, b = static_cast<int>(blockIdx.x) / cluster, me = static_cast<int>(blockIdx.x) % cluster, budget = p.budget;
-  auto sync = [&]() {
-    if (cluster == 1) {
-      __syncthreads();
-    } else {
-      asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-      asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-    }
+  auto arrive = [&]() {
+    if (cluster > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   };
-  // Two neighbouring values of the cluster's CTAs `from` to `to`, in sum. (All loads of a thread are on their way together.)
-  auto sum_over = [&](const int* mine, int from, int to) {
-    if (cluster == 1) return from < to ? *reinterpret_cast<const int2*>(mine) : make_int2(0, 0);
-    int2 v[kMaxCluster], s = make_int2(0, 0);
+  auto wait = [&]() {
+    if (cluster > 1)
+      asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    else
+      __syncthreads();
+  };
+  // Two neighbouring values in sum, of all of the cluster's CTAs (x, y) and of those before this one (z, w). (All loads of a thread are
+  // on their way together.)
+  auto sum_over = [&](const int* mine) {
+    if (cluster == 1) {
+      const int2 v = *reinterpret_cast<const int2*>(mine);
+      return make_int4(v.x, v.y, 0, 0);
+    }
+    int2 v[kMaxCluster];
+    int4 s = make_int4(0, 0, 0, 0);
 #pragma unroll
     for (int k = 0; k < kMaxCluster; ++k) {
       v[k] = make_int2(0, 0);
-      if (k < from || k >= to) continue;
+      if (k >= cluster) continue;
       uint32_t at;
       asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(mine)), "r"(k));
       asm volatile("ld.shared::cluster.v2.b32 {%0, %1}, [%2];" : "=r"(v[k].x), "=r"(v[k].y) : "r"(at) : "memory");
     }
 #pragma unroll
-    for (int k = 0; k < kMaxCluster; ++k) s.x += v[k].x, s.y += v[k].y;
+    for (int k = 0; k < kMaxCluster; ++k) {
+      s.x += v[k].x, s.y += v[k].y;
+      if (k < me) s.z += v[k].x, s.w += v[k].y;
+    }
     return s;
   };
+  auto put = [&](const void* mine, int cta, uint32_t value) {  // into that CTA's shared memory
+    uint32_t at;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(mine)), "r"(cta));
+    asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(at), "r"(value) : "memory");
+  };
+  arrive();  // all CTAs are there once this is waited for
   for (int i = tid; i < kDigits * kBins; i += THREADS) (&bins[0][0])[i] = 0;
+  if (tid == 0) few_count = 0;
   pdl_wait();
   pdl_launch_dependents();
   const int len = c.lens[b], n = max(0, min(len, c.capacity));
@@ -1289,10 +1309,14 @@ __global__ void __launch_bounds__(THREADS, 1) evict_select_kernel(const __grid_c
   const int* position = p.position + b * p.position_stride;
   float* score_out = p.score_out + b * p.score_out_stride;
   int* position_out = p.position_out + b * p.position_out_stride;
-  sync();  // lens_out may be lens
-  if (me == 0 && tid == 0) p.lens_out[b] = min(len, budget);
   if (n <= budget) {
-    if (me == 0 && tid == 0) p.moves[b] = 0;
+    wait();
+    arrive();  // lens_out may be lens: all have read it
+    wait();
+    if (me == 0 && tid == 0) {
+      p.lens_out[b] = min(len, budget);
+      if (!p.few) p.moves[b] = 0;
+    }
     for (int i = me * THREADS + tid; i < n; i += cluster * THREADS) {
       score_out[i] = score[i];
       position_out[i] = position[i];
@@ -1300,57 +1324,92 @@ __global__ void __launch_bounds__(THREADS, 1) evict_select_kernel(const __grid_c
     return;
   }
   const int run = ((n + cluster - 1) / cluster + 31) / 32 * 32, begin = min(n, me * run), count = min(n, begin + run) - begin;
-  int newest = INT_MIN;
-#pragma unroll 8
-  for (int i = tid; i < count; i += THREADS) newest = max(newest, position[begin + i]);
-  newest = __reduce_max_sync(0xffffffffu, newest);
-  if (lane == 0) scratch[warp] = newest;
-  __syncthreads();
-  newest = __reduce_max_sync(0xffffffffu, lane < kWarps ? scratch[lane] : INT_MIN);
-  if (cluster > 1) {  // every CTA's goes to all
-    if (tid < cluster) {
-      uint32_t at;
-      asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(&newest_of[me])), "r"(tid));
-      asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(at), "r"(newest) : "memory");
-    }
-    sync();
-    for (int k = 0; k < cluster; ++k) newest = max(newest, newest_of[k]);
-  }
-  const long long safe_above = static_cast<long long>(newest) - p.recent;
   const int staged = p.staged;
-  int* const holes_list = p.holes + static_cast<long long>(b) * p.most;
-  int* const late_list = p.late + static_cast<long long>(b) * p.most;
-  auto rank_at = [&](int i) { return i < staged ? ranks[i] : rank_of(score[begin + i], position[begin + i], safe_above); };
+  int* const positions = reinterpret_cast<int*>(ranks + staged);
   // Slots below the budget keep what they have for now; those given up are written again by the rows that move there.
   const bool copy_scores = score_out != score, copy_positions = position_out != position;
-#pragma unroll 4
-  for (int i = tid; i < count; i += THREADS) {
-    const float s = score[begin + i];
-    const int at = position[begin + i];
-    const uint32_t r = rank_of(s, at, safe_above);
-    if (i < staged) ranks[i] = r;
-    atomicAdd(&bins[0][r >> (32 - kDigitBits)], 1);
-    if (begin + i < budget) {
-      if (copy_scores) score_out[begin + i] = s;
-      if (copy_positions) position_out[begin + i] = at;
+  int newest = INT_MIN;
+  uint32_t lowest = 0xffffffffu, highest = 0u;
+  for (int i0 = tid; i0 < count; i0 += kAtOnce * THREADS) {  // (stores between them would keep the compiler from loading ahead)
+    float s[kAtOnce];
+    int at[kAtOnce];
+#pragma unroll
+    for (int k = 0; k < kAtOnce; ++k) {
+      if (i0 + k * THREADS >= count) break;
+      s[k] = score[begin + i0 + k * THREADS];
+      at[k] = position[begin + i0 + k * THREADS];
     }
-  }
-  uint32_t bits = 0, mask = 0;
-  int left = budget;  // of the rows that share `bits` under `mask`, how many are kept
-  int bin = 0;
-  for (int digit = 0; digit < kDigits; ++digit) {
-    const bool last = digit == kDigits - 1;
-    const int shift = last ? 0 : 32 - kDigitBits * (digit + 1), width = last ? 1 << (32 - (kDigits - 1) * kDigitBits) : kBins;
-    if (digit > 0) {
-      for (int i = tid; i < count; i += THREADS) {
-        const uint32_t r = rank_at(i);
-        if ((r & mask) == bits) atomicAdd(&bins[digit][(r >> shift) & (width - 1)], 1);
+#pragma unroll
+    for (int k = 0; k < kAtOnce; ++k) {
+      const int i = i0 + k * THREADS;
+      if (i >= count) break;
+      const uint32_t r = rank_of(s[k]);
+      newest = max(newest, at[k]);
+      lowest = min(lowest, r);
+      highest = max(highest, r);
+      if (i < staged) {
+        ranks[i] = r;
+        positions[i] = at[k];
+      }
+      if (begin + i < budget) {
+        if (copy_scores) score_out[begin + i] = s[k];
+        if (copy_positions) position_out[begin + i] = at[k];
       }
     }
-    sync();
-    // Thread t has bins width - 1 - 2 t and the one below: counted from the top.
-    const int high = width - 1 - 2 * tid;
-    const int2 pair = high > 0 ? sum_over(&bins[digit][high - 1], 0, cluster) : make_int2(0, 0);
+  }
+  newest = __reduce_max_sync(0xffffffffu, newest);
+  lowest = __reduce_min_sync(0xffffffffu, lowest);
+  highest = __reduce_max_sync(0xffffffffu, highest);
+  if (lane == 0) {  // (above_words and tie_words have their own use later)
+    scratch[warp] = newest;
+    above_words[warp] = lowest;
+    tie_words[warp] = highest;
+  }
+  __syncthreads();
+  newest = __reduce_max_sync(0xffffffffu, scratch[lane % kWarps]);
+  lowest = __reduce_min_sync(0xffffffffu, above_words[lane % kWarps]);
+  highest = __reduce_max_sync(0xffffffffu, tie_words[lane % kWarps]);
+  if (cluster > 1) {  // every CTA's goes to all
+    wait();
+    if (tid < cluster) {
+      put(&newest_of[me], tid, static_cast<uint32_t>(newest));
+      put(&lowest_of[me], tid, lowest);
+      put(&highest_of[me], tid, highest);
+    }
+    arrive();
+    wait();
+    for (int k = 0; k < cluster; ++k) {
+      newest = max(newest, static_cast<int>(newest_of[k]));
+      lowest = min(lowest, lowest_of[k]);
+      highest = max(highest, highest_of[k]);
+    }
+  }
+  if (me == 0 && tid == 0) p.lens_out[b] = budget;  // (all have read lens, which it may be)
+  const long long safe_above = static_cast<long long>(newest) - p.recent;
+  auto rank_at = [&](int i) {
+    if (i < staged) return ranks[i];
+    return position[begin + i] > safe_above ? kProtected : rank_of(score[begin + i]);
+  };
+  int shift = max(0, 32 - __clz(static_cast<int>(highest - lowest)) - kDigitBits);
+  if ((highest - lowest) >> shift > kBins - 2) ++shift;
+  for (int i = tid; i < count; i += THREADS) {
+    uint32_t r;
+    if (i < staged) {
+      r = ranks[i];
+      if (positions[i] > safe_above) ranks[i] = r = kProtected;
+    } else {
+      r = rank_at(i);
+    }
+    atomicAdd(&bins[0][r == kProtected ? kBins - 1 : (r - lowest) >> shift], 1);
+  }
+  // Of the rows with the rank `lowest`, `left` are kept, of `ties`, of which `ties_before` belong to the CTAs before this one.
+  int left = budget, ties = 0, ties_before = 0;
+  for (int digit = 0;; ++digit) {
+    arrive();
+    wait();
+    // Thread t has bins kBins - 1 - 2 t and the one below: counted from the top.
+    const int high = kBins - 1 - 2 * tid;
+    const int4 pair = sum_over(&bins[digit][high - 1]);
     const int n0 = pair.y, n1 = pair.x;
     int total;
     const int above = threads_before<THREADS>(n0 + n1, scratch, &total);
@@ -1358,72 +1417,136 @@ __global__ void __launch_bounds__(THREADS, 1) evict_select_kernel(const __grid_c
       const bool second = left > above + n0;
       found[0] = high - (second ? 1 : 0);
       found[1] = above + (second ? n0 : 0);
+      found[2] = second ? n1 : n0;
+      found[3] = second ? pair.z : pair.w;
     }
     __syncthreads();
-    bin = found[0];
-    bits |= static_cast<uint32_t>(bin) << shift;
-    mask |= static_cast<uint32_t>(width - 1) << shift;
+    const int bin = found[0];
     left -= found[1];
-    __syncthreads();
+    ties = found[2];
+    ties_before = found[3];
+    const bool safe = digit == 0 && bin == kBins - 1;  // more are protected than stay
+    lowest = safe ? kProtected : lowest + (static_cast<uint32_t>(bin) << shift);
+    if (safe || shift == 0) break;
+    auto inside = [&](uint32_t r) { return r >= lowest && r != kProtected && (r - lowest) >> shift == 0; };
+    if (ties <= kFew) {
+      for (int i = tid; i < count; i += THREADS) {
+        const uint32_t r = rank_at(i);
+        if (!inside(r)) continue;
+        const int to = ties_before + atomicAdd(&few_count, 1);
+        for (int k = 0; k < cluster; ++k) put(&few[to], k, r);
+      }
+      arrive();
+      wait();
+      if (tid < ties) {
+        const uint32_t mine = few[tid];
+        int larger = 0, at_least = 0;
+#pragma unroll 8
+        for (int k = 0; k < ties; ++k) {
+          larger += few[k] > mine;
+          at_least += few[k] >= mine;
+        }
+        if (larger < left && left <= at_least) {  // (threads with the same rank write the same)
+          equal[0] = static_cast<int>(mine);
+          equal[1] = larger;
+          equal[2] = at_least;
+        }
+      }
+      __syncthreads();
+      lowest = static_cast<uint32_t>(equal[0]);
+      left -= equal[1];
+      ties = equal[2] - equal[1];
+      int same_before = 0;
+      for (int k = lane; k < ties_before; k += 32) same_before += few[k] == lowest;
+      ties_before = __reduce_add_sync(0xffffffffu, same_before);
+      break;
+    }
+    const int from = shift;
+    shift = max(0, shift - kDigitBits);
+    for (int i = tid; i < count; i += THREADS) {
+      const uint32_t r = rank_at(i);
+      if (r >= lowest && r != kProtected && (r - lowest) >> from == 0) atomicAdd(&bins[digit + 1][(r - lowest) >> shift], 1);
+    }
   }
-  // Of the rows at the threshold the first `left` stay; ties of the CTAs before this one are in their last counts. A thread takes a
-  // word of 32 slots; slots of more words than threads are gone through in blocks, and then twice.
-  const int2 ties = sum_over(&bins[kDigits - 1][bin & ~1], 0, me);
+  // The first `left` ties stay. A thread takes a word of 32 slots; slots of more words than threads are gone through in blocks, and
+  // then twice.
+  int* const holes_list = p.holes + static_cast<long long>(b) * p.most;
+  int* const late_list = p.late + static_cast<long long>(b) * p.most;
   const int words = (count + 31) / 32, blocks = (words + THREADS - 1) / THREADS;
   int holes_at = 0, late_at = 0, moves = 0;
   for (int pass = 0; pass < 2; ++pass) {
-    int seen = bin & 1 ? ties.y : ties.x, holes = 0, late = 0;
+    int seen = ties_before, holes = 0, late = 0;
     for (int block = 0; block < blocks; ++block) {
-      const int w0 = block * THREADS, here = min(THREADS, words - w0);
+      const int w0 = block * THREADS, here = min(THREADS, words - w0), holes_before = holes_at + holes, late_before = late_at + late;
       if (pass == 0 || blocks > 1) {
         __syncthreads();
+#pragma unroll 4
         for (int w = warp; w < here; w += kWarps) {
           const int i = 32 * (w0 + w) + lane;
           const uint32_t r = i < count ? rank_at(i) : 0u;
-          const uint32_t above = __ballot_sync(0xffffffffu, i < count && r > bits), tie = __ballot_sync(0xffffffffu, i < count && r == bits);
+          const uint32_t above = __ballot_sync(0xffffffffu, i < count && r > lowest), tie = __ballot_sync(0xffffffffu, i < count && r == lowest);
           if (lane == 0) {
             above_words[w] = above;
             tie_words[w] = tie;
           }
         }
         __syncthreads();
+        uint32_t stays = tid < here ? tie_words[tid] : 0u;
+        if (left < ties) {  // the first of the word that stay: those below its (left - rank)-th
+          int all;
+          const int in_word = __popc(stays), rank = seen + threads_before<THREADS>(in_word, scratch, &all), stay = max(0, min(in_word, left - rank));
+          if (stay < in_word) stays = stay == 0 ? 0u : stays & ((2u << __fns(stays, 0, stay)) - 1u);
+          seen += all;
+        }
+        const uint32_t kept = stays | (tid < here ? above_words[tid] : 0u);
+        const int slot = begin + 32 * (w0 + tid), in_run = count - 32 * (w0 + tid);
+        const uint32_t valid = in_run >= 32 ? 0xffffffffu : in_run > 0 ? (1u << in_run) - 1u : 0u;
+        const uint32_t low = budget - slot >= 32 ? 0xffffffffu : budget > slot ? (1u << (budget - slot)) - 1u : 0u;  // below the budget
+        const uint32_t hole = ~kept & valid & low, moved = kept & ~low;
+        int both;  // 16 bits each: at most 32768 slots in a block
+        before_words[tid] = static_cast<uint32_t>(threads_before<THREADS>(__popc(moved) << 16 | __popc(hole), scratch, &both));
+        above_words[tid] = hole;
+        tie_words[tid] = moved;
+        holes += both & 0xffff;
+        late += static_cast<int>(static_cast<uint32_t>(both) >> 16);
       }
-      const uint32_t tie = tid < here ? tie_words[tid] : 0u;
-      int all_ties, all_holes, all_late;
-      const int tie_rank = seen + threads_before<THREADS>(__popc(tie), scratch, &all_ties);
-      // the first ties of the word that stay: those below its (left - tie_rank)-th
-      uint32_t kept = tid < here ? above_words[tid] : 0u;
-      const int stay = max(0, min(__popc(tie), left - tie_rank));
-      kept |= stay == __popc(tie) ? tie : stay == 0 ? 0u : tie & ((2u << __fns(tie, 0, stay)) - 1u);
-      const int slot = begin + 32 * (w0 + tid), in_run = count - 32 * (w0 + tid);
-      const uint32_t valid = in_run >= 32 ? 0xffffffffu : in_run > 0 ? (1u << in_run) - 1u : 0u;
-      const uint32_t low = budget - slot >= 32 ? 0xffffffffu : budget > slot ? (1u << (budget - slot)) - 1u : 0u;  // below the budget
-      uint32_t hole = ~kept & valid & low, moved = kept & ~low;
-      int h = holes_at + holes + threads_before<THREADS>(__popc(hole), scratch, &all_holes);
-      int l = late_at + late + threads_before<THREADS>(__popc(moved), scratch, &all_late);
-      if (pass == 1) {
-        for (; hole != 0; hole &= hole - 1) holes_list[h++] = slot + __ffs(hole) - 1;
-        for (; moved != 0; moved &= moved - 1) late_list[l++] = slot + __ffs(moved) - 1;
+      if (pass == 1) {  // a warp per word, a lane per slot: stores lie together
+        if (blocks > 1) __syncthreads();
+        for (int w = warp; w < here; w += kWarps) {
+          const uint32_t hole = above_words[w], moved = tie_words[w], before = before_words[w], lower = (1u << lane) - 1u;
+          const int slot = begin + 32 * (w0 + w) + lane;
+          const int to = holes_before + static_cast<int>(before & 0xffffu) + __popc(hole & lower);
+          const int of = late_before + static_cast<int>(before >> 16) + __popc(moved & lower);
+          if (p.few) {  // every CTA moves some
+            for (int k = 0; k < cluster; ++k) {
+              if (hole >> lane & 1u) put(&few_to[to], k, static_cast<uint32_t>(slot));
+              if (moved >> lane & 1u) put(&few_of[of], k, static_cast<uint32_t>(slot));
+            }
+          } else {
+            if (hole >> lane & 1u) holes_list[to] = slot;
+            if (moved >> lane & 1u) late_list[of] = slot;
+          }
+        }
       }
-      seen += all_ties;
-      holes += all_holes;
-      late += all_late;
     }
     if (pass == 0) {
       if (tid == 0) {
         totals[0] = holes;
         totals[1] = late;
       }
-      sync();
-      const int2 before = sum_over(totals, 0, me);
-      holes_at = before.x;
-      late_at = before.y;
-      if (me == cluster - 1 && tid == 0) p.moves[b] = holes_at + holes;
-      if (p.few) moves = sum_over(totals, 0, cluster).x;
+      arrive();
+      wait();
+      const int4 sums = sum_over(totals);
+      moves = sums.x;
+      holes_at = sums.z;
+      late_at = sums.w;
+      if (me == 0 && tid == 0 && !p.few) p.moves[b] = moves;
     }
   }
-  sync();  // the lists are complete, and no CTA leaves while another reads its counts
-  for (int i = me * kWarps + warp; i < moves; i += cluster * kWarps) move_row(p, b, i, lane);
+  arrive();
+  wait();  // the lists are complete, and no CTA leaves while another reads its counts
+  if (p.few)
+    for (int i = me * kWarps + warp; i < moves; i += cluster * kWarps) move_row(p, b, few_to[i], few_of[i], lane);
 }
 
 // A warp per moved row: the row, its score and its position.
@@ -1431,8 +1554,10 @@ __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const __grid_c
   pdl_wait();
   pdl_launch_dependents();
   const int b = static_cast<int>(blockIdx.y), warps = static_cast<int>(gridDim.x) * (kMoveThreads / 32), moves = p.moves[b];
-  for (int i = static_cast<int>(blockIdx.x) * (kMoveThreads / 32) + (static_cast<int>(threadIdx.x) >> 5); i < moves; i += warps)
-    move_row(p, b, i, static_cast<int>(threadIdx.x) & 31);
+  for (int i = static_cast<int>(blockIdx.x) * (kMoveThreads / 32) + (static_cast<int>(threadIdx.x) >> 5); i < moves; i += warps) {
+    const long long at = static_cast<long long>(b) * p.most + i;
+    move_row(p, b, p.holes[at], p.late[at], static_cast<int>(threadIdx.x) & 31);
+  }
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -1779,9 +1904,9 @@ int b200_mla_cache_evict(const b200_mla_cache* cache, const float* score, long l
   p.holes = p.moves + cache->batch;
   p.late = p.holes + static_cast<size_t>(cache->batch) * p.most;
   p.vecs = p.cache.d / 8;
-  // CTAs per sequence: 2048 slots each where the batch leaves SMs for it.
+  // CTAs per sequence: 4096 slots each where the batch leaves SMs for it.
   p.cluster = 1;
-  while (p.cluster < kMaxCluster && 2 * p.cluster * cache->batch <= 148 && p.cache.capacity > 2048 * p.cluster) p.cluster *= 2;
+  while (p.cluster < kMaxCluster && 2 * p.cluster * cache->batch <= 148 && p.cache.capacity > 4096 * p.cluster) p.cluster *= 2;
   const int slots = ((p.cache.capacity + p.cluster - 1) / p.cluster + 31) / 32 * 32;
   p.staged = slots < kMaxStaged ? slots : kMaxStaged;
   p.few = p.most <= kFewMoves;
@@ -1789,9 +1914,9 @@ int b200_mla_cache_evict(const b200_mla_cache* cache, const float* score, long l
   static std::atomic<bool> opted[kMaxDevices][2];
   const bool small = slots <= 4096;
   const auto select = small ? evict_select_kernel<256> : evict_select_kernel<1024>;
-  if (device < 0 || !opt_in(select, kMaxStaged * 4, &opted[device][small ? 0 : 1])) return B200_FP8_MM_ERR_DRIVER;
+  if (device < 0 || !opt_in(select, kMaxStaged * 8, &opted[device][small ? 0 : 1])) return B200_FP8_MM_ERR_DRIVER;
   rc = launch_clusters(select, p.cluster, dim3(static_cast<unsigned>(cache->batch * p.cluster)), small ? 256 : 1024,
-                       static_cast<size_t>(p.staged) * 4, stream, p);
+                       static_cast<size_t>(p.staged) * 8, stream, p);
   if (rc != B200_FP8_MM_OK || p.most == 0 || p.few) return rc;
   const int want = (p.most + kMoveThreads / 32 - 1) / (kMoveThreads / 32);
   const int fill = (148 * 8 + cache->batch - 1) / cache->batch;
