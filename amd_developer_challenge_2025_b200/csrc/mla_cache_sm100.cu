@@ -1240,20 +1240,18 @@ __device__ __forceinline__ void move_row(const EvictParams& p, int b, int to, in
 static_assert(kMaxD / 8 <= 96, "move_row holds a row in three pieces a lane");
 
 // A cluster of CTAs per sequence, each with a run of its slots. Finds the budget-th largest rank: the range of the ranks is cut into
-// as many bins as two to a thread (512 or 2048), the bin that holds it again, until the bin is one rank or holds no more of them than
+// 512 bins, the bin that holds it again, until the bin is one rank or holds no more of them than
 // there are threads, which then count for each how many are larger. Then the slots to fill and the slots to move, in order. Scores and
 // positions are read from memory once; from then on ranks and positions lie in shared memory, and the CTAs of a cluster read each
 // other's counts there. What it costs is a chain of barriers, which are dearer the more threads wait: one slot after the other is
 // cheaper up to 4096 slots of a CTA.
 template <int THREADS>
 __global__ void __launch_bounds__(THREADS, 1) evict_select_kernel(const __grid_constant__ EvictParams p) {
-  constexpr int kWarps = THREADS / 32, kBins = 2 * THREADS, kDigitBits = THREADS == 256 ? 9 : 11;
-  // The first cut leaves one bin for the protected rows: 32 bits to 24 (22), then 15 and 6 (11), then none.
-  constexpr int kDigits = THREADS == 256 ? 4 : 3, kAtOnce = THREADS == 256 ? 16 : 8, kFew = THREADS / 4;
-  static_assert(kBins == 1 << kDigitBits && (kDigits - 1) * kDigitBits + kDigitBits - 1 >= 32, "two bins to a thread, cuts down to one rank");
+  constexpr int kWarps = THREADS / 32, kBins = 512, kDigitBits = 9, kScan = kBins / 2, kAtOnce = THREADS == 256 ? 16 : 8, kFew = THREADS / 4;
+  constexpr int kDigits = 4;  // the first cut leaves one bin for the protected rows: 32 bits to 24, then 15, 6, none
   extern __shared__ uint32_t ranks[];
   __shared__ alignas(8) int bins[kDigits][kBins];
-  __shared__ alignas(8) int totals[2];
+  __shared__ int holes_of[kMaxCluster], late_of[kMaxCluster];
   __shared__ uint32_t newest_of[kMaxCluster], lowest_of[kMaxCluster], highest_of[kMaxCluster], few[kFew];
   __shared__ int scratch[kWarps], found[4], equal[3], few_count, few_to[kFewMoves], few_of[kFewMoves];
   // Which of 32 slots lie above the threshold, and on it; then which are to fill, which to move, and how many of both lie before.
@@ -1357,6 +1355,7 @@ __global__ void __launch_bounds__(THREADS, 1) evict_select_kernel(const __grid_c
       }
     }
   }
+  if (tid < 32 && count + tid < min(staged, (count + 31) / 32 * 32)) ranks[count + tid] = 0u;
   newest = __reduce_max_sync(0xffffffffu, newest);
   lowest = __reduce_min_sync(0xffffffffu, lowest);
   highest = __reduce_max_sync(0xffffffffu, highest);
@@ -1390,35 +1389,51 @@ __global__ void __launch_bounds__(THREADS, 1) evict_select_kernel(const __grid_c
     if (i < staged) return ranks[i];
     return position[begin + i] > safe_above ? kProtected : rank_of(score[begin + i]);
   };
+  // f(slot, rank) for the thread's slots, four at a time. (The instructions that 1024 threads issue are what these loops cost.)
+  auto each = [&](auto&& f) {
+    const int near = min(count, staged);
+    int i = tid;
+    for (; i + 3 * THREADS < near; i += 4 * THREADS) {
+      uint32_t r[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) r[k] = ranks[i + k * THREADS];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) f(i + k * THREADS, r[k]);
+    }
+    for (; i < near; i += THREADS) f(i, ranks[i]);
+    for (; i < count; i += THREADS) f(i, rank_at(i));
+  };
   int shift = max(0, 32 - __clz(static_cast<int>(highest - lowest)) - kDigitBits);
   if ((highest - lowest) >> shift > kBins - 2) ++shift;
-  for (int i = tid; i < count; i += THREADS) {
-    uint32_t r;
-    if (i < staged) {
-      r = ranks[i];
-      if (positions[i] > safe_above) ranks[i] = r = kProtected;
-    } else {
-      r = rank_at(i);
-    }
+  each([&](int i, uint32_t r) {
+    if (i < staged && positions[i] > safe_above) ranks[i] = r = kProtected;
     atomicAdd(&bins[0][r == kProtected ? kBins - 1 : (r - lowest) >> shift], 1);
-  }
+  });
   // Of the rows with the rank `lowest`, `left` are kept, of `ties`, of which `ties_before` belong to the CTAs before this one.
   int left = budget, ties = 0, ties_before = 0;
   for (int digit = 0;; ++digit) {
     arrive();
     wait();
-    // Thread t has bins kBins - 1 - 2 t and the one below: counted from the top.
-    const int high = kBins - 1 - 2 * tid;
-    const int4 pair = sum_over(&bins[digit][high - 1]);
-    const int n0 = pair.y, n1 = pair.x;
-    int total;
-    const int above = threads_before<THREADS>(n0 + n1, scratch, &total);
-    if (above < left && left <= above + n0 + n1) {
-      const bool second = left > above + n0;
-      found[0] = high - (second ? 1 : 0);
-      found[1] = above + (second ? n0 : 0);
-      found[2] = second ? n1 : n0;
-      found[3] = second ? pair.z : pair.w;
+    if (tid < kScan) {  // thread t has bins kBins - 1 - 2 t and the one below: counted from the top
+      const int high = kBins - 1 - 2 * tid;
+      const int4 pair = sum_over(&bins[digit][high - 1]);
+      const int n0 = pair.y, n1 = pair.x;
+      int upto = n0 + n1;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int u = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += u;
+      }
+      if (lane == 31) scratch[warp] = upto;
+      asm volatile("bar.sync 1, %0;" ::"n"(kScan) : "memory");
+      const int above = __reduce_add_sync(0xffffffffu, lane < warp ? scratch[lane] : 0) + upto - n0 - n1;
+      if (above < left && left <= above + n0 + n1) {
+        const bool second = left > above + n0;
+        found[0] = high - (second ? 1 : 0);
+        found[1] = above + (second ? n0 : 0);
+        found[2] = second ? n1 : n0;
+        found[3] = second ? pair.z : pair.w;
+      }
     }
     __syncthreads();
     const int bin = found[0];
@@ -1428,14 +1443,27 @@ __global__ void __launch_bounds__(THREADS, 1) evict_select_kernel(const __grid_c
     const bool safe = digit == 0 && bin == kBins - 1;  // more are protected than stay
     lowest = safe ? kProtected : lowest + (static_cast<uint32_t>(bin) << shift);
     if (safe || shift == 0) break;
-    auto inside = [&](uint32_t r) { return r >= lowest && r != kProtected && (r - lowest) >> shift == 0; };
+    const uint32_t span = min(1u << shift, kProtected - lowest);  // (ranks below `lowest` are far above it in the difference)
     if (ties <= kFew) {
-      for (int i = tid; i < count; i += THREADS) {
-        const uint32_t r = rank_at(i);
-        if (!inside(r)) continue;
-        const int to = ties_before + atomicAdd(&few_count, 1);
-        for (int k = 0; k < cluster; ++k) put(&few[to], k, r);
-      }
+      uint32_t hits = 0;  // of up to 32 slots, looked for first: a warp would go through the rest for every slot
+      int at = tid;
+      auto hand_out = [&]() {
+        for (; hits != 0; hits &= hits - 1) {
+          const int to = ties_before + atomicAdd(&few_count, 1);
+          const uint32_t r = rank_at(at + (__ffs(hits) - 1) * THREADS);
+          for (int k = 0; k < cluster; ++k) put(&few[to], k, r);
+        }
+      };
+      int seen = 0;
+      each([&](int i, uint32_t r) {
+        hits |= static_cast<uint32_t>(r - lowest < span) << seen;
+        if (++seen == 32) {
+          hand_out();
+          at = i + THREADS;
+          seen = 0;
+        }
+      });
+      hand_out();
       arrive();
       wait();
       if (tid < ties) {
@@ -1461,12 +1489,10 @@ __global__ void __launch_bounds__(THREADS, 1) evict_select_kernel(const __grid_c
       ties_before = __reduce_add_sync(0xffffffffu, same_before);
       break;
     }
-    const int from = shift;
     shift = max(0, shift - kDigitBits);
-    for (int i = tid; i < count; i += THREADS) {
-      const uint32_t r = rank_at(i);
-      if (r >= lowest && r != kProtected && (r - lowest) >> from == 0) atomicAdd(&bins[digit + 1][(r - lowest) >> shift], 1);
-    }
+    each([&](int, uint32_t r) {
+      if (r - lowest < span) atomicAdd(&bins[digit + 1][(r - lowest) >> shift], 1);
+    });
   }
   // The first `left` ties stay. A thread takes a word of 32 slots; slots of more words than threads are gone through in blocks, and
   // then twice.
@@ -1483,8 +1509,8 @@ __global__ void __launch_bounds__(THREADS, 1) evict_select_kernel(const __grid_c
 #pragma unroll 4
         for (int w = warp; w < here; w += kWarps) {
           const int i = 32 * (w0 + w) + lane;
-          const uint32_t r = i < count ? rank_at(i) : 0u;
-          const uint32_t above = __ballot_sync(0xffffffffu, i < count && r > lowest), tie = __ballot_sync(0xffffffffu, i < count && r == lowest);
+          const uint32_t r = i < staged || i < count ? rank_at(i) : 0u;  // (0, below all ranks, behind the last slot)
+          const uint32_t above = __ballot_sync(0xffffffffu, r > lowest), tie = __ballot_sync(0xffffffffu, r == lowest);
           if (lane == 0) {
             above_words[w] = above;
             tie_words[w] = tie;
@@ -1512,34 +1538,34 @@ __global__ void __launch_bounds__(THREADS, 1) evict_select_kernel(const __grid_c
       }
       if (pass == 1) {  // a warp per word, a lane per slot: stores lie together
         if (blocks > 1) __syncthreads();
+        const uint32_t lower = (1u << lane) - 1u;
         for (int w = warp; w < here; w += kWarps) {
-          const uint32_t hole = above_words[w], moved = tie_words[w], before = before_words[w], lower = (1u << lane) - 1u;
+          const uint32_t hole = above_words[w], moved = tie_words[w], before = before_words[w];
+          if ((hole | moved) == 0) continue;
           const int slot = begin + 32 * (w0 + w) + lane;
           const int to = holes_before + static_cast<int>(before & 0xffffu) + __popc(hole & lower);
           const int of = late_before + static_cast<int>(before >> 16) + __popc(moved & lower);
-          if (p.few) {  // every CTA moves some
-            for (int k = 0; k < cluster; ++k) {
-              if (hole >> lane & 1u) put(&few_to[to], k, static_cast<uint32_t>(slot));
-              if (moved >> lane & 1u) put(&few_of[of], k, static_cast<uint32_t>(slot));
-            }
-          } else {
-            if (hole >> lane & 1u) holes_list[to] = slot;
-            if (moved >> lane & 1u) late_list[of] = slot;
+          const bool fill = hole >> lane & 1u, move = moved >> lane & 1u;
+          if (!p.few) {
+            if (fill) holes_list[to] = slot;
+            if (move) late_list[of] = slot;
+          } else if (fill || move) {  // every CTA moves some
+            for (int k = 0; k < cluster; ++k) put(fill ? &few_to[to] : &few_of[of], k, static_cast<uint32_t>(slot));
           }
         }
       }
     }
     if (pass == 0) {
-      if (tid == 0) {
-        totals[0] = holes;
-        totals[1] = late;
+      if (tid < cluster) {
+        put(&holes_of[me], tid, static_cast<uint32_t>(holes));
+        put(&late_of[me], tid, static_cast<uint32_t>(late));
       }
       arrive();
       wait();
-      const int4 sums = sum_over(totals);
-      moves = sums.x;
-      holes_at = sums.z;
-      late_at = sums.w;
+      for (int k = 0; k < cluster; ++k) {
+        moves += holes_of[k];
+        if (k < me) holes_at += holes_of[k], late_at += late_of[k];
+      }
       if (me == 0 && tid == 0 && !p.few) p.moves[b] = moves;
     }
   }
