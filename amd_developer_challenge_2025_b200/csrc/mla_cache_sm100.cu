@@ -311,6 +311,14 @@ __device__ __forceinline__ void tma_load_5d(uint32_t dst, const CUtensorMap* map
       "l"(map), "r"(0), "r"(c1), "r"(c2), "r"(c3), "r"(c4), "r"(bar)
       : "memory");
 }
+// The same rows on their way to L2 only.
+__device__ __forceinline__ void tma_prefetch_5d(const CUtensorMap* map, int c3, int c4) {
+  asm volatile(
+      "{\n\t.reg .pred leader;\n\t"
+      "elect.sync _|leader, 0xffffffff;\n\t"
+      "@leader cp.async.bulk.prefetch.tensor.5d.L2.global.tile [%0, {%1, %1, %1, %2, %3}];\n\t}" ::"l"(map), "r"(0), "r"(c3), "r"(c4)
+      : "memory");
+}
 __device__ __forceinline__ void tcgen05_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tcgen05_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
@@ -660,6 +668,11 @@ attend_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__
         if (++stage == stages) stage = 0, lap ^= 1, first_lap = false;
         if (tile == 0 && !(ok = copy_queries(segment, walk.b))) break;
         place(walk.t + tile + 1);  // on its way during the waits
+        if (HT == 64 && !first_lap && tile + 1 < count)
+          for (int k = 0; k < pieces; ++k) {
+            const int of = __shfl_sync(0xffffffffu, page, k), at = __shfl_sync(0xffffffffu, slot, k) >> 3;
+            if (of < c.pages) tma_prefetch_5d(&row_map, at, of);
+          }
       }
       ++segment;
     }
