@@ -143,8 +143,9 @@ __device__ __forceinline__ void rotate_rows(const AppendParams& p, const T* src,
   }
 }
 
-// Writes the new rows (the first CTA of a sequence) and rotates the queries (the others, kAppendHeads heads each).
-// Memory-bound where there are many heads: every element of q once in and once out. 128 sequences x 128 heads.
+// Writes the new rows (the first CTA of a sequence) and rotates the queries (the others, kAppendHeads heads each): every element of q
+// once in and once out. 128 sequences x 128 heads: 10.0 us, 38 MB at 3.8 TB/s; a CTA is a chain of waits (position, angles in 64 bits,
+// loads), so the unrotated elements' loads go first (11.7 us with all after the angles). One sequence of 16 heads: 3.9 us, the launch.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_constant__ AppendParams p) {
   __shared__ float2 cs[kMaxPairs];
@@ -457,7 +458,8 @@ struct Walk {
   int slot;                // where a part of it is left
   long long begin, from, to;
 
-  __device__ __forceinline__ Walk(const AttendShared& sh) : b(sh.first_seq - 1), t(0), rows(0), count(0), slot(0), begin(sh.first_begin), from(sh.share), to(sh.share_end) {}
+  __device__ __forceinline__ Walk(const AttendShared& sh)
+      : b(sh.first_seq - 1), t(0), rows(0), count(0), slot(0), begin(sh.first_begin), from(sh.share), to(sh.share_end) {}
   __device__ __forceinline__ bool next(const AttendParams& p) {
     while (begin < to) {
       ++b;
@@ -484,17 +486,19 @@ struct Walk {
 // from chunk to chunk for both operands, and one copy brings all chunks of as many rows as lie together in a page, up to the tile.
 //
 // What bounds it: up to 32 heads, memory (6.2 TB/s while it runs); 64 heads, how long a tile stays. From its copy's way through memory
-// (2200 to 3000 clocks) over the first product (1170), the softmax (1300) and the second product (740) to the next copy it takes 6800, and
-// two tiles of 64 rows are all that fits next to Q: 3400 clocks a tile, where the tensor core needs 1900 and, for 128 heads, memory 1600.
-// Tiles of 32 rows, four of them in flight, were slower (162 against 142 us, 64 sequences of 4096 rows with 128 heads): an MMA takes 27
-// clocks to issue however small it is. So were units of 128 elements as the ring's grain, and halves of a tile freed one by one.
+// (2200 to 3000 clocks) over the first product (1170), the softmax (1300) and the second product (740) to the next copy it took 6800,
+// and two tiles of 64 rows are all that fits next to Q: 3400 clocks a tile, where the tensor core needs 1900 and, for 128 heads, memory
+// 1600. The next tile is therefore fetched to L2 while the ring is full (one sequence of 65536 rows, 128 heads: 45.8 -> 43.5 us).
+// Slower were: tiles of 32 rows, four of them in flight (162 against 142 us, 64 sequences of 4096 rows with 128 heads: an MMA takes 27
+// clocks to issue however small it is); units of 128 elements as the ring's grain; halves of a tile freed one by one; the second product
+// issued between chunks of the next tile's first (153 against 142 us: the issuing loop loses its pace).
 //
 // One CTA per SM and worker: warp 4 copies (with warps 6 and 7, 16 bytes a lane, where pages are not whole groups of 8 rows: TMA would
 // have to bring them in copies of 128 to 512 bytes, 579 against 99 us for pages of one row), warp 5 issues the products, warps 0 to 3 do
 // the softmax (S comes as 16 x 256-bit fragments, 4 threads to a head) and the epilogue. S is double buffered; the next tile's first
-// product runs under this tile's softmax. The running maximum is replaced only when a logit exceeds it by 8 (in base 2): the
-// weights stay below 2^8 in bf16 and 2^15 in fp16, and rescaling the accumulators is rare. Sums are kept in fp32, weights are rounded to the cache's type
-// for the second product, as matrix operands have to be.
+// product runs under this tile's softmax. The running maximum is replaced only when a logit exceeds it by 8 (in base 2): the weights
+// stay below 2^8 in bf16 and 2^15 in fp16, and rescaling the accumulators is rare. Sums are kept in fp32, weights are rounded to the
+// cache's type for the second product, as matrix operands have to be.
 template <typename T, int HT>
 __global__ void __launch_bounds__(kAttendThreads, 1)
 attend_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap row_map, const __grid_constant__ AttendParams p) {
@@ -1053,7 +1057,9 @@ attend_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__
 // Joins the parts of split sequences, in the order of their rows, and writes what sequences without rows get: a CTA per head and
 // sequence, GROUPS groups of a thread for every 4 value elements that share the parts. It reads what the attention left in L2; what
 // it costs is a chain of loads (where the sequence's parts are, their statistics, the parts), so every thread looks up all of it
-// for itself and only the groups' sums go through shared memory.
+// for itself and only the groups' sums go through shared memory. Without it, where no sequence can be split, 128
+// sequences of 60 rows with 32 heads take 11.2 us instead of 16.2.
+// The parts of one sequence of 65536 rows with 128 heads are 19 MB: 11.7 us by itself from cold caches.
 template <typename T, int GROUPS>
 __global__ void __launch_bounds__(128 * GROUPS) attend_join_kernel(const __grid_constant__ AttendParams p, int tile_heads) {
   __shared__ float4 sums[GROUPS][128];
@@ -1144,7 +1150,9 @@ __global__ void __launch_bounds__(128 * GROUPS) attend_join_kernel(const __grid_
   }
 }
 
-// score_out = score + the weights of all heads, from the logits that the attention left: a CTA per tile, a group of threads for every fourth head.
+// score_out = score + the weights of all heads, from the logits that the attention left: a CTA per tile, a group of threads for every
+// fourth head. It needs every head's sum over the whole sequence, so it follows the join. (One kernel for both, in which each tile's CTA
+// takes the sums from the parts itself, was slower: 28 against 18 us for 8 sequences of 2049 rows, 69 against 63 for 32 with 128 heads.)
 constexpr int kScoreGroups = 4;
 
 template <int kTile>
@@ -1252,15 +1260,20 @@ __device__ __forceinline__ void move_row(const EvictParams& p, int b, int to, in
 }
 static_assert(kMaxD / 8 <= 96, "move_row holds a row in three pieces a lane");
 
-// A cluster of CTAs per sequence, each with a run of its slots. Finds the budget-th largest rank: the range of the ranks is cut into
-// 512 bins, the bin that holds it again, until the bin is one rank or holds no more of them than
-// there are threads, which then count for each how many are larger. Then the slots to fill and the slots to move, in order. Scores and
-// positions are read from memory once; from then on ranks and positions lie in shared memory, and the CTAs of a cluster read each
-// other's counts there. What it costs is a chain of barriers, which are dearer the more threads wait: one slot after the other is
-// cheaper up to 4096 slots of a CTA.
+// A cluster of CTAs per sequence, each with a run of its slots. Finds the budget-th largest rank: the range of the ranks is cut into 512
+// bins, the bin that holds it again, until the bin is one rank or holds so few that they can be compared with each other. Then the slots
+// to fill and the slots to move, in order. Scores and positions are read from memory once; from then on ranks and positions lie in
+// shared memory, and the CTAs of a cluster read each other's counts there.
+//
+// What it costs is neither bytes nor operations but a chain: some fifteen barriers (dearer between CTAs, and the more threads wait), the
+// loads behind them, and code that is gone through once and waits for its instructions longer than for anything else. 64 sequences of
+// 2049 slots 7.9 us, 8 of 16384 17.5, one of 131072 26.4 (14.4, 24.5 and 36 with fixed digits of the rank and both arrays read twice).
+// 512 threads up to 8192 slots of a CTA, 1024 above: 7.9, 17.5 and 29.1 us with 512, 8.4, 18.6 and 26.4 with 1024 (with 256, one sequence
+// of 131072 took 45). Up to 128 ranks are compared with each other: with 32, 64 sequences of 2049 slots took 8.7 us, with 256 16 of 5000
+// 18.9 instead of 16.8. Loops rolled to save instructions waited for shared memory instead: 9.2, 19.7 and 30.5.
 template <int THREADS>
 __global__ void __launch_bounds__(THREADS, 1) evict_select_kernel(const __grid_constant__ EvictParams p) {
-  constexpr int kWarps = THREADS / 32, kBins = 512, kDigitBits = 9, kScan = kBins / 2, kAtOnce = THREADS == 256 ? 16 : 8, kFew = THREADS / 4;
+  constexpr int kWarps = THREADS / 32, kBins = 512, kDigitBits = 9, kScan = kBins / 2, kAtOnce = 8, kFew = 128;
   constexpr int kDigits = 4;  // the first cut leaves one bin for the protected rows: 32 bits to 24, then 15, 6, none
   extern __shared__ uint32_t ranks[];
   __shared__ alignas(8) int bins[kDigits][kBins];
@@ -1588,7 +1601,8 @@ __global__ void __launch_bounds__(THREADS, 1) evict_select_kernel(const __grid_c
     for (int i = me * kWarps + warp; i < moves; i += cluster * kWarps) move_row(p, b, few_to[i], few_of[i], lane);
 }
 
-// A warp per moved row: the row, its score and its position.
+// A warp per moved row: the row, its score and its position. 8 sequences that move up to 2048 rows of 1152 bytes each: 8.4 us by itself
+// from cold caches, some 30 MB.
 __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const __grid_constant__ EvictParams p) {
   pdl_wait();
   pdl_launch_dependents();
@@ -1943,7 +1957,8 @@ int b200_mla_cache_evict(const b200_mla_cache* cache, const float* score, long l
   p.holes = p.moves + cache->batch;
   p.late = p.holes + static_cast<size_t>(cache->batch) * p.most;
   p.vecs = p.cache.d / 8;
-  // CTAs per sequence: 4096 slots each where the batch leaves SMs for it.
+  // CTAs per sequence: 4096 slots each where the batch leaves SMs for it. (64 sequences of 2049 slots with 1024 threads: 8.4 us with one
+  // CTA each, 10.7 with two. One of 16000: 15.6 us with four, 15.3 with eight, 18.3 with two.)
   p.cluster = 1;
   while (p.cluster < kMaxCluster && 2 * p.cluster * cache->batch <= 148 && p.cache.capacity > 4096 * p.cluster) p.cluster *= 2;
   const int slots = ((p.cache.capacity + p.cluster - 1) / p.cluster + 31) / 32 * 32;
@@ -1951,10 +1966,10 @@ int b200_mla_cache_evict(const b200_mla_cache* cache, const float* score, long l
   p.few = p.most <= kFewMoves;
   const int device = current_device();
   static std::atomic<bool> opted[kMaxDevices][2];
-  const bool small = slots <= 4096;
-  const auto select = small ? evict_select_kernel<256> : evict_select_kernel<1024>;
-  if (device < 0 || !opt_in(select, kMaxStaged * 8, &opted[device][small ? 0 : 1])) return B200_FP8_MM_ERR_DRIVER;
-  rc = launch_clusters(select, p.cluster, dim3(static_cast<unsigned>(cache->batch * p.cluster)), small ? 256 : 1024,
+  const bool few_slots = slots <= 8192;
+  const auto select = few_slots ? evict_select_kernel<512> : evict_select_kernel<1024>;
+  if (device < 0 || !opt_in(select, kMaxStaged * 8, &opted[device][few_slots])) return B200_FP8_MM_ERR_DRIVER;
+  rc = launch_clusters(select, p.cluster, dim3(static_cast<unsigned>(cache->batch * p.cluster)), few_slots ? 512 : 1024,
                        static_cast<size_t>(p.staged) * 8, stream, p);
   if (rc != B200_FP8_MM_OK || p.most == 0 || p.few) return rc;
   const int want = (p.most + kMoveThreads / 32 - 1) / (kMoveThreads / 32);
