@@ -441,7 +441,7 @@ __device__ __forceinline__ bool softmax_any(bool mine) {
 struct alignas(8) AttendShared {
   uint64_t full[kMaxStages], pv_done[kMaxStages];  // a tile is there; the second product is done with it
   uint64_t s_full[2], s_free[2], p_full, q_full, q_empty, o_free, drained;
-  float factor[2][64];  // by which a head's accumulators are multiplied when its maximum is replaced; tiles take turns
+  float factor[64];     // by which a head's accumulators are multiplied when its maximum is replaced
   float2 stat[64];      // maximum and sum of weights of a head
   float inverse[64];    // 1 / sum
   long long sums[kAttendThreads / 32];
@@ -883,8 +883,29 @@ attend_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__
         if (active) tmem_ld_16x64(tmem + lanes + kTmemLogits + (i & 1) * 64, x);
         tcgen05_fence_before();
         const int left = walk.rows - (walk.t + tile) * kTile;  // rows that exist from this tile on
-        float t0 = -INFINITY, t1 = -INFINITY;
+        float t0 = -INFINITY, t1 = -INFINITY, sum0 = 0.f, sum1 = 0.f;
+        uint32_t w[16];
         bool up = false;
+        auto head_max = [&]() {  // over the four threads of a head
+#pragma unroll
+          for (int o = 1; o < 4; o <<= 1) {
+            t0 = fmaxf(t0, __shfl_xor_sync(0xffffffffu, t0, o));
+            t1 = fmaxf(t1, __shfl_xor_sync(0xffffffffu, t1, o));
+          }
+        };
+        auto weigh = [&]() {
+          const float z0 = m0 == -INFINITY ? 0.f : m0, z1 = m1 == -INFINITY ? 0.f : m1;
+          sum0 = sum1 = 0.f;
+#pragma unroll
+          for (int n = 0; n < kTile / 8; ++n) {
+            const float a = exp2_fast(__uint_as_float(x[4 * n]) - z0), b = exp2_fast(__uint_as_float(x[4 * n + 1]) - z0);
+            const float e = exp2_fast(__uint_as_float(x[4 * n + 2]) - z1), f = exp2_fast(__uint_as_float(x[4 * n + 3]) - z1);
+            sum0 += a + b;
+            sum1 += e + f;
+            w[2 * n] = pack2(a, b, T());
+            w[2 * n + 1] = pack2(e, f, T());
+          }
+        };
         if (active) {
           if (left >= kTile) {
 #pragma unroll
@@ -910,50 +931,44 @@ attend_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__
                 *reinterpret_cast<uint2*>(to + row1 * kTile + 8 * n) = make_uint2(x[4 * n + 2], x[4 * n + 3]);
             }
           }
-#pragma unroll
-          for (int o = 1; o < 4; o <<= 1) {
-            t0 = fmaxf(t0, __shfl_xor_sync(0xffffffffu, t0, o));
-            t1 = fmaxf(t1, __shfl_xor_sync(0xffffffffu, t1, o));
-          }
-          float f0 = 1.f, f1 = 1.f;
+          // Against the maximum that is; the tile's own matters only where it is far above.
           if (tile == 0) {
+            head_max();
             m0 = t0 - kTopWeight<T>;
             m1 = t1 - kTopWeight<T>;
-          } else {
-            t0 -= kTopWeight<T>;
-            t1 -= kTopWeight<T>;
-            const bool up0 = t0 > m0 + kRescaleAbove, up1 = t1 > m1 + kRescaleAbove;
-            up = up0 || up1;
-            if (up0) f0 = exp2_fast(m0 - t0), m0 = t0;
-            if (up1) f1 = exp2_fast(m1 - t1), m1 = t1;
-            l0 *= f0;
-            l1 *= f1;
           }
-          if (lane % 4 == 0) {
-            sh.factor[i & 1][row0] = f0;
-            sh.factor[i & 1][row1] = f1;
-          }
-          const float z0 = m0 == -INFINITY ? 0.f : m0, z1 = m1 == -INFINITY ? 0.f : m1;
-#pragma unroll
-          for (int n = 0; n < kTile / 8; ++n) {
-            const float a = exp2_fast(__uint_as_float(x[4 * n]) - z0), b = exp2_fast(__uint_as_float(x[4 * n + 1]) - z0);
-            const float e = exp2_fast(__uint_as_float(x[4 * n + 2]) - z1), f = exp2_fast(__uint_as_float(x[4 * n + 3]) - z1);
-            l0 += a + b;
-            l1 += e + f;
-            x[2 * n] = pack2(a, b, T());
-            x[2 * n + 1] = pack2(e, f, T());
-          }
+          weigh();
+          up = t0 > m0 + kRescaleAbove + kTopWeight<T> || t1 > m1 + kRescaleAbove + kTopWeight<T>;
         }
+        // The weights before are read, and the accumulators at rest, once the second product of the tile before is over. (Looked at
+        // before the vote, which takes as long.)
+        const bool over = i == 0 || mbar_test(smem_u32(&sh.pv_done[before.stage]), before.lap);
         const bool rescale = tile > 0 && softmax_any(up);
-        // The weights before are read, and the accumulators at rest, once the second product of the tile before is over.
-        if (i > 0) wait(&sh.pv_done[before.stage], before.lap, kAtPvDone);
+        if (rescale && active) {
+          const float from0 = m0, from1 = m1;
+          head_max();
+          float f0 = 1.f, f1 = 1.f;
+          if (t0 - kTopWeight<T> > m0 + kRescaleAbove) m0 = t0 - kTopWeight<T>, f0 = exp2_fast(from0 - m0);
+          if (t1 - kTopWeight<T> > m1 + kRescaleAbove) m1 = t1 - kTopWeight<T>, f1 = exp2_fast(from1 - m1);
+          l0 *= f0;
+          l1 *= f1;
+          if (lane % 4 == 0) {
+            sh.factor[row0] = f0;
+            sh.factor[row1] = f1;
+          }
+          weigh();
+        }
+        l0 += sum0;
+        l1 += sum1;
+        if (!over) wait(&sh.pv_done[before.stage], before.lap, kAtPvDone);
         if (rescale) {
+          softmax_sync();  // (the factors)
           tcgen05_fence_after();
           for (int col = 0; col < v_units * HT; col += 16) {
             uint32_t o[16];
             tmem_ld_32x16(tmem + lanes + col, o);
 #pragma unroll
-            for (int n = 0; n < 16; ++n) o[n] = __float_as_uint(__uint_as_float(o[n]) * sh.factor[i & 1][col % HT + n]);
+            for (int n = 0; n < 16; ++n) o[n] = __float_as_uint(__uint_as_float(o[n]) * sh.factor[col % HT + n]);
             tmem_st_32x16(tmem + lanes + col, o);
           }
           asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
@@ -965,8 +980,8 @@ attend_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__
 #pragma unroll
           for (int n = 0; n < kTile / 8; ++n) {
             const int piece = 16 * (n ^ (lane / 4));
-            *reinterpret_cast<uint32_t*>(to + row0 * kRowBytes + piece) = x[2 * n];
-            *reinterpret_cast<uint32_t*>(to + row1 * kRowBytes + piece) = x[2 * n + 1];
+            *reinterpret_cast<uint32_t*>(to + row0 * kRowBytes + piece) = w[2 * n];
+            *reinterpret_cast<uint32_t*>(to + row1 * kRowBytes + piece) = w[2 * n + 1];
           }
         }
         if (left < kTile) {
