@@ -1069,27 +1069,33 @@ attend_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__
   }
 }
 
-// Joins the parts of split sequences, in the order of their rows, and writes what sequences without rows get: a CTA per head and
-// sequence, GROUPS groups of a thread for every 4 value elements that share the parts. It reads what the attention left in L2; what
-// it costs is a chain of loads (where the sequence's parts are, their statistics, the parts), so every thread looks up all of it
-// for itself and only the groups' sums go through shared memory. Without it, where no sequence can be split, 128
-// sequences of 60 rows with 32 heads take 11.2 us instead of 16.2.
-// The parts of one sequence of 65536 rows with 128 heads are 19 MB: 11.7 us by itself from cold caches.
+// Heads of a CTA of the join: two where sequences have few parts, whose statistics and values are all on their way together. (64 ragged
+// sequences, 128 heads, in a row: 126.9 us with one, 122.4 with two, 127.6 with four.)
+__host__ __device__ constexpr int join_heads(int groups) { return groups == 1 ? 2 : 1; }
+
+// Joins the parts of split sequences, in the order of their rows, and writes what sequences without rows get: a CTA per head (or
+// two) and sequence, GROUPS groups of a thread for every 4 value elements that share the parts. It reads what the attention left in L2;
+// what it costs is a chain of loads (where the sequence's parts are, their statistics, the parts), so every thread looks up all of it
+// for itself and only the groups' sums go through shared memory. Without it, where no sequence can be split, 128 sequences of 60 rows
+// with 32 heads take 11.2 us instead of 16.2. The parts of one sequence of 65536 rows with 128 heads are 19 MB: 11.7 us by itself from
+// cold caches.
 template <typename T, int GROUPS>
 __global__ void __launch_bounds__(128 * GROUPS) attend_join_kernel(const __grid_constant__ AttendParams p, int tile_heads) {
+  constexpr int kHeads = join_heads(GROUPS), kAhead = 3;  // parts whose values are on their way along with the statistics
   __shared__ float4 sums[GROUPS][128];
   pdl_wait();
   pdl_launch_dependents();
-  const int h = static_cast<int>(blockIdx.x), b = static_cast<int>(blockIdx.y), tid = static_cast<int>(threadIdx.x);
+  const int h0 = static_cast<int>(blockIdx.x) * kHeads, heads = min(kHeads, p.heads - h0), b = static_cast<int>(blockIdx.y);
   const long long places = p.begins[p.batch], begin = p.begins[b], end = p.begins[b + 1];
-  const int dv = p.cache.dv, group = tid >> 7, e = tid & 127, lane = tid & 31;
-  T* const out = static_cast<T*>(p.out) + b * p.out_sb + h * p.out_sh;
-  const long long at = static_cast<long long>(b) * p.heads + h;
+  const int tid = static_cast<int>(threadIdx.x), dv = p.cache.dv, group = tid >> 7, e = tid & 127, lane = tid & 31;
+  T* const out = static_cast<T*>(p.out) + b * p.out_sb + h0 * p.out_sh;
+  const long long at = static_cast<long long>(b) * p.heads + h0;
   if (begin == end) {
-    for (int i = tid; i < dv; i += 128 * GROUPS) from_float(0.f, out + i);
-    if (tid == 0) {
-      p.lse2[at] = -INFINITY;
-      if (p.lse != nullptr) p.lse[at] = -INFINITY;
+    for (int n = 0; n < heads; ++n)
+      for (int i = tid; i < dv; i += 128 * GROUPS) from_float(0.f, out + n * p.out_sh + i);
+    if (tid < heads) {
+      p.lse2[at + tid] = -INFINITY;
+      if (p.lse != nullptr) p.lse[at + tid] = -INFINITY;
     }
     return;
   }
@@ -1098,70 +1104,80 @@ __global__ void __launch_bounds__(128 * GROUPS) attend_join_kernel(const __grid_
   const int g0 = cache_walk::worker_of(places, workers, cache_walk::first_place(begin, tiles, p.extra));
   const int parts = cache_walk::worker_of(places, workers, cache_walk::last_place(begin, tiles, p.extra)) - g0 + 1;
   if (parts == 1) return;  // written by its worker
-  const int head_tile = h / tile_heads, in_tile = h - head_tile * tile_heads;
+  const int head_tile = h0 / tile_heads, in_tile = h0 - head_tile * tile_heads;
   // Only the first part can lie behind another sequence's in its worker's share.
   const int slot0 = cache_walk::part_slot(cache_walk::share_begin(places, workers, g0), begin);
   auto part_of = [&](int i) { return (static_cast<long long>(g0 + i) * p.head_tiles + head_tile) * 2 + (i == 0 ? slot0 : 0); };
-  auto stat_of = [&](int i) { return p.part_stat[part_of(i) * tile_heads + in_tile]; };
-  auto value_of = [&](int i) {
-    return *reinterpret_cast<const float4*>(p.part_out + ((part_of(i) * (dv / 128) + e / 32) * tile_heads + in_tile) * 128 + 4 * (e % 32));
+  auto stat_of = [&](int n, int i) { return p.part_stat[part_of(i) * tile_heads + in_tile + n]; };
+  auto value_of = [&](int n, int i) {
+    return *reinterpret_cast<const float4*>(p.part_out + ((part_of(i) * (dv / 128) + e / 32) * tile_heads + in_tile + n) * 128 + 4 * (e % 32));
   };
-  constexpr int kAhead = 4;  // parts whose values are on their way along with the statistics
-  float4 ahead[kAhead];
+  // (A head tile has room for heads that do not exist; what is read there is not used.)
+  float2 stat[kHeads];
+  float4 ahead[kHeads][kAhead];
+#pragma unroll
+  for (int n = 0; n < kHeads; ++n) stat[n] = lane < parts ? stat_of(n, lane) : make_float2(-INFINITY, 0.f);
 #pragma unroll
   for (int k = 0; k < kAhead; ++k)
-    if (group + k * GROUPS < parts && 4 * e < dv) ahead[k] = value_of(group + k * GROUPS);
-  float top = -INFINITY;
-  for (int i = lane; i < parts; i += 32) top = fmaxf(top, stat_of(i).x);
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  const float base = top == -INFINITY ? 0.f : top;
-  float total = 0.f;
-  for (int i = lane; i < parts; i += 32) {
-    const float2 s = stat_of(i);
-    total += s.y * exp2_fast(s.x - base);
-  }
+    for (int n = 0; n < kHeads; ++n)
+      if (group + k * GROUPS < parts && 4 * e < dv) ahead[n][k] = value_of(n, group + k * GROUPS);
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-  float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-  auto add = [&](int i, const float4& v) {
-    const float w = exp2_fast(stat_of(i).x - base);
-    sum.x += w * v.x;
-    sum.y += w * v.y;
-    sum.z += w * v.z;
-    sum.w += w * v.w;
-  };
-  if (4 * e < dv) {
+  for (int n = 0; n < kHeads; ++n) {
+    float top = stat[n].x;
+    for (int i = lane + 32; i < parts; i += 32) top = fmaxf(top, stat_of(n, i).x);
 #pragma unroll
-    for (int k = 0; k < kAhead; ++k)
-      if (group + k * GROUPS < parts) add(group + k * GROUPS, ahead[k]);
-#pragma unroll 4
-    for (int i = group + kAhead * GROUPS; i < parts; i += GROUPS) add(i, value_of(i));
-  }
-  if constexpr (GROUPS > 1) {
-    sums[group][e] = sum;
-    __syncthreads();
-    if (group > 0) return;
-#pragma unroll
-    for (int k = 1; k < GROUPS; ++k) {
-      const float4 v = sums[k][e];
-      sum.x += v.x;
-      sum.y += v.y;
-      sum.z += v.z;
-      sum.w += v.w;
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    const float base = top == -INFINITY ? 0.f : top, mine = exp2_fast(stat[n].x - base);
+    float total = lane < parts ? stat[n].y * mine : 0.f;
+    for (int i = lane + 32; i < parts; i += 32) {
+      const float2 s = stat_of(n, i);
+      total += s.y * exp2_fast(s.x - base);
     }
-  }
-  if (4 * e < dv) {
-    const float inverse = 1.f / total;
-    from_float(sum.x * inverse, out + 4 * e);
-    from_float(sum.y * inverse, out + 4 * e + 1);
-    from_float(sum.z * inverse, out + 4 * e + 2);
-    from_float(sum.w * inverse, out + 4 * e + 3);
-  }
-  if (tid == 0) {
-    const float lse2 = base + log2f(total);
-    p.lse2[at] = lse2;
-    if (p.lse != nullptr) p.lse[at] = lse2 * kLn2;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+    auto add = [&](int i, const float4& v) {  // (i is the same for the warp)
+      const float w = i < 32 ? __shfl_sync(0xffffffffu, mine, i) : exp2_fast(stat_of(n, i).x - base);
+      sum.x += w * v.x;
+      sum.y += w * v.y;
+      sum.z += w * v.z;
+      sum.w += w * v.w;
+    };
+    if (4 * e < dv) {  // (whole warps: dv is a multiple of 128)
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k)
+        if (group + k * GROUPS < parts) add(group + k * GROUPS, ahead[n][k]);
+#pragma unroll 4
+      for (int i = group + kAhead * GROUPS; i < parts; i += GROUPS) add(i, value_of(n, i));
+    }
+    if constexpr (GROUPS > 1) {
+      sums[group][e] = sum;
+      __syncthreads();
+      if (group > 0) return;
+#pragma unroll
+      for (int k = 1; k < GROUPS; ++k) {
+        const float4 v = sums[k][e];
+        sum.x += v.x;
+        sum.y += v.y;
+        sum.z += v.z;
+        sum.w += v.w;
+      }
+    }
+    if (n >= heads) return;
+    if (4 * e < dv) {
+      const float inverse = 1.f / total;
+      T* const to = out + n * p.out_sh + 4 * e;
+      from_float(sum.x * inverse, to);
+      from_float(sum.y * inverse, to + 1);
+      from_float(sum.z * inverse, to + 2);
+      from_float(sum.w * inverse, to + 3);
+    }
+    if (tid == 0) {
+      const float lse2 = base + log2f(total);
+      p.lse2[at + n] = lse2;
+      if (p.lse != nullptr) p.lse[at + n] = lse2 * kLn2;
+    }
   }
 }
 
@@ -1926,13 +1942,15 @@ int b200_mla_cache_attend(const b200_mla_cache* cache, const void* q, long long 
   rc = launch_pdl(fn, dim3(static_cast<unsigned>(p.workers) * p.head_tiles), kAttendThreads, smem, stream, q_map, row_map, p);
   if (rc != B200_FP8_MM_OK) return rc;
   // Eight groups where a sequence has eight parts and more on average, one where most have one or two.
-  const dim3 joins(static_cast<unsigned>(heads), static_cast<unsigned>(cache->batch));
+  auto joins = [&](int groups) {
+    return dim3(static_cast<unsigned>((heads + join_heads(groups) - 1) / join_heads(groups)), static_cast<unsigned>(cache->batch));
+  };
   if (!p.joined)
     rc = B200_FP8_MM_OK;
   else if (p.workers / cache->batch >= 8)
-    rc = launch_pdl(bf16 ? attend_join_kernel<__nv_bfloat16, 8> : attend_join_kernel<__half, 8>, joins, 1024, 0, stream, p, ht);
+    rc = launch_pdl(bf16 ? attend_join_kernel<__nv_bfloat16, 8> : attend_join_kernel<__half, 8>, joins(8), 1024, 0, stream, p, ht);
   else
-    rc = launch_pdl(bf16 ? attend_join_kernel<__nv_bfloat16, 1> : attend_join_kernel<__half, 1>, joins, 128, 0, stream, p, ht);
+    rc = launch_pdl(bf16 ? attend_join_kernel<__nv_bfloat16, 1> : attend_join_kernel<__half, 1>, joins(1), 128, 0, stream, p, ht);
   if (rc != B200_FP8_MM_OK || score_out == nullptr) return rc;
   const dim3 tiles(static_cast<unsigned>(p.logit_tiles), static_cast<unsigned>(cache->batch));
   return launch_pdl(p.tile == 64 ? attend_score_kernel<64> : attend_score_kernel<48>, tiles, kScoreGroups * p.tile, 0, stream, p);
