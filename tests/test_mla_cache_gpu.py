@@ -254,6 +254,23 @@ def test_attend_a_long_tail(heads, dtype, first):
     assert ((bt.attend()[0].double() - want).abs() <= tol).all()
 
 
+@pytest.mark.parametrize("heads", [16, 40, 64])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_attend_rising_and_falling_logits(heads, dtype):
+    """Every tile far above the one before for some heads, far below for the others."""
+    bt = Batch([1500, 30], heads, 256, 64, 48, dtype, seed=heads)
+    bt.q[:, ::2, 256] = 2
+    bt.q[:, 1::2, 256] = -2
+    for i, x in enumerate(bt.rows):
+        slot = torch.arange(len(x), device="cuda")
+        x[:, 256] = (slot // 7 * 7).to(x.dtype)
+        bt.cache[bt.table[i, slot // bt.page].long(), slot % bt.page] = x
+    score = bt.slots(1.0)
+    before = score.clone()
+    out, lse = bt.attend(score=score, return_lse=True)
+    check_attend(bt, out, lse, score, before)
+
+
 @pytest.mark.parametrize("scale", [0.0, -0.05, 3.0])
 def test_attend_scales(scale):
     """No preference, the least alike rows, nearly one row alone; the running maximum rises along the cache in the last."""
@@ -501,6 +518,33 @@ def test_evict_long(n):
     run_evict([n, n // 2], 1000, 100, page=64, seed=n)
 
 
+@pytest.mark.parametrize("lens,budget", [([700, 650, 90], 300), ([9000, 8000], 4100), ([40000], 1500)])
+@pytest.mark.parametrize("spread", ["equal", "two", "neighbours", "outliers", "dense", "one position", "denormal"])
+def test_evict_spreads_of_the_scores(spread, lens, budget):
+    """Ranges of the scores from one value to all there are, with many rows at the border or none."""
+    def make(score, position):
+        g = torch.Generator(device="cuda").manual_seed(len(lens))
+        k = torch.randint(0, 5000, score.shape, generator=g, device="cuda")
+        near = torch.full_like(score, 1.0).view(torch.int32)
+        if spread == "equal":
+            score.fill_(-3.0)
+        elif spread == "two":
+            score.copy_((k % 2).float())
+        elif spread == "neighbours":
+            score.copy_((near + (k % 300).int()).view(torch.float32))
+        elif spread == "outliers":
+            score.copy_((near + k.int()).view(torch.float32))
+            for n, v in ((0, math.inf), (1, -math.inf), (2, NAN), (3, -1e38), (4, 0.0)):
+                score[:, n::613] = v
+        elif spread == "dense":  # a bin that holds most of the rows
+            score.copy_(torch.where(k < 4000, (near + k.int()).view(torch.float32), score))
+        elif spread == "one position":  # all rows are protected, more than stay
+            position.fill_(-7)
+        else:
+            score.copy_((k.int() - 2500).abs().view(torch.float32) * (1 - 2 * (k % 2)))
+    run_evict(lens, budget, budget // 4, page=64, seed=budget, make=make, in_place=True)
+
+
 def test_evict_a_second_time_changes_nothing():
     bt, score, position, outs = run_evict([500, 60], 100, 10)
     before = bt.cache.clone()
@@ -610,6 +654,6 @@ def test_results_without_the_native_module(monkeypatch):
         assert g.shape == w.shape and g.dtype == w.dtype and torch.equal(g, w)
 
 
-@pytest.mark.parametrize("batch,n,budget", [(1, 70001, 30000), (3, 9000, 4000), (20, 5000, 64), (150, 300, 290), (1, 300000, 17)])
+@pytest.mark.parametrize("batch,n,budget", [(1, 70001, 30000), (3, 9000, 4000), (20, 5000, 64), (150, 300, 290), (1, 300000, 17), (75, 21000, 20930)])
 def test_evict_shapes_of_clusters(batch, n, budget):
     run_evict([n - i for i in range(batch)], budget, budget // 3, page=64, seed=n, in_place=True)
