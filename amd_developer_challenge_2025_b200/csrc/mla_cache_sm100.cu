@@ -486,11 +486,12 @@ struct Walk {
 // from chunk to chunk for both operands, and one copy brings all chunks of as many rows as lie together in a page, up to the tile.
 //
 // What bounds it: up to 32 heads, memory (6.2 TB/s while it runs); 64 heads, how long a tile stays. From its copy's way through memory
-// (1900 clocks) over the first product (1200), the softmax (1450, with its hand-overs) and the second product (740) to the next copy it
-// takes 5900, and two tiles of 64 rows are all that fits next to Q: 2950 clocks a tile, where the tensor core needs 1900 and, for 128
-// heads, memory 1600. That is with the next tile fetched to L2 while the ring is full (3400 a tile without; one sequence of 65536 rows
-// with 128 heads 45.8 -> 43.5 us). The softmax waits for the warp that shares a scheduler with the issuing one, 270 clocks behind the
-// others. Beginning costs 3300 clocks of setup and 7000 to 10000 up to the first product, as all SMs fetch at once; a segment's end 9000.
+// (1900 clocks, 39 bytes a clock: what L2 gives when all SMs ask) over the first product (1200), the softmax (1450, with its hand-overs)
+// and the second product (740) to the next copy it takes 5900, and two tiles of 64 rows are all that fits next to Q: 2950 clocks a tile,
+// where the tensor core needs 1900 and, for 128 heads, memory 1600. That is with the next tile fetched to L2 while the ring is full (3400
+// a tile without; one sequence of 65536 rows with 128 heads 45.8 -> 43.5 us). The softmax waits for the warp that shares a scheduler with
+// the issuing one, 270 clocks behind the others. Beginning costs 3300 clocks of setup and 7000 to 10000 up to the first product, as all
+// SMs fetch at once; a segment's end 9000.
 // Slower were: tiles of 32 rows, four of them in flight (162 against 142 us, 64 sequences of 4096 rows with 128 heads: an MMA takes 27
 // clocks to issue however small it is); units of 128 elements as the ring's grain; halves of a tile freed one by one; the second product
 // issued between chunks of the next tile's first (153 against 142 us: the issuing loop loses its pace).

@@ -116,6 +116,7 @@ def mla_cache_append(row, position, cache, block_table, lens, dv: int, theta: fl
     row [batch, dv + dr] (what `kv_down_projection_fp8` returns) goes to slot lens[b] of sequence b, its last dr elements
     rotated for position[b] (int32 [batch]); block_table must name the slot's page already, and lens is not changed. A
     sequence whose lens[b] is negative or at the block table's capacity, or whose page is not one of the cache's, is left alone.
+    No two sequences may name the same page for their new slots.
     q [batch, heads, dv + dr], optional: its last dr elements are rotated for the same positions into q_out (default: q itself;
     the others are copied). score (float32) and slot_position (int32), [batch, slots], optional: the new slot's entries become 0
     and position[b]. The rotation pairs element t with t + dr/2, angle position * theta**(-2t/dr), and unlike `mla_decode`

@@ -40,7 +40,8 @@ typedef struct {
  * or at the capacity is left alone. If `q` is not NULL, the last dr elements of every q[b][h] ([batch][heads][dv + dr]) are
  * rotated for the same position into q_out (which may be q), the others copied.
  *   t < dr/2, a = position * theta^(-2t/dr):  y[t] = x[t] cos a - x[t+dr/2] sin a,  y[t+dr/2] = x[t+dr/2] cos a + x[t] sin a
- * in fp32 with the angle reduced in fp64, rounded once. lens is not changed.
+ * in fp32 with the angle reduced in fp64, rounded once. lens is not changed. No two sequences may name the same page for their new
+ * slots.
  */
 int b200_mla_cache_append(const b200_mla_cache* cache, const void* row, long long row_stride, const int* position,
                           double theta, const void* q, long long q_sb, long long q_sh, void* q_out, long long qo_sb,
