@@ -1276,6 +1276,7 @@ __device__ __forceinline__ int threads_before(int v, int* scratch, int* total) {
 
 __device__ __forceinline__ void move_row(const EvictParams& p, int b, int to, int of, int lane) {
   const CacheView& c = p.cache;
+  if (to < 0 || to >= c.capacity || of < 0 || of >= c.capacity) return;
   const long long dst = slot_offset(c, b, to), src = slot_offset(c, b, of);
   if (dst >= 0) {
     uint4* o = reinterpret_cast<uint4*>(static_cast<uint16_t*>(c.data) + dst);
@@ -1511,7 +1512,7 @@ __global__ void __launch_bounds__(THREADS, 1) evict_select_kernel(const __grid_c
         for (; hits != 0; hits &= hits - 1) {
           const int to = ties_before + atomicAdd(&few_count, 1);
           const uint32_t r = rank_at(at + (__ffs(hits) - 1) * THREADS);
-          for (int k = 0; k < cluster; ++k) put(&few[to], k, r);
+          for (int k = 0; k < cluster && to < kFew; ++k) put(&few[to], k, r);
         }
       };
       int seen = 0;
@@ -1605,7 +1606,8 @@ __global__ void __launch_bounds__(THREADS, 1) evict_select_kernel(const __grid_c
           const int slot = begin + 32 * (w0 + w) + lane;
           const int to = holes_before + static_cast<int>(before & 0xffffu) + __popc(hole & lower);
           const int of = late_before + static_cast<int>(before >> 16) + __popc(moved & lower);
-          const bool fill = hole >> lane & 1u, move = moved >> lane & 1u;
+          // (The lists hold p.most slots, more than there are unless something else writes to the scores meanwhile.)
+          const bool fill = (hole >> lane & 1u) && to < p.most, move = (moved >> lane & 1u) && of < p.most;
           if (!p.few) {
             if (fill) holes_list[to] = slot;
             if (move) late_list[of] = slot;
@@ -1626,6 +1628,7 @@ __global__ void __launch_bounds__(THREADS, 1) evict_select_kernel(const __grid_c
         moves += holes_of[k];
         if (k < me) holes_at += holes_of[k], late_at += late_of[k];
       }
+      moves = min(moves, p.most);
       if (me == 0 && tid == 0 && !p.few) p.moves[b] = moves;
     }
   }
