@@ -213,7 +213,7 @@ struct AttendParams {
   float scale_log2;        // scale * log2(e)
   // Workspace
   long long* begins;       // [batch + 1]: places before each sequence, and all
-  float* lse2;             // [batch][heads]: log2 of the sum of 2^x
+  float* lse2;             // [batch][heads]: log2 of the sum of 2^x; 0 where that sum is 0 (every logit is -inf, and so no weight)
   float2* part_stat;       // [worker][head tile][2][heads of a tile]: maximum and sum
   float* part_out;         // [worker][head tile][2][128-element unit of the value][heads of a tile][128]
   float* logits;           // [batch][tile][heads][rows of a tile] in log2, or null
@@ -414,6 +414,9 @@ __device__ __forceinline__ float exp2_fast(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+
+// What a sum of weights is divided by. It is 0 only where every logit is -inf: such a head gets zeros, as one of a sequence without rows.
+__device__ __forceinline__ float inverse_of(float total) { return total == 0.f ? 0.f : 1.f / total; }
 
 __device__ __forceinline__ uint32_t pack2(float lo, float hi, __nv_bfloat16) {
   uint32_t r;
@@ -1019,8 +1022,8 @@ attend_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__
       if (active && lane % 4 == 0) {
         sh.stat[row0] = make_float2(m0, l0);
         sh.stat[row1] = make_float2(m1, l1);
-        sh.inverse[row0] = 1.f / l0;
-        sh.inverse[row1] = 1.f / l1;
+        sh.inverse[row0] = inverse_of(l0);
+        sh.inverse[row1] = inverse_of(l1);
       }
       softmax_sync();
       tcgen05_fence_after();
@@ -1056,7 +1059,7 @@ attend_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__
           const float2 st = sh.stat[tid];
           const float lse2 = (st.x == -INFINITY ? 0.f : st.x) + log2f(st.y);
           const long long at = static_cast<long long>(walk.b) * heads_all + head0 + tid;
-          p.lse2[at] = lse2;
+          p.lse2[at] = st.y == 0.f ? 0.f : lse2;
           if (p.lse != nullptr) p.lse[at] = lse2 * kLn2;
         }
       } else if (tid < heads) {
@@ -1169,7 +1172,7 @@ __global__ void __launch_bounds__(128 * GROUPS) attend_join_kernel(const __grid_
     }
     if (n >= heads) return;
     if (4 * e < dv) {
-      const float inverse = 1.f / total;
+      const float inverse = inverse_of(total);
       T* const to = out + n * p.out_sh + 4 * e;
       from_float(sum.x * inverse, to);
       from_float(sum.y * inverse, to + 1);
@@ -1178,7 +1181,7 @@ __global__ void __launch_bounds__(128 * GROUPS) attend_join_kernel(const __grid_
     }
     if (tid == 0) {
       const float lse2 = base + log2f(total);
-      p.lse2[at + n] = lse2;
+      p.lse2[at + n] = total == 0.f ? 0.f : lse2;
       if (p.lse != nullptr) p.lse[at + n] = lse2 * kLn2;
     }
   }

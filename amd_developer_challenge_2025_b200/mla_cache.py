@@ -173,8 +173,8 @@ def mla_cache_attend(q, cache, block_table, lens, dv: int, scale: float, out=Non
     (out, lse) with return_lse, lse float32 [batch, heads].
 
     out[b, h] = sum over j < lens[b] of p_j * row_j[:dv], p = softmax(scale * q[b, h] . row_j); q [batch, heads, dv + dr] carries
-    the up-projection of the keys already. A sequence without rows gets zeros (lse -inf); what lies behind a sequence's last row
-    is never looked at. lens above the block table's capacity count as the capacity; a page that is not one of the cache's reads
+    the up-projection of the keys already. A sequence without rows gets zeros (lse -inf), and so does a head whose logits are all
+    -inf (it adds nothing to the scores); what lies behind a sequence's last row is never looked at. lens above the block table's capacity count as the capacity; a page that is not one of the cache's reads
     as rows of zeros. score (float32 [batch, slots]), optional: score_out[b, j] = score[b, j] + the weights that slot j received
     from all heads (score_out default: score itself), j < lens[b]; other entries are left as they were. max_len, optional: no
     sequence is longer (longer ones are cut to it); it sizes the scratch that the weights need, batch * heads * max_len floats.

@@ -50,11 +50,11 @@ int b200_mla_cache_append(const b200_mla_cache* cache, const void* row, long lon
 
 /*
  * out[b][h] = sum_j p_j x_j[0..dv),  p = softmax_j(scale * q[b][h] . x_j),  j < lens[b];  lse[b][h] = log sum_j exp(.) (may be
- * NULL). A sequence without rows gets zeros and -inf. With score_out (else NULL): score_out[b][j] = score[b][j] + sum_h p_j for
- * j < lens[b]; slots behind are left as they were; score_out may be score. max_len: lengths above it count as max_len (0: the
- * capacity). q, out: [batch][heads][dv + dr] and [.. dv], last dimension contiguous; q 16-byte aligned with strides that are
- * multiples of 8. |scale| < 2^127. lse: contiguous. Sums, maxima and the joins of the splits are fp32; the weights are rounded to
- * the cache's type for the second product. Results do not depend on timing.
+ * NULL). A sequence without rows gets zeros and -inf, as does a head whose logits are all -inf. With score_out (else NULL):
+ * score_out[b][j] = score[b][j] + sum_h p_j for j < lens[b]; slots behind are left as they were; score_out may be score. max_len:
+ * lengths above it count as max_len (0: the capacity). q, out: [batch][heads][dv + dr] and [.. dv], last dimension contiguous; q
+ * 16-byte aligned with strides that are multiples of 8. |scale| < 2^127. lse: contiguous. Sums, maxima and the joins of the splits are
+ * fp32; the weights are rounded to the cache's type for the second product. Results do not depend on timing.
  * device_status: int[4] as for b200_fp8_mm (may be NULL).
  */
 int b200_mla_cache_attend(const b200_mla_cache* cache, const void* q, long long q_sb, long long q_sh, int heads, float scale,

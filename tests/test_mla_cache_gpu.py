@@ -657,3 +657,30 @@ def test_results_without_the_native_module(monkeypatch):
 @pytest.mark.parametrize("batch,n,budget", [(1, 70001, 30000), (3, 9000, 4000), (20, 5000, 64), (150, 300, 290), (1, 300000, 17), (75, 21000, 20930)])
 def test_evict_shapes_of_clusters(batch, n, budget):
     run_evict([n - i for i in range(batch)], budget, budget // 3, page=64, seed=n, in_place=True)
+
+
+@pytest.mark.parametrize("lens", [[130, 0, 64], [4000, 100, 0, 60]], ids=["whole", "split"])
+@pytest.mark.parametrize("heads,page,dtype", [(16, 16, "bf16"), (16, 5, "fp16"), (40, 16, "fp16"), (128, 64, "bf16")])
+def test_attend_heads_without_weights(lens, heads, page, dtype):
+    """A head all of whose logits are -inf gets zeros and an lse of -inf, as a sequence without rows does, and adds nothing to the
+    scores; the other heads of its sequence are as they would be without it."""
+    bt = Batch(lens, heads, dv=128, page=page, dtype=dtype, seed=heads)
+    for i, x in enumerate(bt.rows):
+        slot = torch.arange(len(x), device="cuda")
+        x[:, 130] = 1.0
+        bt.cache[bt.table[i, slot // page].long(), slot % page] = x
+    dead = torch.arange(heads, device="cuda") % 5 == 2
+    bt.q[:, dead, 130] = -math.inf
+    score = torch.rand(len(lens), bt.capacity, generator=bt.g, device="cuda")
+    before = score.clone()
+    out, lse = bt.attend(return_lse=True, score=score, max_len=max(lens))
+    assert (out[:, dead] == 0).all() and (lse[:, dead] == -math.inf).all()
+    live = Batch.__new__(Batch)
+    live.__dict__.update(bt.__dict__)
+    live.q = bt.q[:, ~dead]
+    check_attend(live, out[:, ~dead], lse[:, ~dead], score, before)
+    # every head of every sequence: the scores stay as they were
+    bt.q[:, :, 130] = -math.inf
+    score.copy_(before)
+    out, lse = bt.attend(return_lse=True, score=score)
+    assert (out == 0).all() and (lse == -math.inf).all() and torch.equal(score, before)
