@@ -684,3 +684,12 @@ def test_attend_heads_without_weights(lens, heads, page, dtype):
     score.copy_(before)
     out, lse = bt.attend(return_lse=True, score=score)
     assert (out == 0).all() and (lse == -math.inf).all() and torch.equal(score, before)
+
+
+@pytest.mark.parametrize("heads", [64 * 148 + 1, 1 << 16])
+def test_attend_more_head_tiles_than_sms(heads):
+    """Every head tile has one worker then, and the launch more CTAs than the chip takes at a time."""
+    bt = Batch([400, 0, 33], heads, dv=128, dr=0, page=16, seed=3)
+    score = bt.slots()
+    out, lse = bt.attend(return_lse=True, score=score, max_len=400)
+    check_attend(bt, out, lse, score, bt.slots())
