@@ -39,6 +39,7 @@ EXPORTS = (
     # include/b200_mla_cache.h
     "b200_mla_cache_append",
     "b200_mla_cache_attend",
+    "b200_mla_cache_attend_selftest_wait_expiry",
     "b200_mla_cache_attend_workspace_bytes",
     "b200_mla_cache_evict",
     "b200_mla_cache_evict_workspace_bytes",
@@ -187,6 +188,9 @@ def load() -> ctypes.CDLL:
     lib.b200_mla_cache_attend.argtypes = [ctypes.POINTER(CMlaCache), p, n, n, i, ctypes.c_float, p, n, n, p, p, n, p, n, i, p,
                                           ctypes.c_size_t, p, p]
     lib.b200_mla_cache_attend.restype = i
+    lib.b200_mla_cache_attend_selftest_wait_expiry.argtypes = [ctypes.POINTER(CMlaCache), p, n, n, i, ctypes.c_float, p, n, n, p,
+                                                               ctypes.c_size_t, ctypes.c_ulonglong, i, p, p]
+    lib.b200_mla_cache_attend_selftest_wait_expiry.restype = i
     lib.b200_mla_cache_attend_workspace_bytes.argtypes = [i] * 6
     lib.b200_mla_cache_attend_workspace_bytes.restype = ctypes.c_size_t
     lib.b200_mla_cache_evict.argtypes = [ctypes.POINTER(CMlaCache), p, n, p, n, i, i, p, p, n, p, n, p, ctypes.c_size_t, p]

@@ -219,6 +219,8 @@ struct AttendParams {
   float* logits;           // [batch][tile][heads][rows of a tile] in log2, or null
   int logit_tiles;
   int* status;             // may be null
+  unsigned long long selftest_wait_limit_ns;  // the self-test's kernels give up a wait after this long,
+  int selftest_skip_tile;                     // and do not copy this tile of the first sequence
 };
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
@@ -265,10 +267,11 @@ __device__ __forceinline__ unsigned long long global_ns() {
 struct Waits {
   volatile int* expired;  // shared memory
   int* status;            // global, may be null
+  unsigned long long limit_ns;
 
   __device__ bool give_up(unsigned long long t0, uint32_t parity, int where) const {
     if (*expired) return true;
-    if (global_ns() - t0 <= kWaitLimitNs) return false;
+    if (global_ns() - t0 <= limit_ns) return false;
     *expired = 1;
     if (status != nullptr && atomicCAS(status, 0, B200_FP8_MM_DEV_WAIT_EXPIRED) == 0) {
       status[1] = where;
@@ -505,7 +508,7 @@ struct Walk {
 // product runs under this tile's softmax. The running maximum is replaced only when a logit exceeds it by 8 (in base 2): the weights
 // stay below 2^8 in bf16 and 2^15 in fp16, and rescaling the accumulators is rare. Sums are kept in fp32, weights are rounded to the
 // cache's type for the second product, as matrix operands have to be.
-template <typename T, int HT>
+template <typename T, int HT, bool SELFTEST = false>
 __global__ void __launch_bounds__(kAttendThreads, 1)
 attend_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap row_map, const __grid_constant__ AttendParams p) {
   constexpr int kTile = tile_rows_for(HT);
@@ -525,7 +528,7 @@ attend_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__
   const int tid = static_cast<int>(threadIdx.x), warp = tid >> 5, lane = tid & 31;
   const int head_tile = static_cast<int>(blockIdx.x) % p.head_tiles, worker = static_cast<int>(blockIdx.x) / p.head_tiles;
   const int head0 = head_tile * HT;
-  const Waits waits{&sh.expired, p.status};
+  const Waits waits{&sh.expired, p.status, SELFTEST ? p.selftest_wait_limit_ns : kWaitLimitNs};
   if (tid == 0) {
     for (int i = 0; i < kMaxStages; ++i) {
       mbar_init(smem_u32(&sh.full[i]), p.copy_rows > 0 ? 1 : kRowWarps);
@@ -611,22 +614,6 @@ attend_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__
     tma_load_4d(smem_u32(q_smem), &q_map, head0, 0, b, smem_u32(&sh.q_full));
     return true;
   };
-  // At the end of a copying role: where a wait has expired, no copy may still be in flight when the CTA ends. A phase that will not
-  // complete (a use that was not begun) runs out of its 10 ms.
-  auto drain_copies = [&]() {
-    asm volatile("cp.async.wait_all;" ::: "memory");
-    if (__any_sync(0xffffffffu, sh.expired != 0) && lane == 0 && warp == 4) {
-      auto drain = [&](uint64_t* bar) {
-        for (uint32_t parity = 0; parity < 2; ++parity)
-          for (int n = 0; n < 1000 && !mbar_try_wait(smem_u32(bar), parity, 10000); ++n) {
-          }
-      };
-      for (int n = 0; copy_rows > 0 && n < stages; ++n) drain(&sh.full[n]);
-      drain(&sh.q_full);
-    }
-    __syncwarp();
-  };
-
   // Warps 6 and 7: where no join follows, what sequences without rows get.
   auto write_empty = [&]() {
     if (p.joined) return;
@@ -666,13 +653,14 @@ attend_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__
         }
       };
       place(walk.t);
-      const int count = __shfl_sync(0xffffffffu, walk.count, 0);
+      const int count = __shfl_sync(0xffffffffu, walk.count, 0), left_out = SELFTEST && walk.b == 0 ? p.selftest_skip_tile - walk.t : -1;
       for (int tile = 0; tile < count; ++tile) {
         const uint32_t full = smem_u32(&sh.full[stage]), to = smem_u32(ring) + stage * tile_bytes;
         if (!first_lap && !(ok = waits.wait_all(smem_u32(&sh.pv_done[stage]), lap ^ 1, kAtFree))) break;
-        if (lane == 0) mbar_expect_tx(full, tile_bytes);
+        const int copies = SELFTEST && tile == left_out ? 0 : pieces;
+        if (lane == 0 && (!SELFTEST || copies > 0)) mbar_expect_tx(full, tile_bytes);
         __syncwarp();
-        for (int k = 0; k < pieces; ++k)
+        for (int k = 0; k < copies; ++k)
           tma_load_5d(to + k * (copy_rows >> 3) * group_bytes, &row_map, 0, 0, __shfl_sync(0xffffffffu, slot, k) >> 3,
                       __shfl_sync(0xffffffffu, page, k), full);
         if (++stage == stages) stage = 0, lap ^= 1, first_lap = false;
@@ -686,7 +674,6 @@ attend_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__
       }
       ++segment;
     }
-    drain_copies();
   } else if ((warp == 4 || warp > 5) && copy_rows == 0) {
     // Copies row by row, every third row of a tile, 16 bytes a lane. Lane l knows where rows l and l + 32 of a tile come from. A tile
     // is announced once its copies have landed: when the next one's are on their way, or when nothing else can be done.
@@ -722,7 +709,7 @@ attend_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__
         }
       };
       place(walk.t);
-      const int count = __shfl_sync(0xffffffffu, walk.count, 0);
+      const int count = __shfl_sync(0xffffffffu, walk.count, 0), left_out = SELFTEST && walk.b == 0 ? p.selftest_skip_tile - walk.t : -1;
       for (int tile = 0; tile < count; ++tile) {
         if (!first_lap && !__all_sync(0xffffffffu, mbar_test(smem_u32(&sh.pv_done[stage]), lap ^ 1))) {
           announce(true);
@@ -742,7 +729,7 @@ attend_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
         announce(false);
-        landing = stage;
+        landing = SELFTEST && tile == left_out ? -1 : stage;
         if (++stage == stages) stage = 0, lap ^= 1, first_lap = false;
         if (tile == 0 && warp == 4) {
           announce(true);
@@ -753,7 +740,7 @@ attend_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__
       ++segment;
     }
     announce(true);
-    drain_copies();
+    asm volatile("cp.async.wait_all;" ::: "memory");  // (those of a tile that was begun when a wait expired)
     if (warp > 5) write_empty();
   } else if (warp > 5) {
     write_empty();
@@ -856,11 +843,6 @@ attend_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__
       ++segment;
     }
     if (ok && pending && until(false, false)) second();
-    if (__any_sync(kAll, sh.expired != 0)) {  // none in flight past here
-      umma_commit(smem_u32(&sh.drained));
-      for (int n = 0; n < 1000 && !mbar_try_wait(smem_u32(&sh.drained), 0, 10000); ++n) {
-      }
-    }
     __syncwarp();
   } else if (warp < 4) {
     // Softmax: warp w has heads 16 w .. 16 w + 15 of the tile, thread t rows (heads) t / 4 and t / 4 + 8 of these.
@@ -1069,6 +1051,26 @@ attend_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__
   }
   tcgen05_fence_before();
   __syncthreads();
+  // Where a wait has expired, copies and products may still be in flight, whichever role it was: no shared memory and no TMEM is given
+  // back before they have come to rest. (Looked at when all roles are over: one that ended early has not seen a later one's wait expire.)
+  // Each of these waits is bounded too; a phase that will not complete, because its use was not begun, runs out of its 10 ms.
+  if (sh.expired != 0) {
+    auto at_rest = [&](uint64_t* bar, uint32_t parity) {
+      for (int n = 0; n < 1000 && !mbar_try_wait(smem_u32(bar), parity, 10000); ++n) {
+      }
+    };
+    if (warp == 4 && lane == 0) {
+      for (uint32_t parity = 0; parity < 2; ++parity) {
+        for (int n = 0; copy_rows > 0 && n < stages; ++n) at_rest(&sh.full[n], parity);
+        at_rest(&sh.q_full, parity);
+      }
+    }
+    if (warp == 5) {
+      umma_commit(smem_u32(&sh.drained));
+      at_rest(&sh.drained, 0);
+    }
+    __syncwarp();
+  }
   if (warp == 5) {
     tcgen05_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
@@ -1817,6 +1819,11 @@ AttendFn attend_fn(bool bf16, int ht) {
   return ht == 16 ? attend_kernel<__half, 16> : ht == 32 ? attend_kernel<__half, 32> : attend_kernel<__half, 64>;
 }
 
+// Their own kernels: looking for the tile to leave out in every launch cost 0.4 % (128 x 4096 rows, 16 heads: 113.0 against 112.6 us).
+AttendFn attend_selftest_fn(int ht) {
+  return ht == 16 ? attend_kernel<__nv_bfloat16, 16, true> : ht == 32 ? attend_kernel<__nv_bfloat16, 32, true> : attend_kernel<__nv_bfloat16, 64, true>;
+}
+
 // Lets a kernel take that much shared memory, once per device.
 template <typename Fn>
 bool opt_in(Fn fn, int bytes, std::atomic<bool>* done) {
@@ -1827,6 +1834,98 @@ bool opt_in(Fn fn, int bytes, std::atomic<bool>* done) {
   }
   done->store(true, std::memory_order_relaxed);
   return true;
+}
+
+// b200_mla_cache_attend, and its self-test with a shorter limit for the waits and a tile that is left out.
+int run_attend(const b200_mla_cache* cache, const void* q, long long q_sb, long long q_sh, int heads, float scale, void* out,
+               long long out_sb, long long out_sh, float* lse, const float* score, long long score_stride, float* score_out,
+               long long score_out_stride, int max_len, void* workspace, size_t workspace_bytes, int* device_status, void* stream,
+               unsigned long long wait_limit_ns, int selftest_skip_tile) {
+  AttendParams p = {};
+  int rc = view_of(cache, &p.cache);
+  if (rc != B200_FP8_MM_OK) return rc;
+  if (q == nullptr || out == nullptr || (score_out != nullptr && score == nullptr)) return B200_FP8_MM_ERR_NULL;
+  if (heads <= 0 || heads > kMaxHeads || max_len < 0 || !(fabsf(scale) < 0x1p127f)) return B200_FP8_MM_ERR_SHAPE;
+  if (cache->batch == 1) q_sb = p.cache.d;  // (no second one)
+  if (heads == 1) q_sh = p.cache.d;
+  if (q_sb % 8 != 0 || q_sh % 8 != 0 || q_sb < p.cache.d || q_sh < p.cache.d) return B200_FP8_MM_ERR_STRIDE;
+  if (!aligned16(q)) return B200_FP8_MM_ERR_ALIGN;
+  if (max_len == 0 || max_len > p.cache.capacity) max_len = p.cache.capacity;
+  const int sms = sm_count_for_sizing();
+  const AttendWorkspace w = attend_workspace(cache->batch, heads, cache->dv, max_len, score_out != nullptr, sms);
+  if (workspace == nullptr || reinterpret_cast<uintptr_t>(workspace) % 256 != 0 || workspace_bytes < w.bytes) return B200_FP8_MM_ERR_WORKSPACE;
+  const int ht = tile_heads_for(heads), device = current_device();
+  if (device < 0) return B200_FP8_MM_ERR_DRIVER;
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  p.out = out;
+  p.lse = lse;
+  p.score = score;
+  p.score_out = score_out;
+  p.out_sb = out_sb;
+  p.out_sh = out_sh;
+  p.score_stride = score_stride;
+  p.score_out_stride = score_out_stride;
+  p.heads = heads;
+  p.head_tiles = (heads + ht - 1) / ht;
+  p.max_len = max_len;
+  p.batch = cache->batch;
+  p.workers = attend_workers(heads, sms);
+  p.least = kLeastPlaces + extra_for(ht);
+  p.tile = tile_rows_for(ht);
+  p.extra = extra_for(ht);
+  p.copy_rows = cache_walk::copy_rows(cache->page_size, p.tile);
+  if (p.copy_rows < 8) p.copy_rows = 0;
+  p.v_units = cache->dv / 128;
+  p.chunks = p.cache.d / 64;
+  p.scale_log2 = scale * kLog2E;
+  p.joined = cache_walk::tiles_of(max_len, p.tile) > cache_walk::kWholeTiles;
+  p.begins = reinterpret_cast<long long*>(ws);
+  p.lse2 = reinterpret_cast<float*>(ws + w.lse2);
+  p.part_stat = reinterpret_cast<float2*>(ws + w.part_stat);
+  p.part_out = reinterpret_cast<float*>(ws + w.part_out);
+  p.logits = score_out != nullptr ? reinterpret_cast<float*>(ws + w.logits) : nullptr;
+  p.logit_tiles = cache_walk::tiles_of(max_len, p.tile);
+  p.status = device_status;
+  p.selftest_wait_limit_ns = wait_limit_ns;
+  p.selftest_skip_tile = selftest_skip_tile;
+  const size_t smem = plan_ring(ht, &p);
+  const bool bf16 = cache->dtype == B200_MLA_CACHE_BF16;
+  CUtensorMap q_map, row_map;
+  MapDims q_dims, row_dims;
+  q_dims.add(heads, q_sh, ht);
+  q_dims.add(p.chunks, 64, p.chunks);
+  q_dims.add(cache->batch, q_sb, 1);
+  if (p.copy_rows > 0) {
+    row_dims.add(8, cache->slot_stride, 8);
+    row_dims.add(p.chunks, 64, p.chunks);
+    row_dims.add(cache->page_size / 8, 8 * cache->slot_stride, p.copy_rows / 8);
+    row_dims.add(cache->pages, cache->page_stride, 1);
+  }
+  if (!q_dims.encode(&q_map, q, bf16)) return B200_FP8_MM_ERR_DRIVER;
+  if (p.copy_rows == 0)
+    row_map = q_map;  // (not used)
+  else if (!row_dims.encode(&row_map, cache->data, bf16))
+    return B200_FP8_MM_ERR_DRIVER;
+  const bool selftest = selftest_skip_tile >= 0;
+  if (selftest && !bf16) return B200_FP8_MM_ERR_SHAPE;
+  const AttendFn fn = selftest ? attend_selftest_fn(ht) : attend_fn(bf16, ht);
+  static std::atomic<bool> opted[kMaxDevices][9];
+  if (!opt_in(fn, kMaxSmem, &opted[device][(selftest ? 6 : bf16 ? 0 : 3) + (ht == 16 ? 0 : ht == 32 ? 1 : 2)])) return B200_FP8_MM_ERR_DRIVER;
+  rc = launch_pdl(fn, dim3(static_cast<unsigned>(p.workers) * p.head_tiles), kAttendThreads, smem, stream, q_map, row_map, p);
+  if (rc != B200_FP8_MM_OK) return rc;
+  // Eight groups where a sequence has eight parts and more on average, one where most have one or two.
+  auto joins = [&](int groups) {
+    return dim3(static_cast<unsigned>((heads + join_heads(groups) - 1) / join_heads(groups)), static_cast<unsigned>(cache->batch));
+  };
+  if (!p.joined)
+    rc = B200_FP8_MM_OK;
+  else if (p.workers / cache->batch >= 8)
+    rc = launch_pdl(bf16 ? attend_join_kernel<__nv_bfloat16, 8> : attend_join_kernel<__half, 8>, joins(8), 1024, 0, stream, p, ht);
+  else
+    rc = launch_pdl(bf16 ? attend_join_kernel<__nv_bfloat16, 1> : attend_join_kernel<__half, 1>, joins(1), 128, 0, stream, p, ht);
+  if (rc != B200_FP8_MM_OK || score_out == nullptr) return rc;
+  const dim3 tiles(static_cast<unsigned>(p.logit_tiles), static_cast<unsigned>(cache->batch));
+  return launch_pdl(p.tile == 64 ? attend_score_kernel<64> : attend_score_kernel<48>, tiles, kScoreGroups * p.tile, 0, stream, p);
 }
 
 int evict_most(long long capacity, int budget) {
@@ -1882,87 +1981,20 @@ int b200_mla_cache_attend(const b200_mla_cache* cache, const void* q, long long 
                           void* out, long long out_sb, long long out_sh, float* lse, const float* score,
                           long long score_stride, float* score_out, long long score_out_stride, int max_len, void* workspace,
                           size_t workspace_bytes, int* device_status, void* stream) {
-  AttendParams p = {};
-  int rc = view_of(cache, &p.cache);
-  if (rc != B200_FP8_MM_OK) return rc;
-  if (q == nullptr || out == nullptr || (score_out != nullptr && score == nullptr)) return B200_FP8_MM_ERR_NULL;
-  if (heads <= 0 || heads > kMaxHeads || max_len < 0 || !(fabsf(scale) < 0x1p127f)) return B200_FP8_MM_ERR_SHAPE;
-  if (cache->batch == 1) q_sb = p.cache.d;  // (no second one)
-  if (heads == 1) q_sh = p.cache.d;
-  if (q_sb % 8 != 0 || q_sh % 8 != 0 || q_sb < p.cache.d || q_sh < p.cache.d) return B200_FP8_MM_ERR_STRIDE;
-  if (!aligned16(q)) return B200_FP8_MM_ERR_ALIGN;
-  if (max_len == 0 || max_len > p.cache.capacity) max_len = p.cache.capacity;
-  const int sms = sm_count_for_sizing();
-  const AttendWorkspace w = attend_workspace(cache->batch, heads, cache->dv, max_len, score_out != nullptr, sms);
-  if (workspace == nullptr || reinterpret_cast<uintptr_t>(workspace) % 256 != 0 || workspace_bytes < w.bytes) return B200_FP8_MM_ERR_WORKSPACE;
-  const int ht = tile_heads_for(heads), device = current_device();
-  if (device < 0) return B200_FP8_MM_ERR_DRIVER;
-  uint8_t* ws = static_cast<uint8_t*>(workspace);
-  p.out = out;
-  p.lse = lse;
-  p.score = score;
-  p.score_out = score_out;
-  p.out_sb = out_sb;
-  p.out_sh = out_sh;
-  p.score_stride = score_stride;
-  p.score_out_stride = score_out_stride;
-  p.heads = heads;
-  p.head_tiles = (heads + ht - 1) / ht;
-  p.max_len = max_len;
-  p.batch = cache->batch;
-  p.workers = attend_workers(heads, sms);
-  p.least = kLeastPlaces + extra_for(ht);
-  p.tile = tile_rows_for(ht);
-  p.extra = extra_for(ht);
-  p.copy_rows = cache_walk::copy_rows(cache->page_size, p.tile);
-  if (p.copy_rows < 8) p.copy_rows = 0;
-  p.v_units = cache->dv / 128;
-  p.chunks = p.cache.d / 64;
-  p.scale_log2 = scale * kLog2E;
-  p.joined = cache_walk::tiles_of(max_len, p.tile) > cache_walk::kWholeTiles;
-  p.begins = reinterpret_cast<long long*>(ws);
-  p.lse2 = reinterpret_cast<float*>(ws + w.lse2);
-  p.part_stat = reinterpret_cast<float2*>(ws + w.part_stat);
-  p.part_out = reinterpret_cast<float*>(ws + w.part_out);
-  p.logits = score_out != nullptr ? reinterpret_cast<float*>(ws + w.logits) : nullptr;
-  p.logit_tiles = cache_walk::tiles_of(max_len, p.tile);
-  p.status = device_status;
-  const size_t smem = plan_ring(ht, &p);
-  const bool bf16 = cache->dtype == B200_MLA_CACHE_BF16;
-  CUtensorMap q_map, row_map;
-  MapDims q_dims, row_dims;
-  q_dims.add(heads, q_sh, ht);
-  q_dims.add(p.chunks, 64, p.chunks);
-  q_dims.add(cache->batch, q_sb, 1);
-  if (p.copy_rows > 0) {
-    row_dims.add(8, cache->slot_stride, 8);
-    row_dims.add(p.chunks, 64, p.chunks);
-    row_dims.add(cache->page_size / 8, 8 * cache->slot_stride, p.copy_rows / 8);
-    row_dims.add(cache->pages, cache->page_stride, 1);
-  }
-  if (!q_dims.encode(&q_map, q, bf16)) return B200_FP8_MM_ERR_DRIVER;
-  if (p.copy_rows == 0)
-    row_map = q_map;  // (not used)
-  else if (!row_dims.encode(&row_map, cache->data, bf16))
-    return B200_FP8_MM_ERR_DRIVER;
-  const AttendFn fn = attend_fn(bf16, ht);
-  static std::atomic<bool> opted[kMaxDevices][6];
-  if (!opt_in(fn, kMaxSmem, &opted[device][(bf16 ? 0 : 3) + (ht == 16 ? 0 : ht == 32 ? 1 : 2)])) return B200_FP8_MM_ERR_DRIVER;
-  rc = launch_pdl(fn, dim3(static_cast<unsigned>(p.workers) * p.head_tiles), kAttendThreads, smem, stream, q_map, row_map, p);
-  if (rc != B200_FP8_MM_OK) return rc;
-  // Eight groups where a sequence has eight parts and more on average, one where most have one or two.
-  auto joins = [&](int groups) {
-    return dim3(static_cast<unsigned>((heads + join_heads(groups) - 1) / join_heads(groups)), static_cast<unsigned>(cache->batch));
-  };
-  if (!p.joined)
-    rc = B200_FP8_MM_OK;
-  else if (p.workers / cache->batch >= 8)
-    rc = launch_pdl(bf16 ? attend_join_kernel<__nv_bfloat16, 8> : attend_join_kernel<__half, 8>, joins(8), 1024, 0, stream, p, ht);
-  else
-    rc = launch_pdl(bf16 ? attend_join_kernel<__nv_bfloat16, 1> : attend_join_kernel<__half, 1>, joins(1), 128, 0, stream, p, ht);
-  if (rc != B200_FP8_MM_OK || score_out == nullptr) return rc;
-  const dim3 tiles(static_cast<unsigned>(p.logit_tiles), static_cast<unsigned>(cache->batch));
-  return launch_pdl(p.tile == 64 ? attend_score_kernel<64> : attend_score_kernel<48>, tiles, kScoreGroups * p.tile, 0, stream, p);
+  return run_attend(cache, q, q_sb, q_sh, heads, scale, out, out_sb, out_sh, lse, score, score_stride, score_out, score_out_stride,
+                    max_len, workspace, workspace_bytes, device_status, stream, kWaitLimitNs, -1);
+}
+
+int b200_mla_cache_attend_selftest_wait_expiry(const b200_mla_cache* cache, const void* q, long long q_sb, long long q_sh, int heads,
+                                               float scale, void* out, long long out_sb, long long out_sh, void* workspace,
+                                               size_t workspace_bytes, unsigned long long wait_limit_ns, int skip_tile,
+                                               int* device_status, void* stream) {
+  if (device_status == nullptr) return B200_FP8_MM_ERR_NULL;
+  if (skip_tile < 0) return B200_FP8_MM_ERR_SHAPE;
+  // Soon, because the GPU is busy until then, but later than any wait that is only slow.
+  if (wait_limit_ns < 1000000ull || wait_limit_ns > 100000000ull) return B200_FP8_MM_ERR_PLAN;
+  return run_attend(cache, q, q_sb, q_sh, heads, scale, out, out_sb, out_sh, nullptr, nullptr, 0, nullptr, 0, 0, workspace,
+                    workspace_bytes, device_status, stream, wait_limit_ns, skip_tile);
 }
 
 size_t b200_mla_cache_evict_workspace_bytes(int batch, int capacity, int budget) {

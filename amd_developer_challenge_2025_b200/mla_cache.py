@@ -230,6 +230,37 @@ def mla_cache_attend(q, cache, block_table, lens, dv: int, scale: float, out=Non
     return (out, lse) if return_lse else out
 
 
+def selftest_wait_expiry(device="cuda", heads: int = 16, page_size: int = 16, limit_ms: float = 5.0):
+    """Diagnostics: makes waits inside the attention's kernel run out on purpose, in the allowed way. A sequence of four tiles is attended
+    to with every wait limited to `limit_ms` and the second tile's copy left out; the kernel gives up, returns by itself and reports the
+    wait. Returns the four status words [code, wait, block, phase]; code 1 is WAIT_EXPIRED. The words are cleared again."""
+    dev = torch.device(device)
+    if dev.index is None:
+        dev = torch.device("cuda", torch.cuda.current_device())
+    lib, dv, d = _lib.load(), 512, 576
+    with torch.cuda.device(dev):
+        rows = 192
+        pages = -(-rows // page_size)
+        cache = torch.zeros(pages, page_size, d, dtype=torch.bfloat16, device=dev)
+        table = torch.arange(pages, dtype=torch.int32, device=dev)[None]
+        lens = torch.full((1,), rows, dtype=torch.int32, device=dev)
+        q, out = (torch.zeros(1, heads, width, dtype=torch.bfloat16, device=dev) for width in (d, dv))
+        ws = _workspace(dev, lib.b200_mla_cache_attend_workspace_bytes(1, heads, dv, d - dv, table.shape[1] * page_size, 0))
+        st = _status_words(dev)
+        torch.cuda.synchronize(dev)
+        rc = lib.b200_mla_cache_attend_selftest_wait_expiry(
+            ctypes.byref(_c_cache(cache, table, lens, dv)), q.data_ptr(), q.stride(0), q.stride(1), heads, 1.0, out.data_ptr(),
+            out.stride(0), out.stride(1), ws.data_ptr(), ws.numel(), int(limit_ms * 1e6), 1, st.data_ptr(),
+            torch.cuda.current_stream(dev).cuda_stream)
+        if rc != 0:
+            raise Fp8MmError(rc, "selftest_wait_expiry")
+        torch.cuda.synchronize(dev)
+        words = st.tolist()
+        st.zero_()
+        torch.cuda.synchronize(dev)
+    return words
+
+
 def mla_cache_evict(cache, block_table, lens, score, slot_position, budget: int, recent: int, lens_out=None, score_out=None,
                     position_out=None):
     """Shortens every sequence of more than `budget` rows to `budget`, on the current stream; returns lens_out.

@@ -62,6 +62,17 @@ int b200_mla_cache_attend(const b200_mla_cache* cache, const void* q, long long 
                           long long score_stride, float* score_out, long long score_out_stride, int max_len, void* workspace,
                           size_t workspace_bytes, int* device_status, void* stream);
 
+/*
+ * Self-test of the bounded waits (diagnostics): b200_mla_cache_attend with every wait inside the kernel limited to wait_limit_ns (1 ms ..
+ * 100 ms), and with tile `skip_tile` of the first sequence left uncopied (a tile is 48 rows with up to 32 heads, else 64), so the waits
+ * that depend on it run out. The kernel returns by itself; device_status (required) then reads
+ * {B200_FP8_MM_DEV_WAIT_EXPIRED, wait, block, phase}, out is not valid, and the context stays usable. bf16 caches only. Workspace as without scores.
+ */
+int b200_mla_cache_attend_selftest_wait_expiry(const b200_mla_cache* cache, const void* q, long long q_sb, long long q_sh, int heads,
+                                               float scale, void* out, long long out_sb, long long out_sh, void* workspace,
+                                               size_t workspace_bytes, unsigned long long wait_limit_ns, int skip_tile,
+                                               int* device_status, void* stream);
+
 /* Bytes that b200_mla_cache_attend needs (256-byte aligned, no particular contents). */
 size_t b200_mla_cache_attend_workspace_bytes(int batch, int heads, int dv, int dr, int max_len, int with_score);
 

@@ -225,3 +225,19 @@ def test_no_read_only_loads():
     assert "griddepcontrol.wait" in code
     for form in (r"__ldg\s*\(", r"\bld\.global\.nc", r"\bconst\s+[\w:]+\s*\*\s*__restrict__"):
         assert not re.search(form, code), form
+
+
+def test_error_codes_of_the_wait_self_test(built_library):
+    import ctypes
+
+    from amd_developer_challenge_2025_b200 import _lib
+
+    lib, one = _lib.load(), 4096  # never dereferenced
+
+    def call(limit=5000000, skip=1, status=one, ws=None):
+        c = _lib.CMlaCache(one, one, one, 0, 20, PS, DV, D - DV, B, PER, PS * D, D, PER)
+        return lib.b200_mla_cache_attend_selftest_wait_expiry(ctypes.byref(c), one, H * D, D, H, 1.0, one, H * DV, DV, ws, 1 << 30, limit, skip,
+                                                              status, None)
+
+    assert call(status=None) == 1 and call(skip=-1) == 2 and call() == 6
+    assert call(limit=999999) == call(limit=100000001) == call(limit=0) == 7

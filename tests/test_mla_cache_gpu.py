@@ -693,3 +693,17 @@ def test_attend_more_head_tiles_than_sms(heads):
     score = bt.slots()
     out, lse = bt.attend(return_lse=True, score=score, max_len=400)
     check_attend(bt, out, lse, score, bt.slots())
+
+
+@pytest.mark.parametrize("heads", [16, 40, 128])
+@pytest.mark.parametrize("page", [16, 5])
+def test_attend_an_expired_wait_is_reported_and_the_context_stays_usable(heads, page):
+    """In the allowed form: every wait is limited to 5 ms, a tile is not copied, the kernel gives up by itself and says which wait it was.
+    The next ordinary call, which finds shared memory and TMEM as that one left them, is right."""
+    from amd_developer_challenge_2025_b200.mla_cache import selftest_wait_expiry
+
+    check_device_status()
+    words = selftest_wait_expiry("cuda", heads, page)
+    assert words[0] == 1 and 0x201 <= words[1] <= 0x205, [hex(w) for w in words]
+    bt = Batch([300, 0, 1, 2000], heads, page=page, seed=heads)
+    check_attend(bt, *bt.attend(return_lse=True))
