@@ -553,7 +553,6 @@ attend_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   pdl_wait();
-  pdl_launch_dependents();
   // Places before each thread's run of sequences, and where this worker's share begins.
   const int run = (p.batch + kAttendThreads - 1) / kAttendThreads;
   const int b0 = min(p.batch, tid * run), b1 = min(p.batch, b0 + run);
@@ -569,6 +568,9 @@ attend_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__
   tcgen05_fence_before();
   __syncthreads();
   tcgen05_fence_after();
+  // Not before this CTA has its TMEM: a CTA of the next kernel that took some of it first would wait for this one's end, and this one
+  // for its columns.
+  pdl_launch_dependents();
   constexpr uint32_t tmem = 0;  // all columns are this CTA's, so they begin at the first (checked here)
   if (tid == 0 && sh.tmem_base != tmem) sh.expired = 1;
   {

@@ -22,3 +22,11 @@ def test_copies_and_products_come_to_rest_behind_the_last_barrier():
     assert "sh.drained" not in roles.split("mbar_init(smem_u32(&sh.drained), 1);")[1]
     # copies of the rows' own kind end in the role that issued them, which is their only owner
     assert "cp.async.wait_all" in roles
+
+
+def test_the_next_kernel_begins_once_tmem_is_allocated():
+    """Its CTAs may come to the same SM. One that allocates TMEM before this CTA has its own, and then waits for this kernel's end, would
+    never get there."""
+    code = attend_kernel()
+    alloc, go = code.index("tcgen05.alloc"), code.index("pdl_launch_dependents();")
+    assert code.count("pdl_launch_dependents();") == 1 and alloc < go and "__syncthreads();" in code[alloc:go]
