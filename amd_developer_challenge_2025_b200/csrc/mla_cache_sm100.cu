@@ -1729,16 +1729,18 @@ int current_device() {
   return dev;
 }
 
+constexpr int kSmsOfB200 = 148;
+
 // SM count of the current device, looked up once; B200's where there is none (sizes are asked for on hosts without a GPU too).
 int sm_count_for_sizing() {
   static std::atomic<int> known[kMaxDevices];
   const int dev = current_device();
-  if (dev < 0) return 148;
+  if (dev < 0) return kSmsOfB200;
   int n = known[dev].load(std::memory_order_relaxed);
   if (n == 0) {
     if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) {
       (void)cudaGetLastError();
-      return 148;
+      return kSmsOfB200;
     }
     known[dev].store(n, std::memory_order_relaxed);
   }
@@ -2036,7 +2038,8 @@ int b200_mla_cache_evict(const b200_mla_cache* cache, const float* score, long l
   // CTAs per sequence: 4096 slots each where the batch leaves SMs for it. (64 sequences of 2049 slots with 1024 threads: 8.4 us with one
   // CTA each, 10.7 with two. One of 16000: 15.6 us with four, 15.3 with eight, 18.3 with two.)
   p.cluster = 1;
-  while (p.cluster < kMaxCluster && 2 * p.cluster * cache->batch <= 148 && p.cache.capacity > 4096 * p.cluster) p.cluster *= 2;
+  const int sms = sm_count_for_sizing();
+  while (p.cluster < kMaxCluster && 2 * p.cluster * cache->batch <= sms && p.cache.capacity > 4096 * p.cluster) p.cluster *= 2;
   const int slots = ((p.cache.capacity + p.cluster - 1) / p.cluster + 31) / 32 * 32;
   p.staged = slots < kMaxStaged ? slots : kMaxStaged;
   p.few = p.most <= kFewMoves;
@@ -2049,7 +2052,7 @@ int b200_mla_cache_evict(const b200_mla_cache* cache, const float* score, long l
                        static_cast<size_t>(p.staged) * 8, stream, p);
   if (rc != B200_FP8_MM_OK || p.most == 0 || p.few) return rc;
   const int want = (p.most + kMoveThreads / 32 - 1) / (kMoveThreads / 32);
-  const int fill = (148 * 8 + cache->batch - 1) / cache->batch;
+  const int fill = (sms * 8 + cache->batch - 1) / cache->batch;
   const dim3 grid(static_cast<unsigned>(want < fill ? want : fill), static_cast<unsigned>(cache->batch));
   return launch_pdl(evict_move_kernel, grid, kMoveThreads, 0, stream, p);
 }

@@ -241,3 +241,10 @@ def test_error_codes_of_the_wait_self_test(built_library):
 
     assert call(status=None) == 1 and call(skip=-1) == 2 and call() == 6
     assert call(limit=999999) == call(limit=100000001) == call(limit=0) == 7
+
+
+def test_plans_ask_the_device_for_its_sms():
+    """No rule takes a number of SMs as given; where there is no device, sizes are worked out for a B200."""
+    with open(os.path.join(os.path.dirname(pkg.__file__), "csrc", "mla_cache_sm100.cu")) as f:
+        code = re.sub(r"//[^\n]*", "", f.read())
+    assert re.findall(r"[^\n]*\b148\b[^\n]*", code) == ["constexpr int kSmsOfB200 = 148;"]
