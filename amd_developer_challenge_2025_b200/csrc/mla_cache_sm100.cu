@@ -491,7 +491,8 @@ struct Walk {
 // A tile lies in shared memory as [groups of 8 rows][chunk of 64 elements][8 rows x 128 bytes]: one stride from group to group and one
 // from chunk to chunk for both operands, and one copy brings all chunks of as many rows as lie together in a page, up to the tile.
 //
-// What bounds it: up to 32 heads, memory (6.2 TB/s while it runs); 64 heads, how long a tile stays. From its copy's way through memory
+// What bounds it: up to 32 heads, memory (5.4 TB/s over a whole launch of 128 sequences of 4096 rows, beginning and end included, where a
+// copy reaches 6.5); 64 heads, how long a tile stays. From its copy's way through memory
 // (1900 clocks, 39 bytes a clock: what L2 gives when all SMs ask) over the first product (1200), the softmax (1450, with its hand-overs)
 // and the second product (740) to the next copy it takes 5900, and two tiles of 64 rows are all that fits next to Q: 2950 clocks a tile,
 // where the tensor core needs 1900 and, for 128 heads, memory 1600. That is with the next tile fetched to L2 while the ring is full (3400
@@ -507,7 +508,9 @@ struct Walk {
 // the softmax (S comes as 16 x 256-bit fragments, 4 threads to a head) and the epilogue. S is double buffered; the next tile's first
 // product runs under this tile's softmax. The running maximum is replaced only when a logit exceeds it by 8 (in base 2): the weights
 // stay below 2^8 in bf16 and 2^15 in fp16, and rescaling the accumulators is rare. Sums are kept in fp32, weights are rounded to the
-// cache's type for the second product, as matrix operands have to be.
+// cache's type for the second product, as matrix operands have to be: half a step each, as the result's own rounding, so that bf16 outputs
+// are off by 0.0021 of their size instead of 0.0017 (77 rows, in the mean square; 0.0017 both for 65536 rows with 128 heads). A second
+// matrix instruction for what the rounding leaves would double the second product.
 template <typename T, int HT, bool SELFTEST = false>
 __global__ void __launch_bounds__(kAttendThreads, 1)
 attend_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap row_map, const __grid_constant__ AttendParams p) {
@@ -1716,8 +1719,11 @@ constexpr int kMaxHeads = 1 << 16;
 constexpr int kMaxDevices = 64;
 constexpr int kLeastPlaces = 1;
 
-// What beginning and ending a sequence costs a worker, in tiles: its accumulators are read out and written while the tensor core
-// has little to do. 64 heads: 128 KB at the 32 bytes that an SM stores per clock, 5000 clocks against 3400 of a tile.
+// What beginning and ending a sequence costs a worker, in tiles: its accumulators are read out and written while the tensor core has
+// little to do, with 64 heads 128 KB at the 32 bytes that an SM stores per clock. A segment's end takes 9000 clocks there and a tile 2950,
+// but a place more also moves borders in short sequences, and neither is better throughout. With 64 heads to a tile, us with 1, 2 and 3:
+// 64 ragged sequences up to 8192 rows, 128 heads 125.0, 121.0, 118.5; 128 up to 2048 88.8, 87.4, 85.8; 128 up to 400 49.3, 46.3, 47.5; 32
+// up to 4096 50.3, 48.4, 48.1; 7 up to 3001 with 40 heads and dv 256 17.1, 18.1, 18.6.
 int extra_for(int ht) { return ht < 64 ? 1 : 2; }
 
 int current_device() {
